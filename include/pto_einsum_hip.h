@@ -38,7 +38,8 @@ enum pe_status {
     PE_ERR_WORKSPACE = -4    /* workspace missing or too small */
 };
 
-enum pe_dtype { PE_F32 = 0, PE_F16 = 1 };
+/* PE_BF16: the state-space operators and the 4-bit product only. */
+enum pe_dtype { PE_F32 = 0, PE_F16 = 1, PE_BF16 = 2 };
 
 /* Contraction-free product over a row-major float32 output:
  *   out[o] = (add_zero ? 0.0f + a*b : a*b),  a = (float)in0[sum_d o_d*a_stride[d]],
@@ -211,6 +212,93 @@ int64_t pe_reduce_workspace_bytes(const pe_reduce_desc* d);
 /* The (V, L, C) of the summation order above for d and a source at src (V
  * depends on src's 16-byte alignment), into order[0..2]. */
 int pe_reduce_order(const pe_reduce_desc* d, const void* src, int64_t* order);
+
+/* ---- state-space layer: short causal convolution, selective scan ----
+ * No counterpart in the reference.  Sequences are either dense (cu == NULL:
+ * nseq sequences of T tokens, `bs` apart) or packed one after another along
+ * the token axis (cu: nseq + 1 int32 offsets on the device, cu[0] = 0, T the
+ * tokens of the buffer; sequences may be empty; outputs of tokens past
+ * cu[nseq] are zero).  cu and slots are read on the device: offsets are
+ * clamped to the buffer there, and a slot outside [0, nslots) marks a row
+ * without a sequence, whose output is zero and which touches no state.
+ * Strides are in elements; the innermost axis of every tensor is contiguous. */
+
+/* y[t, d] = act(bias[d] + sum_{j < W} weight[d, j] * x[t - W + 1 + j, d]), sums
+ * in float32, rounded once to dtype.  Inputs before a sequence's start come
+ * from its state (the last W - 1 inputs, oldest first; NULL: zeros), and
+ * state_out (may be NULL) receives the last W - 1 inputs at its end.
+ * y [.., D] and the states [nseq][W - 1][D] are contiguous, weight is [D][W]. */
+typedef struct pe_conv_desc {
+    int32_t dtype;                      /* of every tensor */
+    int32_t width;                      /* W, 2..PE_CONV_MAX_WIDTH */
+    int32_t silu;                       /* act: 1 = v / (1 + exp(-v)), 0 = none */
+    int32_t reserved;                   /* must be 0 */
+    int64_t nseq, T, D;
+    int64_t x_bs, x_ts;                 /* sequence and token strides of x */
+    int64_t nslots;                     /* step: rows of the state cache */
+    int64_t x_numel;
+} pe_conv_desc;
+#define PE_CONV_MAX_WIDTH 8
+
+int pe_causal_conv(const pe_conv_desc* d, const void* x, const void* weight, const void* bias,
+                   const void* state_in, const int32_t* cu, void* y, void* state_out, void* stream);
+/* One token of each of nseq sequences (T is not read; x_bs is the row
+ * stride): the state of row b is state[slots[b]] (slots == NULL: b), updated
+ * in place.  Two rows must not share a slot. */
+int pe_causal_conv_step(const pe_conv_desc* d, const void* x, const void* weight, const void* bias,
+                        void* state, const int32_t* slots, void* y, void* stream);
+
+/* Per sequence and head h of H, with group g = h / (H / G) of B and C:
+ *   d_t = dt_t + dt_bias, through log(1 + exp(.)) if softplus is set
+ *   S_t[p, n] = exp(A d_t) S_{t-1}[p, n] + d_t x_t[p] B_t[n]
+ *   y_t[p] = (sum_n C_t[n] S_t[p, n] + D x_t[p]) * (z ? z_t[p] / (1 + exp(-z_t[p])) : 1)
+ * A, D, dt_bias are float32 [H]; states are float32 [P][N] per sequence and
+ * head, contiguous; y is contiguous [..][H][P].  D, z, dt_bias, state_in
+ * (zeros) and state_out may be NULL.  N <= PE_SCAN_MAX_N. */
+typedef struct pe_scan_desc {
+    int32_t dtype;                      /* of x, B, C, z and y */
+    int32_t dt_dtype;                   /* dtype or PE_F32 */
+    int32_t softplus;
+    int32_t reserved;                   /* must be 0 */
+    int64_t nseq, T, H, P, G, N;
+    int64_t x_bs, x_ts, x_hs;           /* sequence, token and head strides */
+    int64_t z_bs, z_ts, z_hs;
+    int64_t dt_bs, dt_ts, dt_hs;
+    int64_t b_bs, b_ts, b_gs;
+    int64_t c_bs, c_ts, c_gs;
+    int64_t nslots;                     /* step: rows of the state cache */
+    int64_t x_numel, z_numel, dt_numel, b_numel, c_numel;
+} pe_scan_desc;
+#define PE_SCAN_MAX_N 256
+
+int64_t pe_selective_scan_workspace_bytes(const pe_scan_desc* d, int packed);
+int pe_selective_scan(const pe_scan_desc* d, const void* x, const void* dt, const float* A, const void* B,
+                      const void* C, const float* D, const void* z, const float* dt_bias,
+                      const float* state_in, const int32_t* cu, void* y, float* state_out,
+                      void* ws, int64_t ws_bytes, void* stream);
+/* One token of each of nseq sequences (token strides and T are not read): the
+ * state of row b is state[slots[b]] (slots == NULL: b), updated in place.  Two
+ * rows must not share a slot. */
+int pe_selective_scan_step(const pe_scan_desc* d, const void* x, const void* dt, const float* A, const void* B,
+                           const void* C, const float* D, const void* z, const float* dt_bias, float* state,
+                           const int32_t* slots, void* y, void* stream);
+
+/* y[m, n] = sum_k x[m, k] * scales[n, k / group] * (q[n, k] - zero), zero =
+ * zeros[n, k / group] or 8, sums in float32, rounded once to dtype.  packed is
+ * [N][ceil(K / 2)] bytes, contiguous, element k in the low half of byte k / 2
+ * if k is even, else the high half; scales and zeros are [N][ceil(K / group)]
+ * of dtype, contiguous; y is [M][N] contiguous.  For few rows of x: the
+ * weights are read once for every 64 of them. */
+typedef struct pe_q4_desc {
+    int32_t dtype;                      /* of x, scales, zeros and y */
+    int32_t group;                      /* 32, 64 or 128 */
+    int64_t M, N, K;
+    int64_t x_ms;                       /* row stride of x */
+    int64_t x_numel;
+} pe_q4_desc;
+
+int pe_matvec_q4(const pe_q4_desc* d, const void* x, const void* packed, const void* scales, const void* zeros,
+                 void* y, void* stream);
 
 /* Plan executor: the body of every per-shape run_einsum_exec.  Every
  * workspace region a plan uses is written before it is read, so a workspace

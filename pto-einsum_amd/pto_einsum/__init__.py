@@ -12,6 +12,11 @@ Beyond the reference's surface:
                                                only (e.g. "ij,jk->k"), which the
                                                reference rejects
     linear_attention(q, k, v, m)            -> fused einsum("tn,sn,sp,ts->tp"), float32
+    causal_conv(x, weight, ...)             -> short causal convolution of each channel, and
+    causal_conv_step(x, weight, state, ...)    the same for one token, its state in place
+    selective_scan(x, dt, A, B, C, ...)     -> state-space scan of prompts, and
+    selective_scan_step(x, ..., state)         the same for one token, its state in place
+    matvec_q4(x, packed, scales, ...)       -> product of few rows with 4-bit weights
     StageGraph(fn)                          -> fn's launches captured into one HIP graph
 
 Example:
@@ -22,6 +27,9 @@ Example:
 from .builder import EinsumBuilder, INCLUDE_DIR, einsum
 from .graph import StageGraph
 from .linattn import linear_attention
+from .quant import matvec_q4
+from .ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 
-__all__ = ["einsum", "EinsumBuilder", "INCLUDE_DIR", "linear_attention", "StageGraph"]
+__all__ = ["einsum", "EinsumBuilder", "INCLUDE_DIR", "linear_attention", "StageGraph", "causal_conv",
+           "causal_conv_step", "selective_scan", "selective_scan_step", "matvec_q4"]
 __version__ = "0.2.0"

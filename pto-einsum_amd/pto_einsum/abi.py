@@ -2,7 +2,7 @@
 
 Lets Python callers (and the component tests) drive the core launchers
 directly: ``pe_product``, ``pe_permute``, ``pe_gemm``, ``pe_linear_attention``,
-``pe_reduce_axes`` and the plan executor.
+``pe_reduce_axes``, the state-space and 4-bit operators and the plan executor.
 """
 from __future__ import annotations
 
@@ -63,6 +63,24 @@ class ReduceDesc(ctypes.Structure):
                 ("reserved", ctypes.c_int32),
                 ("keep_shape", _I64x8), ("keep_stride", _I64x8), ("red_shape", _I64x8), ("red_stride", _I64x8),
                 ("src_numel", ctypes.c_int64)]
+
+
+class ConvDesc(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "width", "silu", "reserved")]
+                + [(f, ctypes.c_int64) for f in ("nseq", "T", "D", "x_bs", "x_ts", "nslots", "x_numel")])
+
+
+class ScanDesc(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "dt_dtype", "softplus", "reserved")]
+                + [(f, ctypes.c_int64) for f in ("nseq", "T", "H", "P", "G", "N", "x_bs", "x_ts", "x_hs",
+                                                 "z_bs", "z_ts", "z_hs", "dt_bs", "dt_ts", "dt_hs",
+                                                 "b_bs", "b_ts", "b_gs", "c_bs", "c_ts", "c_gs", "nslots",
+                                                 "x_numel", "z_numel", "dt_numel", "b_numel", "c_numel")])
+
+
+class Q4Desc(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "group")]
+                + [(f, ctypes.c_int64) for f in ("M", "N", "K", "x_ms", "x_numel")])
 
 
 def _set(arr, values: Sequence[int]):
@@ -145,12 +163,21 @@ def bind(lib=None):
     lib.pe_reduce_workspace_bytes.argtypes = [ctypes.POINTER(ReduceDesc)]
     lib.pe_reduce_workspace_bytes.restype = ctypes.c_int64
     lib.pe_reduce_order.argtypes = [ctypes.POINTER(ReduceDesc), vp, ctypes.POINTER(ctypes.c_int64)]
+    lib.pe_causal_conv.argtypes = [ctypes.POINTER(ConvDesc)] + [vp] * 8
+    lib.pe_causal_conv_step.argtypes = [ctypes.POINTER(ConvDesc)] + [vp] * 7
+    lib.pe_selective_scan.argtypes = [ctypes.POINTER(ScanDesc)] + [vp] * 13 + [ctypes.c_int64, vp]
+    lib.pe_selective_scan_workspace_bytes.argtypes = [ctypes.POINTER(ScanDesc), ctypes.c_int]
+    lib.pe_selective_scan_workspace_bytes.restype = ctypes.c_int64
+    lib.pe_selective_scan_step.argtypes = [ctypes.POINTER(ScanDesc)] + [vp] * 12
+    lib.pe_matvec_q4.argtypes = [ctypes.POINTER(Q4Desc)] + [vp] * 6
     lib.pe_probe_mfma.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int64, vp, ctypes.c_int64, vp]
     lib.pe_probe_mfma_flops.argtypes = [ctypes.c_int, ctypes.c_int64]
     lib.pe_probe_mfma_flops.restype = ctypes.c_int64
     lib.pe_probe_out_len.restype = ctypes.c_int64
     lib.pe_probe_launch.argtypes = [vp, vp]
     for f in ("pe_product", "pe_permute", "pe_gemm", "pe_einsum_exec", "pe_einsum_teardown", "pe_einsum_run", "pe_probe_mfma", "pe_probe_launch", "pe_gemm_choice",
-              "pe_einsum_exec_noalloc", "pe_linear_attention", "pe_reduce_axes", "pe_reduce_order"):
+              "pe_einsum_exec_noalloc", "pe_linear_attention", "pe_reduce_axes", "pe_reduce_order",
+              "pe_causal_conv", "pe_causal_conv_step", "pe_selective_scan", "pe_selective_scan_step",
+              "pe_matvec_q4"):
         getattr(lib, f).restype = ctypes.c_int
     return lib

@@ -30,7 +30,7 @@ from .planner import row_major_strides, split_equation, transpose_config
 ROUTE_PRODUCT = 0
 ROUTE_GEMM = 1
 MAX_DIMS = 8
-DT_F32, DT_F16 = 0, 1
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 
 
 @dataclass
