@@ -1,5 +1,8 @@
-// Entry points of the selective scan: checks, and the choice of kernel.
-#include "pe_scan.h"
+// Entry points of the selective scan: checks, the choice of kernel, and the
+// states at the starts of a sequence's pieces.
+#include "pe_scan_chunk.h"
+
+#include <algorithm>
 
 namespace pe {
 namespace ssm {
@@ -47,6 +50,129 @@ ScanArgs arguments(const pe_scan_desc& d, const void* x, const void* dt, const f
     return g;
 }
 
+// How a prompt is run: token by token (rows), or in chunks.
+struct Plan {
+    bool chunks = false;
+    int nt = 0, waves = 0;
+    int64_t ptiles = 0, piece = 0, per_seq = 0, pieces = 0;
+    int64_t state_floats = 0, decay_floats = 0;   // workspace
+};
+
+Plan plan_of(const pe_scan_desc& d, bool packed) {
+    Plan p;
+    // Up to 16 tokens the recurrence is as quick; rows of less than eight
+    // elements cannot be loaded as whole vectors.
+    if (d.T <= 16 || d.N < 8 || d.P < 8) return p;
+    p.chunks = true;
+    p.nt = d.N <= 32 ? 32 : d.N <= 64 ? 64 : d.N <= 128 ? 128 : 256;
+    p.waves = d.P <= 32 && p.nt < 256 ? 2 : d.P <= 64 ? 4 : 8;
+    p.ptiles = ceil_div(d.P, 16 * p.waves);
+    // Pieces: of as many tokens as leave kBlocks blocks (some four for each CU),
+    // and no more than kMostPieces of a sequence, whose states are joined one
+    // after another.
+    constexpr int64_t kBlocks = 1024, kMostPieces = 96;
+    const int64_t seqs = packed ? 1 : d.nseq, across = d.H * p.ptiles;
+    int64_t piece = 64;
+    const __int128 work = __int128(d.T) * seqs * across;
+    piece = std::max<int64_t>(piece, int64_t(work / kBlocks));
+    piece = std::max(piece, ceil_div(d.T, kMostPieces));
+    if (!packed && d.nseq * across >= kBlocks / 2) piece = d.T;
+    if (!packed) piece = ceil_div(d.T, ceil_div(d.T, piece));
+    p.piece = ceil_div(piece, 64) * 64;
+    p.per_seq = ceil_div(d.T, p.piece);
+    p.pieces = packed ? p.per_seq + d.nseq : p.per_seq * d.nseq;
+    if (packed || p.per_seq > 1) {
+        p.decay_floats = ceil_div(p.pieces * d.H, 4) * 4;
+        p.state_floats = p.pieces * d.H * p.ptiles * p.waves * (p.nt / 16) * 256;
+    }
+    return p;
+}
+
+// From the pieces' contributions to the states at their starts, in place, and
+// the final states.  A thread follows four n of a row p through its sequence;
+// the next kAhead contributions are on their way.
+constexpr int kCarryThreads = 256, kAhead = 8;
+
+__global__ __launch_bounds__(kCarryThreads) void carry_kernel(ChunkArgs g, uint32_t vecs, uint32_t frags, uint32_t wave_rows,
+                                                              uint32_t head_blocks) {
+    const ScanArgs& a = g.s;
+    const uint32_t sh = blockIdx.x / head_blocks, per_head = g.ptiles * vecs;
+    const uint32_t at = (blockIdx.x - sh * head_blocks) * kCarryThreads + threadIdx.x;
+    if (at >= per_head) return;
+    const int s = int(sh / uint32_t(a.H)), h = int(sh - uint32_t(s) * uint32_t(a.H));
+    const uint32_t pt = at / vecs, v = at - pt * vecs, lane = v & 63, frag = v >> 6;
+    const uint32_t wave = frag / frags, i = frag - wave * frags;
+    const int64_t p = int64_t(pt) * 16 * wave_rows + 16 * wave + (lane & 15), n = 16 * i + 4 * (lane >> 4);
+    int64_t id, count;
+    if (a.cu) {
+        const int64_t from = offset_of(a.cu, s, a.T), to = offset_of(a.cu, s + 1, a.T);
+        id = from / g.piece + s;
+        count = to > from ? (to - 1) / g.piece + s - id + 1 : 0;
+    } else {
+        id = int64_t(s) * g.per_seq;
+        count = g.per_seq;
+    }
+    const int64_t state_at = ((int64_t(s) * a.H + h) * a.P + p) * a.N + n;
+    f32x4 S = {0, 0, 0, 0};
+    if (a.state_in && p < a.P) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (n + k < a.N) S[k] = a.state_in[state_at + k];
+    }
+    const int64_t stride = int64_t(a.H) * per_head;
+    f32x4* ws = reinterpret_cast<f32x4*>(g.ws_state) + (id * a.H + h) * per_head + at;
+    const float* decay = g.ws_decay + id * a.H + h;
+    // The last piece's contribution is its own block's.
+    for (int64_t j = 0; j < count; j += kAhead) {
+        f32x4 add[kAhead];
+        float f[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int64_t u = min(j + k, max(count - 2, int64_t(0)));
+            add[k] = ws[u * stride];
+            f[k] = decay[u * a.H];
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (j + k < count) ws[(j + k) * stride] = S;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[e] = __builtin_fmaf(f[k], S[e], add[k][e]);
+        }
+    }
+    if (count == 0 && a.state_out && p < a.P) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (n + k < a.N) a.state_out[state_at + k] = S[k];
+    }
+}
+
+int launch_plan(const pe_scan_desc& d, const Plan& p, const ScanArgs& a, void* ws, hipStream_t stream) {
+    const __int128 blocks = __int128(p.pieces) * d.H * p.ptiles;
+    // Fewer than 2^32 threads in each launch (a head has at least as many pieces
+    // as sequences, and 16 NT WAVES / 4 threads of the carry to 64 WAVES).
+    if ((blocks + kScanTailBlocks) * 64 * p.waves * (p.nt / 16) >= int64_t(1) << 32)
+        return fail(PE_ERR_UNSUPPORTED, "selective_scan: too many rows");
+    ChunkArgs g{};
+    g.s = a;
+    g.piece = uint32_t(p.piece); g.pieces = uint32_t(p.pieces); g.per_seq = uint32_t(p.per_seq);
+    g.ptiles = uint32_t(p.ptiles); g.blocks = uint32_t(blocks);
+    g.state4 = a.N % 4 == 0 && aligned(a.state_in, 16) && aligned(a.state_out, 16);
+    if (p.state_floats) {
+        g.ws_decay = static_cast<float*>(ws);
+        g.ws_state = g.ws_decay + p.decay_floats;
+    }
+    const auto run = d.dtype == PE_F16 ? launch_chunks_f16 : d.dtype == PE_BF16 ? launch_chunks_bf16 : launch_chunks_f32;
+    if (p.state_floats) {
+        run(g, p.nt, p.waves, false, stream);
+        const uint32_t frags = uint32_t(p.nt / 16), vecs = uint32_t(p.waves) * frags * 64;
+        const uint32_t head_blocks = uint32_t(ceil_div(p.ptiles * vecs, kCarryThreads));
+        carry_kernel<<<uint32_t(d.nseq * d.H) * head_blocks, kCarryThreads, 0, stream>>>(g, vecs, frags,
+                                                                                         uint32_t(p.waves), head_blocks);
+    }
+    run(g, p.nt, p.waves, true, stream);
+    return hip_status_of_launch("selective_scan");
+}
+
 }  // namespace
 }  // namespace ssm
 }  // namespace pe
@@ -55,9 +181,9 @@ using namespace pe;
 using namespace pe::ssm;
 
 extern "C" int64_t pe_selective_scan_workspace_bytes(const pe_scan_desc* d, int packed) {
-    (void)d;
-    (void)packed;
-    return 0;
+    if (check(d, false, packed != 0, nullptr) != PE_OK || d->nseq == 0 || d->H == 0 || d->P == 0) return 0;
+    const Plan p = plan_of(*d, packed != 0);
+    return 4 * (p.state_floats + p.decay_floats);
 }
 
 extern "C" int pe_selective_scan(const pe_scan_desc* d, const void* x, const void* dt, const float* A, const void* B,
@@ -69,12 +195,15 @@ extern "C" int pe_selective_scan(const pe_scan_desc* d, const void* x, const voi
     if (d->nseq == 0 || d->H == 0 || d->P == 0) return PE_OK;
     if (!A || (d->T > 0 && (!x || !dt || !y || (d->N > 0 && (!B || !C)))))
         return fail(PE_ERR_INVALID, "selective_scan: null pointer");
-    (void)ws;
-    (void)ws_bytes;
+    const Plan p = plan_of(*d, cu != nullptr);
+    const int64_t need = 4 * (p.state_floats + p.decay_floats);
+    if (need && (!ws || ws_bytes < need || !aligned(ws, 16)))
+        return fail(PE_ERR_WORKSPACE, "selective_scan: workspace missing, misaligned or too small");
     ScanArgs g = arguments(*d, x, dt, A, B, C, D, z, dt_bias);
     g.cu = cu; g.T = d->T; g.y = y; g.state_in = state_in; g.state_out = state_out;
     g.nslots = d->nseq;
-    return launch_rows(d->dtype, g, static_cast<hipStream_t>(stream));
+    auto s = static_cast<hipStream_t>(stream);
+    return p.chunks ? launch_plan(*d, p, g, ws, s) : launch_rows(d->dtype, g, s);
 }
 
 extern "C" int pe_selective_scan_step(const pe_scan_desc* d, const void* x, const void* dt, const float* A,

@@ -1,0 +1,735 @@
+// Selective scan of prompts in chunks of Q tokens on the matrix cores.
+//
+// Within a chunk, with run_t = sum_{r <= t} A d_r from the chunk's start, G = C
+// B^T and S the state at the start,
+//
+//   y_t = exp(run_t) C_t S + sum_{s <= t} G_ts exp(run_t - run_s) d_s x_s
+//   S'  = exp(run_Q) S + sum_s B_s exp(run_Q - run_s) d_s x_s^T
+//
+// so all work but the state's hand-over from chunk to chunk is products.  A
+// block walks a piece of a sequence for one head and 16 WAVES rows p of it.
+// Each wave keeps its 16 columns of S^T [N x 16] in matrix-core accumulators all
+// the way; in an accumulator a lane holds four n of one p, which is an operand
+// fragment of C S^T when the order of n in that product is chosen to match, so S
+// moves through neither LDS nor other lanes.  G^T is computed once a block, a
+// wave per 16 tokens t, weighted in registers (a lane holds one t) and passed
+// through LDS; B and x reach the products over s by transposing LDS reads.
+//
+// With few sequences and heads, sequences are cut into pieces that run at once:
+// a first launch forms each piece's contribution to the state (the second line
+// alone), carry_kernel the states at the pieces' starts, and the main launch
+// the outputs.
+//
+// Rounding: the products take 16-bit operands, so a float32 value enters as a
+// sum of terms, each the 16-bit value nearest to what the earlier ones left:
+//   bfloat16  state's input three bfloat16 terms (2^-24), S and the weighted
+//             scores, which only reach the bfloat16 output, two (2^-16)
+//   float16   two float16 terms (2^-21) of the value times a power of two that
+//             puts a column's (row's) largest at 2^14: float16's range is not
+//             met, and what is lost is below 2^-38 of the largest
+//   float32   three bfloat16 terms of everything, products of terms i + j <= 2
+// Operands of 16 bits enter as they are.  Sums are float32; run_t is summed in 64
+// bits and kept as two float32, since differences of large sums count.
+#pragma once
+
+#include "pe_scan.h"
+
+namespace pe {
+namespace ssm {
+
+struct ChunkArgs {
+    ScanArgs s;
+    float* ws_state;     // [pieces][H][ptiles][columns of 16 p][NT / 16][64 lanes][4], or null: one piece each
+    float* ws_decay;     // [pieces][H]
+    uint32_t piece;      // tokens
+    uint32_t pieces;     // in all
+    uint32_t per_seq;    // dense: of a sequence
+    uint32_t ptiles;
+    uint32_t blocks;     // pieces * H * ptiles
+    int32_t state4;      // rows of the states are whole aligned 16-byte vectors
+};
+
+constexpr int kScanTailBlocks = 64;
+
+// A piece of a sequence: its tokens [t0, t1) and where it stands.
+struct Piece {
+    int64_t t0, t1;
+    int32_t seq;
+    bool first, last;
+};
+
+// Piece `id`.  Packed pieces end at multiples of g.piece of the buffer and at
+// sequences' ends: the one of sequence s in stretch j of the buffer is j + s,
+// which grows from piece to piece.
+__device__ __forceinline__ bool find_piece(const ChunkArgs& g, uint32_t id, Piece& o) {
+    const ScanArgs& a = g.s;
+    if (!a.cu) {
+        o.seq = int32_t(id / g.per_seq);
+        const uint32_t j = id - uint32_t(o.seq) * g.per_seq;
+        o.t0 = int64_t(j) * g.piece;
+        o.t1 = min(a.T, o.t0 + int64_t(g.piece));
+        o.first = j == 0;
+        o.last = j + 1 == g.per_seq;
+        return true;
+    }
+    int32_t lo = 0, hi = a.nseq;
+    while (hi - lo > 1) {
+        const int32_t mid = lo + (hi - lo) / 2;
+        if (uint32_t(offset_of(a.cu, mid, a.T)) / g.piece + uint32_t(mid) <= id) lo = mid;
+        else hi = mid;
+    }
+    const int64_t from = offset_of(a.cu, lo, a.T), to = offset_of(a.cu, lo + 1, a.T);
+    const uint32_t j0 = uint32_t(from) / g.piece, j = id - uint32_t(lo);
+    if (id < uint32_t(lo) || j < j0) return false;
+    o.seq = lo;
+    o.t0 = max(from, int64_t(j) * g.piece);
+    o.t1 = min(to, (int64_t(j) + 1) * g.piece);
+    o.first = j == j0;
+    o.last = to <= (int64_t(j) + 1) * g.piece;
+    return o.t0 < o.t1;
+}
+
+// ------------------------------------------------------- terms and products --
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <typename E>
+struct Scheme {  // BF16
+    using V8 = bf16x8;
+    static constexpr int kIn = 1, kState = 3, kOut = 2;
+    static constexpr bool kScaled = false;
+};
+template <>
+struct Scheme<F16> {
+    using V8 = f16x8;
+    static constexpr int kIn = 1, kState = 2, kOut = 2;
+    static constexpr bool kScaled = true;
+};
+template <>
+struct Scheme<F32> {
+    using V8 = bf16x8;
+    static constexpr int kIn = 3, kState = 3, kOut = 3;
+    static constexpr bool kScaled = false;
+};
+
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// Sum of a_i b_j, the small ones first; of three terms each, those with i + j <= 2.
+template <int NA, int NB, typename V8>
+__device__ __forceinline__ f32x4 mma(const V8 (&a)[NA], const V8 (&b)[NB], f32x4 c) {
+#pragma unroll
+    for (int o = NA + NB - 2; o >= 0; --o) {
+        if (o > 2) continue;
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (o - i >= 0 && o - i < NB) c = mfma(a[i], b[o - i], c);
+    }
+    return c;
+}
+
+// The two 16-bit values nearest to x (float16: toward zero, what is left over is
+// whole in float32 either way), and x less those.
+__device__ __forceinline__ uint32_t take_term(const bf16x8*, f32x2& x) {
+    const uint32_t t = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+    x[0] -= __builtin_bit_cast(float, t << 16);
+    x[1] -= __builtin_bit_cast(float, t & 0xffff0000u);
+    return t;
+}
+__device__ __forceinline__ uint32_t take_term(const f16x8*, f32x2& x) {
+    const f16x2 t = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));
+    x[0] -= (float)t[0];
+    x[1] -= (float)t[1];
+    return __builtin_bit_cast(uint32_t, t);
+}
+
+template <int NT, typename V8>
+__device__ __forceinline__ void split8(const float (&v)[8], V8 (&o)[NT]) {
+    u32x4 w[NT];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f32x2 x = {v[2 * i], v[2 * i + 1]};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) w[t][i] = take_term((const V8*)nullptr, x);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t] = __builtin_bit_cast(V8, w[t]);
+}
+
+__device__ __forceinline__ float elem_f32(f16x8 v, int i) { return (float)v[i]; }
+__device__ __forceinline__ float elem_f32(bf16x8 v, int i) {
+    const u32x4 w = __builtin_bit_cast(u32x4, v);
+    return __builtin_bit_cast(float, (i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+}
+
+// A power of two that takes m > 0 into [2^14, 2^15) (clamped; any for 0, for
+// infinities and NaN), and its inverse.
+__device__ __forceinline__ float scale_for(float m, float& inverse) {
+    int e = int((__float_as_uint(m) >> 23) & 0xff) - 127;
+    e = min(max(e, -100), 100);
+    inverse = __uint_as_float(uint32_t(e - 14 + 127) << 23);
+    return __uint_as_float(uint32_t(14 - e + 127) << 23);
+}
+
+// The largest of the four lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float max_of_groups(float m) {
+    m = fmaxf(m, __shfl_xor(m, 16));
+    return fmaxf(m, __shfl_xor(m, 32));
+}
+
+// Eight 16-bit elements, the first `by` dropped and zeros moved in.
+__device__ __forceinline__ u32x4 shift_out(u32x4 v, int by) {
+    if (by & 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (v[i] >> 16) | (i < 3 ? v[i + 1 < 4 ? i + 1 : 3] << 16 : 0u);
+    if (by & 2) v = u32x4{v[1], v[2], v[3], 0};
+    if (by & 4) v = u32x4{v[2], v[3], 0, 0};
+    return by & 8 ? u32x4{0, 0, 0, 0} : v;
+}
+
+// Eight elements of a row as loaded, and as terms.
+template <typename E>
+struct Raw {
+    u32x4 v;
+    __device__ __forceinline__ void load(const typename E::T* p) {
+        typedef u32x4 uv __attribute__((aligned(2)));
+        v = *reinterpret_cast<const uv*>(p);
+    }
+    __device__ __forceinline__ void drop(int by) { v = shift_out(v, by); }
+    __device__ __forceinline__ void keep_if(bool keep) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = keep ? v[i] : 0u;
+    }
+    __device__ __forceinline__ void terms(u32x4 (&o)[1]) const { o[0] = v; }
+};
+template <>
+struct Raw<F32> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p) {
+        typedef f32x4 uv __attribute__((aligned(4)));
+        const f32x4 a = *reinterpret_cast<const uv*>(p), b = *reinterpret_cast<const uv*>(p + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = a[i];
+            v[i + 4] = b[i];
+        }
+    }
+    __device__ __forceinline__ void drop(int by) {
+#pragma unroll
+        for (int s = 1; s <= 8; s *= 2)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (by & s) ? (i + s < 8 ? v[(i + s) & 7] : 0.0f) : v[i];
+    }
+    __device__ __forceinline__ void keep_if(bool keep) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = keep ? v[i] : 0.0f;
+    }
+    __device__ __forceinline__ void terms(u32x4 (&o)[3]) const {
+        bf16x8 t[3];
+        split8(v, t);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) o[i] = __builtin_bit_cast(u32x4, t[i]);
+    }
+};
+
+// Rows of a chunk on their way to LDS: Q rows of COLS elements over THREADS
+// threads, eight at a time.  Every load is whole and inside its row: a vector
+// that would pass the row's end starts earlier, if need be before `base`, and is
+// moved into place (whole rows hold at least eight elements).
+template <typename E, int Q, int COLS, int THREADS>
+struct Rows {
+    static constexpr int kVecs = Q * COLS / 8, kEach = (kVecs + THREADS - 1) / THREADS, kPitch = COLS + 8;
+    Raw<E> r[kEach];
+    // Rows from token t on, the last at most tokens - 1 past it.
+    __device__ __forceinline__ void load(const typename E::T* base, int64_t ts, int tokens, int width) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int at = threadIdx.x + i * THREADS, row = min(at / (COLS / 8), tokens - 1), c = at % (COLS / 8) * 8;
+            r[i].load(base + row * ts + min(c, width - 8));
+        }
+    }
+    // To kIn planes of [Q][kPitch].
+    __device__ __forceinline__ void store(uint16_t* lds, int tokens, int width) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int at = threadIdx.x + i * THREADS, row = at / (COLS / 8), c = at % (COLS / 8) * 8;
+            if (width < COLS) r[i].drop(min(8, c - min(c, width - 8)));
+            r[i].keep_if(row < tokens);
+            if (kVecs % THREADS == 0 || at < kVecs) {
+                u32x4 t[Scheme<E>::kIn];
+                r[i].terms(t);
+#pragma unroll
+                for (int k = 0; k < Scheme<E>::kIn; ++k)
+                    *reinterpret_cast<u32x4*>(lds + (k * Q + row) * kPitch + c) = t[k];
+            }
+        }
+    }
+};
+
+// Operand fragments of a [rows][PITCH] plane in LDS.
+// Lane l: row l % 16, eight columns from 8 (l / 16).
+template <typename V8>
+__device__ __forceinline__ V8 frag_row(const uint16_t* p) {
+    return *reinterpret_cast<const V8*>(p);
+}
+// Lane l: row l % 16, columns 4 (l / 16) .. + 3 and those 16 further on.
+template <typename V8>
+__device__ __forceinline__ V8 frag_split(const uint16_t* p) {
+    const u32x2 a = *reinterpret_cast<const u32x2*>(p), b = *reinterpret_cast<const u32x2*>(p + 16);
+    return __builtin_bit_cast(V8, u32x4{a[0], a[1], b[0], b[1]});
+}
+// Transposing read: lane 4 j + q of each 16 points at row j, columns 4 q .. + 3;
+// lane i receives column i of the four rows.
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x2 read_tr(const uint16_t* p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) i16x4*)(p)));
+}
+template <typename V8, int PITCH>
+__device__ __forceinline__ V8 frag_tr(const uint16_t* p) {
+    const u32x2 a = read_tr(p), b = read_tr(p + 4 * PITCH);
+    return __builtin_bit_cast(V8, u32x4{a[0], a[1], b[0], b[1]});
+}
+
+// ------------------------------------------------------------------- kernel --
+
+template <typename E, int NT, int Q, int WAVES>
+struct ChunkShape {
+    static constexpr int kPT = 16 * WAVES, kThreads = 64 * WAVES, kIn = Scheme<E>::kIn, kOut = Scheme<E>::kOut;
+    static constexpr int kBP = NT + 8, kXP = kPT + 8, kPP = Q + 8;
+    static constexpr int kTokens = 256;  // whose step sizes are prepared at a time
+    struct Lds {
+        alignas(16) uint16_t b[kIn * Q * kBP], c[kIn * Q * kBP], x[kIn * Q * kXP], p[kOut * Q * kPP];
+        alignas(16) float step[kTokens], hi[kTokens], lo[kTokens], weight[kTokens], fade[kTokens], row[Q];
+        float whole[kTokens / Q];
+    };
+    struct LdsStates {
+        alignas(16) uint16_t b[kIn * Q * kBP], x[kIn * Q * kXP];
+        alignas(16) float weight[kTokens];
+        float whole[kTokens / Q];
+    };
+};
+
+// MAIN: outputs (and the final states); else the pieces' contributions.
+template <typename E, int NT, int Q, int WAVES, bool MAIN>
+__global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
+    using T = typename E::T;
+    using Sch = Scheme<E>;
+    using V8 = typename Sch::V8;
+    using Shape = ChunkShape<E, NT, Q, WAVES>;
+    constexpr int kThreads = Shape::kThreads, kPT = Shape::kPT, kIn = Sch::kIn, kState = Sch::kState, kOut = Sch::kOut;
+    constexpr int kBP = Shape::kBP, kXP = Shape::kXP, kPP = Shape::kPP, kTokens = Shape::kTokens;
+    constexpr int kTT = Q / 16, kNN = NT / 16, kKS = Q / 32, kKN = NT / 32;
+    __shared__ std::conditional_t<MAIN, typename Shape::Lds, typename Shape::LdsStates> m;
+    const ScanArgs& a = g.s;
+
+    if (blockIdx.x >= g.blocks) {  // tokens past the packed sequences
+        const int64_t row = int64_t(a.H) * a.P, from = offset_of(a.cu, a.nseq, a.T) * row, to = a.T * row;
+        for (int64_t i = from + int64_t(blockIdx.x - g.blocks) * kThreads + threadIdx.x; i < to;
+             i += kScanTailBlocks * kThreads)
+            static_cast<T*>(a.y)[i] = T(0.0f);
+        return;
+    }
+    // Blocks go round the eight XCDs in turn; each XCD gets a run of work, whose
+    // heads read the same B and C through its L2.
+    const uint32_t xcd = blockIdx.x & 7, each = g.blocks >> 3, more = g.blocks & 7;
+    const uint32_t job = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
+    const uint32_t ph = job / g.ptiles, pt = job - ph * g.ptiles;
+    const uint32_t id = ph / uint32_t(a.H), h = ph - id * uint32_t(a.H);
+    Piece piece;
+    if (!find_piece(g, id, piece)) return;
+    if (!MAIN && piece.last) return;
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lr = lane & 15, lg = lane >> 4;
+    const int p0 = int(pt) * kPT, width = min(kPT, a.P - p0);  // columns of x
+    const bool active = 16 * wave < width;
+    const int p = p0 + 16 * wave + lr;
+    const int64_t seq = a.cu ? 0 : piece.seq;
+    const int group = int(h) / (a.H / a.G);
+    const T* bb = static_cast<const T*>(a.B) + seq * a.b_bs + piece.t0 * a.b_ts + group * a.b_gs;
+    const T* cb = static_cast<const T*>(a.C) + seq * a.c_bs + piece.t0 * a.c_ts + group * a.c_gs;
+    const T* xb = static_cast<const T*>(a.x) + seq * a.x_bs + piece.t0 * a.x_ts + h * a.x_hs + p0;
+    const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
+    const double A2 = double(A) * 1.4426950408889634;  // exponents are of 2
+    const int64_t dt_at = seq * a.dt_bs + piece.t0 * a.dt_ts + h * a.dt_hs;
+    const int tokens = int(piece.t1 - piece.t0);
+
+    f32x4 S[kNN];  // lane: p = lr; n = 16 i + 4 lg + element
+    float* ws = g.ws_state ? g.ws_state + ((((int64_t(id) * a.H + h) * g.ptiles + pt) * WAVES + wave) * kNN * 64 + lane) * 4
+                           : nullptr;
+    bool have_state = false;
+#pragma unroll
+    for (int i = 0; i < kNN; ++i) S[i] = f32x4{0, 0, 0, 0};
+    const int64_t state_at = ((int64_t(piece.seq) * a.H + h) * a.P + p) * a.N;
+    if (MAIN && (ws || a.state_in)) {
+        have_state = true;
+        if (ws) {
+#pragma unroll
+            for (int i = 0; i < kNN; ++i) S[i] = *reinterpret_cast<const f32x4*>(ws + i * 256);
+        } else if (p < a.P) {
+#pragma unroll
+            for (int i = 0; i < kNN; ++i) {
+                const int n = 16 * i + 4 * lg;
+                if (g.state4) {
+                    if (n < a.N) S[i] = *reinterpret_cast<const f32x4*>(a.state_in + state_at + n);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (n + k < a.N) S[i][k] = a.state_in[state_at + n + k];
+                }
+            }
+        }
+    }
+
+    Rows<E, Q, NT, kThreads> rb;
+    Rows<E, Q, MAIN ? NT : 32, kThreads> rc;
+    Rows<E, Q, kPT, kThreads> rx;
+    auto fetch = [&](int t) {
+        const int left = tokens - t;
+        rb.load(bb + t * a.b_ts, a.b_ts, left, a.N);
+        rx.load(xb + t * a.x_ts, a.x_ts, left, a.P - p0);
+        if constexpr (MAIN) rc.load(cb + t * a.c_ts, a.c_ts, left, a.N);
+    };
+    fetch(0);
+    // Raw step sizes of the next kTokens, a wave 64 of them at a time.
+    constexpr int kParts = kTokens / 64, kOwn = (kParts + WAVES - 1) / WAVES;
+    float raw[kOwn];
+    auto fetch_dt = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            raw[i] = load_dt<E>(a, dt_at + min(t + 64 * (wave + i * WAVES) + lane, tokens - 1) * a.dt_ts);
+    };
+    fetch_dt(0);
+    double sum = 0.0;  // of this piece's exponents
+    const float skip = a.D ? a.D[h] : 0.0f;
+
+    for (int t0 = 0; t0 < tokens; t0 += Q) {
+        const int left = tokens - t0, at = t0 & (kTokens - 1);
+        __syncthreads();
+        rb.store(m.b, left, a.N);
+        rx.store(m.x, left, a.P - p0);
+        if constexpr (MAIN) rc.store(m.c, left, a.N);
+        if (at == 0) {
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                const int part = wave + i * WAVES, tok = 64 * part + lane;
+                if (part < kParts) {
+                    const float d = t0 + tok < tokens ? step_size(a, raw[i], bias) : 0.0f;
+                    // Decays below 2^-4096 are 0 all the same.
+                    double e = A2 * double(d);
+                    e = e < -4096.0 ? -4096.0 : e;
+#pragma unroll
+                    for (int o = 1; o < Q; o *= 2) {
+                        const double v = __shfl_up(e, o);
+                        if ((lane & (Q - 1)) >= o) e += v;
+                    }
+                    const double all = __shfl(e, lane | (Q - 1));
+                    m.weight[tok] = d * __builtin_amdgcn_exp2f(float(all - e));
+                    if constexpr (MAIN) {
+                        const float hi = float(e);
+                        m.step[tok] = d;
+                        m.hi[tok] = hi;
+                        m.lo[tok] = float(e - double(hi));
+                        m.fade[tok] = __builtin_amdgcn_exp2f(hi);
+                        if ((lane & (Q - 1)) == 0) m.whole[tok / Q] = __builtin_amdgcn_exp2f(float(all));
+                    } else {
+                        if ((lane & (Q - 1)) == 0) m.whole[tok / Q] = float(all);
+                    }
+                }
+            }
+            if (t0 + kTokens < tokens) fetch_dt(t0 + kTokens);
+        }
+        // The gate's inputs, in the order of the outputs.
+        T zr[MAIN ? 4 * kTT : 1];
+        if constexpr (MAIN) {
+            if (a.z && active) {
+                const T* zp = static_cast<const T*>(a.z) + seq * a.z_bs + (piece.t0 + t0) * a.z_ts + h * a.z_hs +
+                              min(p, a.P - 1);
+#pragma unroll
+                for (int i = 0; i < 4 * kTT; ++i) zr[i] = zp[min(16 * (i / 4) + 4 * lg + i % 4, left - 1) * a.z_ts];
+            }
+        }
+        if (t0 + Q < tokens) fetch(t0 + Q);
+        __syncthreads();
+
+        // G^T, weighted: P[t][s] = G_ts exp(run_t - run_s) d_s, s <= t.
+        if constexpr (MAIN) {
+#pragma unroll
+            for (int it = 0; it < (kTT + WAVES - 1) / WAVES; ++it) {
+                const int tt = it == 0 ? wave : kTT - 1 - wave;
+                if (tt < kTT) {
+                    const int t = 16 * tt + lr;
+                    f32x4 w[kTT];
+#pragma unroll
+                    for (int s = 0; s < kTT; ++s) w[s] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int kk = 0; kk < kKN; ++kk) {
+                        V8 cf[kIn];
+#pragma unroll
+                        for (int k = 0; k < kIn; ++k) cf[k] = frag_row<V8>(m.c + (k * Q + t) * kBP + 32 * kk + 8 * lg);
+#pragma unroll
+                        for (int s = 0; s < kTT; ++s)
+                            if (s <= tt) {
+                                V8 bf[kIn];
+#pragma unroll
+                                for (int k = 0; k < kIn; ++k)
+                                    bf[k] = frag_row<V8>(m.b + (k * Q + 16 * s + lr) * kBP + 32 * kk + 8 * lg);
+                                w[s] = mma(bf, cf, w[s]);
+                            }
+                    }
+                    const float hi = m.hi[at + t], lo = m.lo[at + t];
+                    float top = 0.0f;
+#pragma unroll
+                    for (int s = 0; s < kTT; ++s)
+                        if (s <= tt) {
+                            const int s0 = 16 * s + 4 * lg;
+                            const f32x4 sh = *reinterpret_cast<const f32x4*>(m.hi + at + s0);
+                            const f32x4 sl = *reinterpret_cast<const f32x4*>(m.lo + at + s0);
+                            const f32x4 sd = *reinterpret_cast<const f32x4*>(m.step + at + s0);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float e = __builtin_amdgcn_exp2f((hi - sh[i]) + (lo - sl[i]));
+                                w[s][i] = s0 + i <= t ? w[s][i] * (e * sd[i]) : 0.0f;
+                                if constexpr (Sch::kScaled) top = fmaxf(top, fabsf(w[s][i]));
+                            }
+                        }
+                    float factor = 1.0f;
+                    if constexpr (Sch::kScaled) {
+                        float inverse;
+                        factor = scale_for(max_of_groups(top), inverse);
+                        if (lg == 0) m.row[t] = inverse;
+                    }
+#pragma unroll
+                    for (int s = 0; s < kTT; ++s)
+                        if (s <= (tt | 1)) {
+                            f32x2 u = {w[s][0] * factor, w[s][1] * factor}, v = {w[s][2] * factor, w[s][3] * factor};
+#pragma unroll
+                            for (int k = 0; k < kOut; ++k)
+                                *reinterpret_cast<u32x2*>(m.p + (k * Q + t) * kPP + 16 * s + 4 * lg) =
+                                    u32x2{take_term((const V8*)nullptr, u), take_term((const V8*)nullptr, v)};
+                        }
+                }
+            }
+        }
+
+        V8 xf[kKS][kIn];  // x^T: lane p, eight s
+        int bad = Q;      // the first token whose x is not finite
+        f32x4 y[MAIN ? kTT : 1];
+        if (active) {
+#pragma unroll
+            for (int ks = 0; ks < kKS; ++ks)
+#pragma unroll
+                for (int k = 0; k < kIn; ++k)
+                    xf[ks][k] = frag_tr<V8, kXP>(m.x + (k * Q + 32 * ks + 8 * lg + (lr >> 2)) * kXP + 16 * wave +
+                                                 4 * (lr & 3));
+            if constexpr (MAIN) {
+                // exp(run_t) C S
+#pragma unroll
+                for (int tt = 0; tt < kTT; ++tt) y[tt] = f32x4{0, 0, 0, 0};
+                if (have_state) {
+                    float factor = 1.0f, inverse = 1.0f;
+                    if constexpr (Sch::kScaled) {
+                        float top = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < kNN; ++i)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) top = fmaxf(top, fabsf(S[i][k]));
+                        factor = scale_for(max_of_groups(top), inverse);
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < kKN; ++kk) {
+                        float v[8];
+                        V8 sf[kOut];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            v[i] = S[2 * kk + i / 4][i % 4];
+                            if constexpr (Sch::kScaled) v[i] *= factor;
+                        }
+                        split8(v, sf);
+#pragma unroll
+                        for (int tt = 0; tt < kTT; ++tt) {
+                            V8 cf[kIn];
+#pragma unroll
+                            for (int k = 0; k < kIn; ++k)
+                                cf[k] = frag_split<V8>(m.c + (k * Q + 16 * tt + lr) * kBP + 32 * kk + 4 * lg);
+                            y[tt] = mma(cf, sf, y[tt]);
+                        }
+                    }
+#pragma unroll
+                    for (int tt = 0; tt < kTT; ++tt) {
+                        const f32x4 f = *reinterpret_cast<const f32x4*>(m.fade + at + 16 * tt + 4 * lg);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[tt][i] *= Sch::kScaled ? f[i] * inverse : f[i];
+                    }
+                }
+            }
+            // S' = exp(run_Q) S + B^T (w x)
+            float whole = m.whole[at / Q];
+            if constexpr (!MAIN) {
+                sum += double(whole);
+                whole = __builtin_amdgcn_exp2f(whole);
+            }
+            V8 wx[kKS][kState];
+            float wv[kKS][8], top = 0.0f, factor = 1.0f, inverse = 1.0f;
+#pragma unroll
+            for (int ks = 0; ks < kKS; ++ks)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float v = elem_f32(xf[ks][0], i);
+#pragma unroll
+                    for (int k = 1; k < kIn; ++k) v += elem_f32(xf[ks][k], i);
+                    wv[ks][i] = v * m.weight[at + 32 * ks + 8 * lg + i];
+                    if constexpr (Sch::kScaled) top = fmaxf(top, fabsf(wv[ks][i]));
+                }
+            if constexpr (Sch::kScaled) factor = scale_for(max_of_groups(top), inverse);
+#pragma unroll
+            for (int ks = 0; ks < kKS; ++ks) {
+                if constexpr (Sch::kScaled)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) wv[ks][i] *= factor;
+                split8(wv[ks], wx[ks]);
+            }
+#pragma unroll
+            for (int i = 0; i < kNN; ++i) {
+                f32x4 d = f32x4{0, 0, 0, 0};
+                if constexpr (!Sch::kScaled)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) d[k] = S[i][k] * whole;
+#pragma unroll
+                for (int ks = 0; ks < kKS; ++ks) {
+                    V8 bf[kIn];
+#pragma unroll
+                    for (int k = 0; k < kIn; ++k)
+                        bf[k] = frag_tr<V8, kBP>(m.b + (k * Q + 32 * ks + 8 * lg + (lr >> 2)) * kBP + 16 * i +
+                                                 4 * (lr & 3));
+                    d = mma(bf, wx[ks], d);
+                }
+                if constexpr (Sch::kScaled) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) S[i][k] = __builtin_fmaf(d[k], inverse, S[i][k] * whole);
+                } else {
+                    S[i] = d;
+                }
+            }
+            have_state = true;
+            if constexpr (MAIN) {
+                // Tokens before one whose x is an infinity or NaN must not see
+                // it times their weight of 0: it is taken out and put back below.
+                bool some = false;
+#pragma unroll
+                for (int ks = 0; ks < kKS; ++ks)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        some |= !(fabsf(elem_f32(xf[ks][0], i)) <= 3.4028235e38f);
+                if (__any(some)) {
+#pragma unroll
+                    for (int ks = 0; ks < kKS; ++ks)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (!(fabsf(elem_f32(xf[ks][0], i)) <= 3.4028235e38f)) {
+                                bad = min(bad, 32 * ks + 8 * lg + i);
+#pragma unroll
+                                for (int k = 0; k < kIn; ++k) xf[ks][k][i] = {};
+                            }
+                    bad = min(bad, __shfl_xor(bad, 16));
+                    bad = min(bad, __shfl_xor(bad, 32));
+                }
+            }
+        }
+        if constexpr (MAIN) {
+            __syncthreads();
+            if (active) {
+                T* yp = static_cast<T*>(a.y) + ((a.cu ? 0 : int64_t(piece.seq) * a.T) + piece.t0 + t0) * a.H * a.P +
+                        int64_t(h) * a.P + p;
+#pragma unroll
+                for (int tt = 0; tt < kTT; ++tt) {
+                    f32x4 d = Sch::kScaled ? f32x4{0, 0, 0, 0} : y[tt];
+#pragma unroll
+                    for (int ks = 0; ks <= tt / 2; ++ks) {
+                        V8 pf[kOut];
+#pragma unroll
+                        for (int k = 0; k < kOut; ++k)
+                            pf[k] = frag_row<V8>(m.p + (k * Q + 16 * tt + lr) * kPP + 32 * ks + 8 * lg);
+                        d = mma(pf, xf[ks], d);
+                    }
+                    if constexpr (Sch::kScaled) {
+                        const f32x4 r = *reinterpret_cast<const f32x4*>(m.row + 16 * tt + 4 * lg);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) d[i] = __builtin_fmaf(d[i], r[i], y[tt][i]);
+                    }
+                    // x of the outputs' tokens, for the skip
+                    float xv[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < kIn; ++k) {
+                        const u32x2 v = read_tr(m.x + (k * Q + 16 * tt + 4 * lg + (lr >> 2)) * kXP + 16 * wave +
+                                                4 * (lr & 3));
+                        const V8 v8 = __builtin_bit_cast(V8, u32x4{v[0], v[1], 0, 0});
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) xv[i] += elem_f32(v8, i);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int t = 16 * tt + 4 * lg + i;
+                        float v = __builtin_fmaf(skip, xv[i], d[i]);
+                        if (t >= bad) v = __builtin_nanf("");
+                        if (a.z) v *= silu(E::to_f32(zr[4 * tt + i]));
+                        if (t < left && p < a.P) yp[t * int64_t(a.H) * a.P] = T(v);
+                    }
+                }
+            }
+        }
+    }
+
+    if (!active) return;
+    if constexpr (!MAIN) {
+#pragma unroll
+        for (int i = 0; i < kNN; ++i) *reinterpret_cast<f32x4*>(ws + i * 256) = S[i];
+        if (pt == 0 && threadIdx.x == 0) g.ws_decay[int64_t(id) * a.H + h] = __builtin_amdgcn_exp2f(float(sum));
+    } else if (piece.last && a.state_out && p < a.P) {
+#pragma unroll
+        for (int i = 0; i < kNN; ++i) {
+            const int n = 16 * i + 4 * lg;
+            if (g.state4) {
+                if (n < a.N) *reinterpret_cast<f32x4*>(a.state_out + state_at + n) = S[i];
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (n + k < a.N) a.state_out[state_at + n + k] = S[i][k];
+            }
+        }
+    }
+}
+
+// The kernels of one element type; `main` 0 the contributions, 1 the outputs.
+void launch_chunks_f16(const ChunkArgs& g, int nt, int waves, bool main, hipStream_t stream);
+void launch_chunks_bf16(const ChunkArgs& g, int nt, int waves, bool main, hipStream_t stream);
+void launch_chunks_f32(const ChunkArgs& g, int nt, int waves, bool main, hipStream_t stream);
+
+template <typename E, int NT, int Q, int WAVES>
+void launch_chunks(const ChunkArgs& g, bool main, hipStream_t stream) {
+    if (main) {
+        const uint32_t blocks = g.blocks + (g.s.cu ? kScanTailBlocks : 0);
+        chunk_kernel<E, NT, Q, WAVES, true><<<blocks, 64 * WAVES, 0, stream>>>(g);
+    } else {
+        chunk_kernel<E, NT, Q, WAVES, false><<<g.blocks, 64 * WAVES, 0, stream>>>(g);
+    }
+}
+
+template <typename E, int NT, int Q>
+void launch_chunks(const ChunkArgs& g, int waves, bool main, hipStream_t stream) {
+    if constexpr (NT < 256) {
+        if (waves == 2) return launch_chunks<E, NT, Q, 2>(g, main, stream);
+    }
+    if (waves == 8) return launch_chunks<E, NT, Q, 8>(g, main, stream);
+    launch_chunks<E, NT, Q, 4>(g, main, stream);
+}
+
+}  // namespace ssm
+}  // namespace pe
