@@ -207,6 +207,7 @@ struct Raw {
         for (int i = 0; i < 4; ++i) v[i] = keep ? v[i] : 0u;
     }
     __device__ __forceinline__ void terms(u32x4 (&o)[1]) const { o[0] = v; }
+    __device__ __forceinline__ void put(typename E::T* p) const { *reinterpret_cast<u32x4*>(p) = v; }
 };
 template <>
 struct Raw<F32> {
@@ -230,6 +231,10 @@ struct Raw<F32> {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = keep ? v[i] : 0.0f;
     }
+    __device__ __forceinline__ void put(float* p) const {
+        *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    }
     __device__ __forceinline__ void terms(u32x4 (&o)[3]) const {
         bf16x8 t[3];
         split8(v, t);
@@ -252,6 +257,16 @@ struct Rows {
         for (int i = 0; i < kEach; ++i) {
             const int at = threadIdx.x + i * THREADS, row = min(at / (COLS / 8), tokens - 1), c = at % (COLS / 8) * 8;
             r[i].load(base + row * ts + min(c, width - 8));
+        }
+    }
+    // As they are, to [Q][PITCH] of T.
+    template <int PITCH>
+    __device__ __forceinline__ void store_raw(typename E::T* lds, int width) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int at = threadIdx.x + i * THREADS, row = at / (COLS / 8), c = at % (COLS / 8) * 8;
+            if (width < COLS) r[i].drop(min(8, c - min(c, width - 8)));
+            if (kVecs % THREADS == 0 || at < kVecs) r[i].put(lds + row * PITCH + c);
         }
     }
     // To kIn planes of [Q][kPitch].
@@ -302,12 +317,13 @@ __device__ __forceinline__ V8 frag_tr(const uint16_t* p) {
 template <typename E, int NT, int Q, int WAVES>
 struct ChunkShape {
     static constexpr int kPT = 16 * WAVES, kThreads = 64 * WAVES, kIn = Scheme<E>::kIn, kOut = Scheme<E>::kOut;
-    static constexpr int kBP = NT + 8, kXP = kPT + 8, kPP = Q + 8;
+    static constexpr int kBP = NT + 8, kXP = kPT + 8, kPP = Q + 8, kZP = kPT + 16 / E::kBytes;
     static constexpr int kTokens = 256;  // whose step sizes are prepared at a time
     struct Lds {
         alignas(16) uint16_t b[kIn * Q * kBP], c[kIn * Q * kBP], x[kIn * Q * kXP], p[kOut * Q * kPP];
         alignas(16) float step[kTokens], hi[kTokens], lo[kTokens], weight[kTokens], fade[kTokens], row[Q];
         float whole[kTokens / Q];
+        alignas(16) typename E::T z[Q * kZP];  // the gate's inputs, then the outputs
     };
     struct LdsStates {
         alignas(16) uint16_t b[kIn * Q * kBP], x[kIn * Q * kXP];
@@ -324,7 +340,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
     using V8 = typename Sch::V8;
     using Shape = ChunkShape<E, NT, Q, WAVES>;
     constexpr int kThreads = Shape::kThreads, kPT = Shape::kPT, kIn = Sch::kIn, kState = Sch::kState, kOut = Sch::kOut;
-    constexpr int kBP = Shape::kBP, kXP = Shape::kXP, kPP = Shape::kPP, kTokens = Shape::kTokens;
+    constexpr int kBP = Shape::kBP, kXP = Shape::kXP, kPP = Shape::kPP, kZP = Shape::kZP, kTokens = Shape::kTokens;
     constexpr int kTT = Q / 16, kNN = NT / 16, kKS = Q / 32, kKN = NT / 32;
     __shared__ std::conditional_t<MAIN, typename Shape::Lds, typename Shape::LdsStates> m;
     const ScanArgs& a = g.s;
@@ -356,6 +372,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
     const T* bb = static_cast<const T*>(a.B) + seq * a.b_bs + piece.t0 * a.b_ts + group * a.b_gs;
     const T* cb = static_cast<const T*>(a.C) + seq * a.c_bs + piece.t0 * a.c_ts + group * a.c_gs;
     const T* xb = static_cast<const T*>(a.x) + seq * a.x_bs + piece.t0 * a.x_ts + h * a.x_hs + p0;
+    const T* zb = static_cast<const T*>(a.z) + seq * a.z_bs + piece.t0 * a.z_ts + h * a.z_hs + p0;
     const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
     const double A2 = double(A) * 1.4426950408889634;  // exponents are of 2
     const int64_t dt_at = seq * a.dt_bs + piece.t0 * a.dt_ts + h * a.dt_hs;
@@ -367,6 +384,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
     bool have_state = false;
 #pragma unroll
     for (int i = 0; i < kNN; ++i) S[i] = f32x4{0, 0, 0, 0};
+    const int64_t ys = int64_t(a.H) * a.P;  // token stride of y
     const int64_t state_at = ((int64_t(piece.seq) * a.H + h) * a.P + p) * a.N;
     if (MAIN && (ws || a.state_in)) {
         have_state = true;
@@ -390,12 +408,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
 
     Rows<E, Q, NT, kThreads> rb;
     Rows<E, Q, MAIN ? NT : 32, kThreads> rc;
-    Rows<E, Q, kPT, kThreads> rx;
+    Rows<E, Q, kPT, kThreads> rx, rz;
+    const bool gated = MAIN && a.z;
     auto fetch = [&](int t) {
         const int left = tokens - t;
         rb.load(bb + t * a.b_ts, a.b_ts, left, a.N);
         rx.load(xb + t * a.x_ts, a.x_ts, left, a.P - p0);
-        if constexpr (MAIN) rc.load(cb + t * a.c_ts, a.c_ts, left, a.N);
+        if constexpr (MAIN) {
+            rc.load(cb + t * a.c_ts, a.c_ts, left, a.N);
+            if (gated) rz.load(zb + t * a.z_ts, a.z_ts, left, a.P - p0);
+        }
     };
     fetch(0);
     // Raw step sizes of the next kTokens, a wave 64 of them at a time.
@@ -415,7 +437,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
         __syncthreads();
         rb.store(m.b, left, a.N);
         rx.store(m.x, left, a.P - p0);
-        if constexpr (MAIN) rc.store(m.c, left, a.N);
+        if constexpr (MAIN) {
+            rc.store(m.c, left, a.N);
+            if (gated) rz.template store_raw<kZP>(m.z, a.P - p0);
+        }
         if (at == 0) {
 #pragma unroll
             for (int i = 0; i < kOwn; ++i) {
@@ -446,19 +471,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
             }
             if (t0 + kTokens < tokens) fetch_dt(t0 + kTokens);
         }
-        // The gate's inputs, in the order of the outputs.
-        T zr[MAIN ? 4 * kTT : 1];
-        if constexpr (MAIN) {
-            if (a.z && active) {
-                const T* zp = static_cast<const T*>(a.z) + seq * a.z_bs + (piece.t0 + t0) * a.z_ts + h * a.z_hs +
-                              min(p, a.P - 1);
-#pragma unroll
-                for (int i = 0; i < 4 * kTT; ++i) zr[i] = zp[min(16 * (i / 4) + 4 * lg + i % 4, left - 1) * a.z_ts];
-            }
-        }
         if (t0 + Q < tokens) fetch(t0 + Q);
         __syncthreads();
 
+        __builtin_amdgcn_sched_barrier(0);
         // G^T, weighted: P[t][s] = G_ts exp(run_t - run_s) d_s, s <= t.
         if constexpr (MAIN) {
 #pragma unroll
@@ -519,6 +535,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
             }
         }
 
+        __builtin_amdgcn_sched_barrier(0);
         V8 xf[kKS][kIn];  // x^T: lane p, eight s
         int bad = Q;      // the first token whose x is not finite
         f32x4 y[MAIN ? kTT : 1];
@@ -570,6 +587,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
                     }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
             // S' = exp(run_Q) S + B^T (w x)
             float whole = m.whole[at / Q];
             if constexpr (!MAIN) {
@@ -646,8 +664,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
         if constexpr (MAIN) {
             __syncthreads();
             if (active) {
-                T* yp = static_cast<T*>(a.y) + ((a.cu ? 0 : int64_t(piece.seq) * a.T) + piece.t0 + t0) * a.H * a.P +
-                        int64_t(h) * a.P + p;
 #pragma unroll
                 for (int tt = 0; tt < kTT; ++tt) {
                     f32x4 d = Sch::kScaled ? f32x4{0, 0, 0, 0} : y[tt];
@@ -674,13 +690,44 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) xv[i] += elem_f32(v8, i);
                     }
+                    float zv[4];
+                    T* zt = m.z + (16 * tt + 4 * lg) * kZP + 16 * wave + lr;
+                    if constexpr (E::kBytes == 2) {
+                        const u32x2 v = read_tr(reinterpret_cast<const uint16_t*>(m.z) +
+                                                (16 * tt + 4 * lg + (lr >> 2)) * kZP + 16 * wave + 4 * (lr & 3));
+                        const V8 v8 = __builtin_bit_cast(V8, u32x4{v[0], v[1], 0, 0});
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) zv[i] = elem_f32(v8, i);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) zv[i] = E::to_f32(zt[i * kZP]);
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int t = 16 * tt + 4 * lg + i;
                         float v = __builtin_fmaf(skip, xv[i], d[i]);
-                        if (t >= bad) v = __builtin_nanf("");
-                        if (a.z) v *= silu(E::to_f32(zr[4 * tt + i]));
-                        if (t < left && p < a.P) yp[t * int64_t(a.H) * a.P] = T(v);
+                        if (16 * tt + 4 * lg + i >= bad) v = __builtin_nanf("");
+                        if (gated) v *= silu(zv[i]);
+                        zt[i * kZP] = T(v);
+                    }
+                }
+                // The wave's columns of y, 16 bytes a lane.
+                constexpr int kV = 16 / E::kBytes, kL = 16 / kV, kR = 64 / kL;
+                const int pc = 16 * wave + kV * (lane % kL), have = width - pc;
+                T* yp = static_cast<T*>(a.y) + ((a.cu ? 0 : int64_t(piece.seq) * a.T) + piece.t0 + t0 + lane / kL) * ys +
+                        int64_t(h) * a.P + p0 + pc;
+#pragma unroll
+                for (int i = 0; i < Q / kR; ++i) {
+                    const int t = lane / kL + i * kR;
+                    const T* from = m.z + t * kZP + pc;
+                    if (t < left) {
+                        if (have >= kV) {
+                            *reinterpret_cast<typename Vec<E, kV>::utype*>(yp + i * kR * ys) =
+                                *reinterpret_cast<const typename Vec<E, kV>::type*>(from);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < kV; ++k)
+                                if (k < have) yp[i * kR * ys + k] = from[k];
+                        }
                     }
                 }
             }

@@ -55,8 +55,13 @@ __device__ __forceinline__ void store_f32(typename E::T* p, int n, const float (
     }
 }
 
-// v / (1 + exp(-v)); -0 for v far below 0, where exp(-v) is infinite.
-__device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
+// v / (1 + exp(-v)); -0 for v far below 0, where exp(-v) is infinite.  Through
+// the hardware's 2^x and reciprocal, good to a unit each (the exponent's own
+// rounding counts where the result is small): the library's exp and divide made
+// the convolution of a large prompt compute longer than its memory takes.
+__device__ __forceinline__ float silu(float v) {
+    return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * v));
+}
 
 // log(1 + exp(v)) without overflow; exp(-|v|) below 2^-24 leaves max(v, 0).
 __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))); }
