@@ -3,6 +3,7 @@
 #include "pe_scan_chunk.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace pe {
 namespace ssm {
@@ -58,27 +59,40 @@ struct Plan {
     int64_t state_floats = 0, decay_floats = 0;   // workspace
 };
 
+auto chunks_of(int dtype) { return dtype == PE_F16 ? chunks_f16 : dtype == PE_BF16 ? chunks_bf16 : chunks_f32; }
+
 Plan plan_of(const pe_scan_desc& d, bool packed) {
     Plan p;
     // Up to 16 tokens the recurrence is as quick; rows of less than eight
     // elements cannot be loaded as whole vectors.
     if (d.T <= 16 || d.N < 8 || d.P < 8) return p;
+    // Offsets within a chunk are 32 bits.
+    constexpr int64_t kMostStride = int64_t(1) << 24;
+    for (const int64_t ts : {d.x_ts, d.z_ts, d.b_ts, d.c_ts, d.H * d.P})
+        if (ts >= kMostStride) return p;
     p.chunks = true;
     p.nt = d.N <= 32 ? 32 : d.N <= 64 ? 64 : d.N <= 128 ? 128 : 256;
-    p.waves = d.P <= 32 && p.nt < 256 ? 2 : d.P <= 64 ? 4 : 8;
-    p.ptiles = ceil_div(d.P, 16 * p.waves);
-    // Pieces: of as many tokens as leave kBlocks blocks (some four for each CU),
-    // and no more than kMostPieces of a sequence, whose states are joined one
-    // after another.
-    constexpr int64_t kBlocks = 1024, kMostPieces = 96;
-    const int64_t seqs = packed ? 1 : d.nseq, across = d.H * p.ptiles;
-    int64_t piece = 64;
-    const __int128 work = __int128(d.T) * seqs * across;
-    piece = std::max<int64_t>(piece, int64_t(work / kBlocks));
-    piece = std::max(piece, ceil_div(d.T, kMostPieces));
-    if (!packed && d.nseq * across >= kBlocks / 2) piece = d.T;
-    if (!packed) piece = ceil_div(d.T, ceil_div(d.T, piece));
-    p.piece = ceil_div(piece, 64) * 64;
+    // Tiles of up to 64 rows p, as even as waves of 16 allow.
+    p.ptiles = ceil_div(d.P, 64);
+    p.waves = int(std::max<int64_t>(p.nt == 256 ? 3 : 2, ceil_div(ceil_div(d.P, 16), p.ptiles)));
+    // Pieces of a sequence (packed: of the whole buffer).  What a choice costs, in
+    // chunks of 32 tokens that a block walks: those of a piece and one for its
+    // start, in as many rounds as the blocks need; half of that again for the
+    // pieces' contributions, and 6 for the states of 1000 blocks of 64 x 128.
+    const int64_t seqs = packed ? 1 : d.nseq, across = d.H * p.ptiles, chunks = ceil_div(d.T, 32);
+    const double slots = 256.0 * chunks_of(d.dtype)(nullptr, p.nt, p.waves, true, nullptr);
+    double best = 0.0;
+    for (int64_t k = 1; k <= std::min<int64_t>(chunks, 96); ++k) {
+        const int64_t piece = ceil_div(chunks, k);
+        if (k > 1 && ceil_div(chunks, k - 1) == piece) continue;
+        const double blocks = double(seqs) * double(across) * double(ceil_div(chunks, piece));
+        double cost = std::ceil(blocks / slots) * double(piece + 1);
+        if (k > 1) cost = 1.5 * cost + 0.006 * blocks * (p.waves * p.nt / 512.0);
+        if (k == 1 || cost < best) {
+            best = cost;
+            p.piece = 32 * piece;
+        }
+    }
     p.per_seq = ceil_div(d.T, p.piece);
     p.pieces = packed ? p.per_seq + d.nseq : p.per_seq * d.nseq;
     if (packed || p.per_seq > 1) {
@@ -161,15 +175,15 @@ int launch_plan(const pe_scan_desc& d, const Plan& p, const ScanArgs& a, void* w
         g.ws_decay = static_cast<float*>(ws);
         g.ws_state = g.ws_decay + p.decay_floats;
     }
-    const auto run = d.dtype == PE_F16 ? launch_chunks_f16 : d.dtype == PE_BF16 ? launch_chunks_bf16 : launch_chunks_f32;
+    const auto run = chunks_of(d.dtype);
     if (p.state_floats) {
-        run(g, p.nt, p.waves, false, stream);
+        run(&g, p.nt, p.waves, false, stream);
         const uint32_t frags = uint32_t(p.nt / 16), vecs = uint32_t(p.waves) * frags * 64;
         const uint32_t head_blocks = uint32_t(ceil_div(p.ptiles * vecs, kCarryThreads));
         carry_kernel<<<uint32_t(d.nseq * d.H) * head_blocks, kCarryThreads, 0, stream>>>(g, vecs, frags,
                                                                                          uint32_t(p.waves), head_blocks);
     }
-    run(g, p.nt, p.waves, true, stream);
+    run(&g, p.nt, p.waves, true, stream);
     return hip_status_of_launch("selective_scan");
 }
 

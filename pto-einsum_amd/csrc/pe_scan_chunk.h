@@ -34,6 +34,8 @@
 
 #include "pe_scan.h"
 
+#include <algorithm>
+
 namespace pe {
 namespace ssm {
 
@@ -144,9 +146,12 @@ __device__ __forceinline__ uint32_t take_term(const bf16x8*, f32x2& x) {
 }
 __device__ __forceinline__ uint32_t take_term(const f16x8*, f32x2& x) {
     const f16x2 t = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));
-    x[0] -= (float)t[0];
-    x[1] -= (float)t[1];
-    return __builtin_bit_cast(uint32_t, t);
+    // x - t in one instruction each, t a half of a register (from a conversion and
+    // a difference the compiler does not form it).
+    const uint32_t u = __builtin_bit_cast(uint32_t, t);
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(x[0]) : "v"(u), "v"(x[0]));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(x[1]) : "v"(u), "v"(x[1]));
+    return u;
 }
 
 template <int NT, typename V8>
@@ -168,6 +173,21 @@ __device__ __forceinline__ float elem_f32(bf16x8 v, int i) {
     return __builtin_bit_cast(float, (i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
 }
 
+// Nonzero if an element is an infinity or NaN: the exponent of each half of a
+// word plus 1 reaches the half's top bit just when it was all ones.
+__device__ __forceinline__ uint32_t not_finite(u32x4 w, uint32_t exponent, uint32_t one) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r |= (w[i] & exponent) + one;
+    return r & 0x80008000u;
+}
+__device__ __forceinline__ uint32_t not_finite(f16x8 v) {
+    return not_finite(__builtin_bit_cast(u32x4, v), 0x7c007c00u, 0x04000400u);
+}
+__device__ __forceinline__ uint32_t not_finite(bf16x8 v) {
+    return not_finite(__builtin_bit_cast(u32x4, v), 0x7f807f80u, 0x00800080u);
+}
+
 // A power of two that takes m > 0 into [2^14, 2^15) (clamped; any for 0, for
 // infinities and NaN), and its inverse.
 __device__ __forceinline__ float scale_for(float m, float& inverse) {
@@ -181,6 +201,14 @@ __device__ __forceinline__ float scale_for(float m, float& inverse) {
 __device__ __forceinline__ float max_of_groups(float m) {
     m = fmaxf(m, __shfl_xor(m, 16));
     return fmaxf(m, __shfl_xor(m, 32));
+}
+
+// x, which the compiler takes for another value: what is formed from it inside a
+// loop is not kept in registers across it (some 40 LDS
+// addresses and 40 lane masks otherwise).
+__device__ __forceinline__ int fresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 // Eight 16-bit elements, the first `by` dropped and zeros moved in.
@@ -197,7 +225,7 @@ __device__ __forceinline__ u32x4 shift_out(u32x4 v, int by) {
 template <typename E>
 struct Raw {
     u32x4 v;
-    __device__ __forceinline__ void load(const typename E::T* p) {
+    __device__ __forceinline__ void load(const char* p) {
         typedef u32x4 uv __attribute__((aligned(2)));
         v = *reinterpret_cast<const uv*>(p);
     }
@@ -212,9 +240,9 @@ struct Raw {
 template <>
 struct Raw<F32> {
     float v[8];
-    __device__ __forceinline__ void load(const float* p) {
+    __device__ __forceinline__ void load(const char* p) {
         typedef f32x4 uv __attribute__((aligned(4)));
-        const f32x4 a = *reinterpret_cast<const uv*>(p), b = *reinterpret_cast<const uv*>(p + 4);
+        const f32x4 a = *reinterpret_cast<const uv*>(p), b = *reinterpret_cast<const uv*>(p + 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             v[i] = a[i];
@@ -243,60 +271,109 @@ struct Raw<F32> {
     }
 };
 
+// A plane of [rows][COLS] 16-bit elements in LDS without padding: the 16-byte
+// groups of a row are XORed by a number of the row, chosen so that the reads
+// below meet every bank once a phase: of M = COLS / 8 groups (16 at most, 256
+// bytes) and k the row in units of 256 bytes, k with its bits rotated left by
+// one.  Sixteen rows at one group then take all of them, and so do the group
+// pairs of eight rows.  The number has a period of 16 rows.
+template <int COLS>
+__device__ __forceinline__ int swizzle(int row) {
+    constexpr int M = COLS < 128 ? COLS / 8 : 16, L = M == 16 ? 4 : M == 8 ? 3 : 2;
+    static_assert(M >= 4, "at least 32 columns");
+    const int k = (row / (16 / M)) & (M - 1);
+    return ((2 * k) & (M - 1)) | (k >> (L - 1));
+}
+template <int COLS>
+__device__ __forceinline__ int place(int row, int col) {
+    return row * COLS + (((col >> 3) ^ swizzle<COLS>(row)) << 3) + (col & 7);
+}
+
 // Rows of a chunk on their way to LDS: Q rows of COLS elements over THREADS
 // threads, eight at a time.  Every load is whole and inside its row: a vector
 // that would pass the row's end starts earlier, if need be before `base`, and is
-// moved into place (whole rows hold at least eight elements).
-template <typename E, int Q, int COLS, int THREADS>
+// moved into place (whole rows hold at least eight elements).  Offsets are 32
+// bits from the chunk's first row (the host checks the strides).
+// LDS planes have LC columns.
+template <typename E, int Q, int COLS, int THREADS, int LC = COLS>
 struct Rows {
-    static constexpr int kVecs = Q * COLS / 8, kEach = (kVecs + THREADS - 1) / THREADS, kPitch = COLS + 8;
+    static constexpr int kVecs = Q * COLS / 8, kEach = (kVecs + THREADS - 1) / THREADS;
     Raw<E> r[kEach];
-    // Rows from token t on, the last at most tokens - 1 past it.
+    int32_t at[kEach];   // of a whole chunk, in bytes
+    __device__ __forceinline__ int32_t offset(int i, int64_t ts, int tokens, int width) const {
+        const int v = threadIdx.x + i * THREADS, row = min(v / (COLS / 8), min(tokens, Q) - 1), c = v % (COLS / 8) * 8;
+        return (row * int32_t(ts) + min(c, width - 8)) * E::kBytes;
+    }
+    __device__ __forceinline__ void init(int64_t ts, int width) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) at[i] = offset(i, ts, Q, width);
+    }
+    // Of a whole chunk whose first row lies at `base`, and of one of `tokens` rows.
+    __device__ __forceinline__ void load(const typename E::T* base) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) r[i].load(reinterpret_cast<const char*>(base) + at[i]);
+    }
     __device__ __forceinline__ void load(const typename E::T* base, int64_t ts, int tokens, int width) {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int at = threadIdx.x + i * THREADS, row = min(at / (COLS / 8), tokens - 1), c = at % (COLS / 8) * 8;
-            r[i].load(base + row * ts + min(c, width - 8));
+        for (int i = 0; i < kEach; ++i) r[i].load(reinterpret_cast<const char*>(base) + offset(i, ts, tokens, width));
+    }
+    __device__ __forceinline__ void trim(int tokens, int width) {
+        if (width < COLS) {
+            const int v = fresh(threadIdx.x);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int c = (v + i * THREADS) % (COLS / 8) * 8;
+                r[i].drop(min(8, c - min(c, width - 8)));
+            }
+        }
+        if (tokens < Q) {
+            const int v = fresh(threadIdx.x);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) r[i].keep_if((v + i * THREADS) / (COLS / 8) < tokens);
         }
     }
     // As they are, to [Q][PITCH] of T.
     template <int PITCH>
-    __device__ __forceinline__ void store_raw(typename E::T* lds, int width) {
+    __device__ __forceinline__ void store_raw(typename E::T* lds, int tokens, int width) {
+        trim(tokens, width);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int at = threadIdx.x + i * THREADS, row = at / (COLS / 8), c = at % (COLS / 8) * 8;
-            if (width < COLS) r[i].drop(min(8, c - min(c, width - 8)));
-            if (kVecs % THREADS == 0 || at < kVecs) r[i].put(lds + row * PITCH + c);
+            const int v = threadIdx.x + i * THREADS;
+            if (kVecs % THREADS == 0 || v < kVecs) r[i].put(lds + v / (COLS / 8) * PITCH + v % (COLS / 8) * 8);
         }
     }
-    // To kIn planes of [Q][kPitch].
+    // To kIn planes.
     __device__ __forceinline__ void store(uint16_t* lds, int tokens, int width) {
+        trim(tokens, width);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int at = threadIdx.x + i * THREADS, row = at / (COLS / 8), c = at % (COLS / 8) * 8;
-            if (width < COLS) r[i].drop(min(8, c - min(c, width - 8)));
-            r[i].keep_if(row < tokens);
-            if (kVecs % THREADS == 0 || at < kVecs) {
+            const int v = threadIdx.x + i * THREADS;
+            if (kVecs % THREADS == 0 || v < kVecs) {
                 u32x4 t[Scheme<E>::kIn];
                 r[i].terms(t);
 #pragma unroll
                 for (int k = 0; k < Scheme<E>::kIn; ++k)
-                    *reinterpret_cast<u32x4*>(lds + (k * Q + row) * kPitch + c) = t[k];
+                    *reinterpret_cast<u32x4*>(lds + k * Q * LC + place<LC>(v / (COLS / 8), v % (COLS / 8) * 8)) = t[k];
             }
         }
     }
 };
 
-// Operand fragments of a [rows][PITCH] plane in LDS.
-// Lane l: row l % 16, eight columns from 8 (l / 16).
-template <typename V8>
-__device__ __forceinline__ V8 frag_row(const uint16_t* p) {
-    return *reinterpret_cast<const V8*>(p);
+// Operand fragments of planes of COLS columns.  r16 is a multiple of 16 rows.
+// Lane l: row r16 + l % 16, eight columns from c + 8 (l / 16).
+template <typename V8, int COLS>
+__device__ __forceinline__ V8 frag_row(const uint16_t* p, int r16, int c, int lane) {
+    const int row = lane & 15;
+    return *reinterpret_cast<const V8*>(p + r16 * COLS + row * COLS +
+                                        (((c >> 3) ^ ((lane >> 4) ^ swizzle<COLS>(row))) << 3));
 }
-// Lane l: row l % 16, columns 4 (l / 16) .. + 3 and those 16 further on.
-template <typename V8>
-__device__ __forceinline__ V8 frag_split(const uint16_t* p) {
-    const u32x2 a = *reinterpret_cast<const u32x2*>(p), b = *reinterpret_cast<const u32x2*>(p + 16);
+// Lane l: row r16 + l % 16, columns c + 4 (l / 16) .. + 3 and those 16 further on.
+template <typename V8, int COLS>
+__device__ __forceinline__ V8 frag_split(const uint16_t* p, int r16, int c, int lane) {
+    const int row = lane & 15, g = (lane >> 5) ^ swizzle<COLS>(row);
+    const uint16_t* q = p + r16 * COLS + row * COLS + 4 * ((lane >> 4) & 1);
+    const u32x2 a = *reinterpret_cast<const u32x2*>(q + (((c >> 3) ^ g) << 3));
+    const u32x2 b = *reinterpret_cast<const u32x2*>(q + (((c >> 3) ^ 2 ^ g) << 3));
     return __builtin_bit_cast(V8, u32x4{a[0], a[1], b[0], b[1]});
 }
 // Transposing read: lane 4 j + q of each 16 points at row j, columns 4 q .. + 3;
@@ -306,41 +383,56 @@ __device__ __forceinline__ u32x2 read_tr(const uint16_t* p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                          (__attribute__((address_space(3))) i16x4*)(p)));
 }
-template <typename V8, int PITCH>
-__device__ __forceinline__ V8 frag_tr(const uint16_t* p) {
-    const u32x2 a = read_tr(p), b = read_tr(p + 4 * PITCH);
+// Lane l: column c + l % 16 (c a multiple of 16), rows r16 + 4 (l / 16) .. + 3.
+template <int COLS>
+__device__ __forceinline__ u32x2 read_tr(const uint16_t* p, int r16, int c, int lane) {
+    const int row = 4 * (lane >> 4) + ((lane >> 2) & 3);
+    return read_tr(p + r16 * COLS + row * COLS + (((c >> 3) ^ (((lane >> 1) & 1) ^ swizzle<COLS>(row))) << 3) +
+                   4 * (lane & 1));
+}
+// The same rows and those 16 further on.
+template <typename V8, int COLS>
+__device__ __forceinline__ V8 frag_tr(const uint16_t* p, int r16, int c, int lane) {
+    const u32x2 a = read_tr<COLS>(p, r16, c, lane), b = read_tr<COLS>(p, r16 + 16, c, lane);
     return __builtin_bit_cast(V8, u32x4{a[0], a[1], b[0], b[1]});
 }
 
 // ------------------------------------------------------------------- kernel --
 
+
 template <typename E, int NT, int Q, int WAVES>
 struct ChunkShape {
     static constexpr int kPT = 16 * WAVES, kThreads = 64 * WAVES, kIn = Scheme<E>::kIn, kOut = Scheme<E>::kOut;
-    static constexpr int kBP = NT + 8, kXP = kPT + 8, kPP = Q + 8, kZP = kPT + 16 / E::kBytes;
+    static constexpr int kXC = WAVES == 3 ? 64 : kPT;          // columns of x's planes: a power of two
+    static constexpr int kZP = kPT + 16 / E::kBytes;
     static constexpr int kTokens = 256;  // whose step sizes are prepared at a time
+    // Waves of a SIMD that the registers are held to.
+    static constexpr int kPerSimd = E::kBytes == 2 && NT <= 128 && (NT < 128 || WAVES > 2) ? 3 : 2;
     struct Lds {
-        alignas(16) uint16_t b[kIn * Q * kBP], c[kIn * Q * kBP], x[kIn * Q * kXP], p[kOut * Q * kPP];
+        alignas(16) uint16_t b[kIn * Q * NT], c[kIn * Q * NT], x[kIn * Q * kXC], p[kOut * Q * Q];
         alignas(16) float step[kTokens], hi[kTokens], lo[kTokens], weight[kTokens], fade[kTokens], row[Q];
         float whole[kTokens / Q];
         alignas(16) typename E::T z[Q * kZP];  // the gate's inputs, then the outputs
     };
     struct LdsStates {
-        alignas(16) uint16_t b[kIn * Q * kBP], x[kIn * Q * kXP];
+        alignas(16) uint16_t b[kIn * Q * NT], x[kIn * Q * kXC];
         alignas(16) float weight[kTokens];
         float whole[kTokens / Q];
     };
+    // Blocks of the main kernel that a CU of 160 KB holds.
+    static constexpr int kResident = std::min(4 * kPerSimd / WAVES, int(160 * 1024 / sizeof(Lds)));
+    static_assert(kResident >= 1, "too much LDS");
 };
 
 // MAIN: outputs (and the final states); else the pieces' contributions.
 template <typename E, int NT, int Q, int WAVES, bool MAIN>
-__global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
+__global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)) void chunk_kernel(ChunkArgs g) {
     using T = typename E::T;
     using Sch = Scheme<E>;
     using V8 = typename Sch::V8;
     using Shape = ChunkShape<E, NT, Q, WAVES>;
     constexpr int kThreads = Shape::kThreads, kPT = Shape::kPT, kIn = Sch::kIn, kState = Sch::kState, kOut = Sch::kOut;
-    constexpr int kBP = Shape::kBP, kXP = Shape::kXP, kPP = Shape::kPP, kZP = Shape::kZP, kTokens = Shape::kTokens;
+    constexpr int kZP = Shape::kZP, kXC = Shape::kXC, kTokens = Shape::kTokens;
     constexpr int kTT = Q / 16, kNN = NT / 16, kKS = Q / 32, kKN = NT / 32;
     __shared__ std::conditional_t<MAIN, typename Shape::Lds, typename Shape::LdsStates> m;
     const ScanArgs& a = g.s;
@@ -385,6 +477,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
 #pragma unroll
     for (int i = 0; i < kNN; ++i) S[i] = f32x4{0, 0, 0, 0};
     const int64_t ys = int64_t(a.H) * a.P;  // token stride of y
+    T* yb = static_cast<T*>(a.y) + ((a.cu ? 0 : int64_t(piece.seq) * a.T) + piece.t0) * ys + int64_t(h) * a.P + p0;
     const int64_t state_at = ((int64_t(piece.seq) * a.H + h) * a.P + p) * a.N;
     if (MAIN && (ws || a.state_in)) {
         have_state = true;
@@ -408,18 +501,40 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
 
     Rows<E, Q, NT, kThreads> rb;
     Rows<E, Q, MAIN ? NT : 32, kThreads> rc;
-    Rows<E, Q, kPT, kThreads> rx, rz;
+    Rows<E, Q, kPT, kThreads, kXC> rx;
+    Rows<E, Q, kPT, kThreads> rz;
     const bool gated = MAIN && a.z;
-    auto fetch = [&](int t) {
-        const int left = tokens - t;
-        rb.load(bb + t * a.b_ts, a.b_ts, left, a.N);
-        rx.load(xb + t * a.x_ts, a.x_ts, left, a.P - p0);
+    rb.init(a.b_ts, a.N);
+    rx.init(a.x_ts, a.P - p0);
+    if constexpr (MAIN) {
+        rc.init(a.c_ts, a.N);
+        rz.init(a.z_ts, a.P - p0);
+    }
+    // The next chunk's rows: `left` tokens from where the pointers stand.
+    auto fetch = [&](int left) {
+        if (left >= Q) {
+            rb.load(bb);
+            rx.load(xb);
+            if constexpr (MAIN) {
+                rc.load(cb);
+                if (gated) rz.load(zb);
+            }
+        } else {
+            rb.load(bb, a.b_ts, left, a.N);
+            rx.load(xb, a.x_ts, left, a.P - p0);
+            if constexpr (MAIN) {
+                rc.load(cb, a.c_ts, left, a.N);
+                if (gated) rz.load(zb, a.z_ts, left, a.P - p0);
+            }
+        }
+        bb += Q * a.b_ts;
+        xb += Q * a.x_ts;
         if constexpr (MAIN) {
-            rc.load(cb + t * a.c_ts, a.c_ts, left, a.N);
-            if (gated) rz.load(zb + t * a.z_ts, a.z_ts, left, a.P - p0);
+            cb += Q * a.c_ts;
+            zb += Q * a.z_ts;
         }
     };
-    fetch(0);
+    fetch(tokens);
     // Raw step sizes of the next kTokens, a wave 64 of them at a time.
     constexpr int kParts = kTokens / 64, kOwn = (kParts + WAVES - 1) / WAVES;
     float raw[kOwn];
@@ -439,7 +554,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
         rx.store(m.x, left, a.P - p0);
         if constexpr (MAIN) {
             rc.store(m.c, left, a.N);
-            if (gated) rz.template store_raw<kZP>(m.z, a.P - p0);
+            if (gated) rz.template store_raw<kZP>(m.z, left, a.P - p0);
         }
         if (at == 0) {
 #pragma unroll
@@ -471,9 +586,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
             }
             if (t0 + kTokens < tokens) fetch_dt(t0 + kTokens);
         }
-        if (t0 + Q < tokens) fetch(t0 + Q);
+        if (left > Q) fetch(left - Q);
         __syncthreads();
 
+        int ln = fresh(lane);
         __builtin_amdgcn_sched_barrier(0);
         // G^T, weighted: P[t][s] = G_ts exp(run_t - run_s) d_s, s <= t.
         if constexpr (MAIN) {
@@ -489,14 +605,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
                     for (int kk = 0; kk < kKN; ++kk) {
                         V8 cf[kIn];
 #pragma unroll
-                        for (int k = 0; k < kIn; ++k) cf[k] = frag_row<V8>(m.c + (k * Q + t) * kBP + 32 * kk + 8 * lg);
+                        for (int k = 0; k < kIn; ++k) cf[k] = frag_row<V8, NT>(m.c + k * Q * NT, 16 * tt, 32 * kk, ln);
 #pragma unroll
                         for (int s = 0; s < kTT; ++s)
                             if (s <= tt) {
                                 V8 bf[kIn];
 #pragma unroll
                                 for (int k = 0; k < kIn; ++k)
-                                    bf[k] = frag_row<V8>(m.b + (k * Q + 16 * s + lr) * kBP + 32 * kk + 8 * lg);
+                                    bf[k] = frag_row<V8, NT>(m.b + k * Q * NT, 16 * s, 32 * kk, ln);
                                 w[s] = mma(bf, cf, w[s]);
                             }
                     }
@@ -512,7 +628,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const float e = __builtin_amdgcn_exp2f((hi - sh[i]) + (lo - sl[i]));
-                                w[s][i] = s0 + i <= t ? w[s][i] * (e * sd[i]) : 0.0f;
+                                w[s][i] *= e * sd[i];
+                                if (s == tt) w[s][i] = s0 + i <= t ? w[s][i] : 0.0f;
                                 if constexpr (Sch::kScaled) top = fmaxf(top, fabsf(w[s][i]));
                             }
                         }
@@ -528,7 +645,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
                             f32x2 u = {w[s][0] * factor, w[s][1] * factor}, v = {w[s][2] * factor, w[s][3] * factor};
 #pragma unroll
                             for (int k = 0; k < kOut; ++k)
-                                *reinterpret_cast<u32x2*>(m.p + (k * Q + t) * kPP + 16 * s + 4 * lg) =
+                                *reinterpret_cast<u32x2*>(m.p + k * Q * Q + place<Q>(t, 16 * s + 4 * lg)) =
                                     u32x2{take_term((const V8*)nullptr, u), take_term((const V8*)nullptr, v)};
                         }
                 }
@@ -536,16 +653,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
         }
 
         __builtin_amdgcn_sched_barrier(0);
-        V8 xf[kKS][kIn];  // x^T: lane p, eight s
-        int bad = Q;      // the first token whose x is not finite
+        ln = fresh(ln);
+        // x^T: lane p, s = 32 ks + 4 lg .. + 3 and those 16 further on, the order of
+        // all products over s.
+        V8 xf[kKS][kIn];
+        int bad = Q;  // the first token whose x is not finite
+        bool any_bad = false;
         f32x4 y[MAIN ? kTT : 1];
         if (active) {
 #pragma unroll
             for (int ks = 0; ks < kKS; ++ks)
 #pragma unroll
                 for (int k = 0; k < kIn; ++k)
-                    xf[ks][k] = frag_tr<V8, kXP>(m.x + (k * Q + 32 * ks + 8 * lg + (lr >> 2)) * kXP + 16 * wave +
-                                                 4 * (lr & 3));
+                    xf[ks][k] = frag_tr<V8, kXC>(m.x + k * Q * kXC, 32 * ks, 16 * wave, ln);
             if constexpr (MAIN) {
                 // exp(run_t) C S
 #pragma unroll
@@ -575,7 +695,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
                             V8 cf[kIn];
 #pragma unroll
                             for (int k = 0; k < kIn; ++k)
-                                cf[k] = frag_split<V8>(m.c + (k * Q + 16 * tt + lr) * kBP + 32 * kk + 4 * lg);
+                                cf[k] = frag_split<V8, NT>(m.c + k * Q * NT, 16 * tt, 32 * kk, ln);
                             y[tt] = mma(cf, sf, y[tt]);
                         }
                     }
@@ -588,6 +708,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
+            ln = fresh(ln);
             // S' = exp(run_Q) S + B^T (w x)
             float whole = m.whole[at / Q];
             if constexpr (!MAIN) {
@@ -597,15 +718,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
             V8 wx[kKS][kState];
             float wv[kKS][8], top = 0.0f, factor = 1.0f, inverse = 1.0f;
 #pragma unroll
-            for (int ks = 0; ks < kKS; ++ks)
+            for (int ks = 0; ks < kKS; ++ks) {
+                const f32x4 w0 = *reinterpret_cast<const f32x4*>(m.weight + at + 32 * ks + 4 * lg);
+                const f32x4 w1 = *reinterpret_cast<const f32x4*>(m.weight + at + 32 * ks + 16 + 4 * lg);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     float v = elem_f32(xf[ks][0], i);
 #pragma unroll
                     for (int k = 1; k < kIn; ++k) v += elem_f32(xf[ks][k], i);
-                    wv[ks][i] = v * m.weight[at + 32 * ks + 8 * lg + i];
+                    wv[ks][i] = v * (i < 4 ? w0[i & 3] : w1[i & 3]);
                     if constexpr (Sch::kScaled) top = fmaxf(top, fabsf(wv[ks][i]));
                 }
+            }
             if constexpr (Sch::kScaled) factor = scale_for(max_of_groups(top), inverse);
 #pragma unroll
             for (int ks = 0; ks < kKS; ++ks) {
@@ -625,8 +749,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
                     V8 bf[kIn];
 #pragma unroll
                     for (int k = 0; k < kIn; ++k)
-                        bf[k] = frag_tr<V8, kBP>(m.b + (k * Q + 32 * ks + 8 * lg + (lr >> 2)) * kBP + 16 * i +
-                                                 4 * (lr & 3));
+                        bf[k] = frag_tr<V8, NT>(m.b + k * Q * NT, 32 * ks, 16 * i, ln);
                     d = mma(bf, wx[ks], d);
                 }
                 if constexpr (Sch::kScaled) {
@@ -640,19 +763,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
             if constexpr (MAIN) {
                 // Tokens before one whose x is an infinity or NaN must not see
                 // it times their weight of 0: it is taken out and put back below.
-                bool some = false;
+                uint32_t some = 0;
 #pragma unroll
-                for (int ks = 0; ks < kKS; ++ks)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        some |= !(fabsf(elem_f32(xf[ks][0], i)) <= 3.4028235e38f);
-                if (__any(some)) {
+                for (int ks = 0; ks < kKS; ++ks) some |= not_finite(xf[ks][0]);
+                any_bad = __any(some != 0);
+                if (any_bad) {
 #pragma unroll
                     for (int ks = 0; ks < kKS; ++ks)
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
                             if (!(fabsf(elem_f32(xf[ks][0], i)) <= 3.4028235e38f)) {
-                                bad = min(bad, 32 * ks + 8 * lg + i);
+                                bad = min(bad, 32 * ks + 16 * (i / 4) + 4 * lg + i % 4);
 #pragma unroll
                                 for (int k = 0; k < kIn; ++k) xf[ks][k][i] = {};
                             }
@@ -663,6 +784,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
         }
         if constexpr (MAIN) {
             __syncthreads();
+            ln = fresh(ln);
             if (active) {
 #pragma unroll
                 for (int tt = 0; tt < kTT; ++tt) {
@@ -672,7 +794,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
                         V8 pf[kOut];
 #pragma unroll
                         for (int k = 0; k < kOut; ++k)
-                            pf[k] = frag_row<V8>(m.p + (k * Q + 16 * tt + lr) * kPP + 32 * ks + 8 * lg);
+                            pf[k] = frag_split<V8, Q>(m.p + k * Q * Q, 16 * tt, 32 * ks, ln);
                         d = mma(pf, xf[ks], d);
                     }
                     if constexpr (Sch::kScaled) {
@@ -680,15 +802,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) d[i] = __builtin_fmaf(d[i], r[i], y[tt][i]);
                     }
+                    if (any_bad)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (16 * tt + 4 * lg + i >= bad) d[i] = __builtin_nanf("");
                     // x of the outputs' tokens, for the skip
-                    float xv[4] = {0, 0, 0, 0};
+                    float xv[4];
 #pragma unroll
                     for (int k = 0; k < kIn; ++k) {
-                        const u32x2 v = read_tr(m.x + (k * Q + 16 * tt + 4 * lg + (lr >> 2)) * kXP + 16 * wave +
-                                                4 * (lr & 3));
+                        const u32x2 v = read_tr<kXC>(m.x + k * Q * kXC, 16 * tt, 16 * wave, ln);
                         const V8 v8 = __builtin_bit_cast(V8, u32x4{v[0], v[1], 0, 0});
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) xv[i] += elem_f32(v8, i);
+                        for (int i = 0; i < 4; ++i) xv[i] = k ? xv[i] + elem_f32(v8, i) : elem_f32(v8, i);
                     }
                     float zv[4];
                     T* zt = m.z + (16 * tt + 4 * lg) * kZP + 16 * wave + lr;
@@ -703,34 +828,35 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
                         for (int i = 0; i < 4; ++i) zv[i] = E::to_f32(zt[i * kZP]);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float v = __builtin_fmaf(skip, xv[i], d[i]);
-                        if (16 * tt + 4 * lg + i >= bad) v = __builtin_nanf("");
-                        if (gated) v *= silu(zv[i]);
-                        zt[i * kZP] = T(v);
-                    }
+                    for (int i = 0; i < 4; ++i) d[i] = __builtin_fmaf(skip, xv[i], d[i]);
+                    if (gated)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) d[i] *= silu(zv[i]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) zt[i * kZP] = T(d[i]);
                 }
                 // The wave's columns of y, 16 bytes a lane.
                 constexpr int kV = 16 / E::kBytes, kL = 16 / kV, kR = 64 / kL;
                 const int pc = 16 * wave + kV * (lane % kL), have = width - pc;
-                T* yp = static_cast<T*>(a.y) + ((a.cu ? 0 : int64_t(piece.seq) * a.T) + piece.t0 + t0 + lane / kL) * ys +
-                        int64_t(h) * a.P + p0 + pc;
+                char* yp = reinterpret_cast<char*>(yb);
+                const int32_t yo = ((lane / kL) * int32_t(ys) + pc) * E::kBytes, yr = kR * int32_t(ys) * E::kBytes;
 #pragma unroll
                 for (int i = 0; i < Q / kR; ++i) {
                     const int t = lane / kL + i * kR;
                     const T* from = m.z + t * kZP + pc;
                     if (t < left) {
                         if (have >= kV) {
-                            *reinterpret_cast<typename Vec<E, kV>::utype*>(yp + i * kR * ys) =
+                            *reinterpret_cast<typename Vec<E, kV>::utype*>(yp + (yo + i * yr)) =
                                 *reinterpret_cast<const typename Vec<E, kV>::type*>(from);
                         } else {
 #pragma unroll
                             for (int k = 0; k < kV; ++k)
-                                if (k < have) yp[i * kR * ys + k] = from[k];
+                                if (k < have) reinterpret_cast<T*>(yp + (yo + i * yr))[k] = from[k];
                         }
                     }
                 }
             }
+            yb += Q * ys;
         }
     }
 
@@ -754,28 +880,41 @@ __global__ __launch_bounds__(64 * WAVES, 2) void chunk_kernel(ChunkArgs g) {
     }
 }
 
-// The kernels of one element type; `main` 0 the contributions, 1 the outputs.
-void launch_chunks_f16(const ChunkArgs& g, int nt, int waves, bool main, hipStream_t stream);
-void launch_chunks_bf16(const ChunkArgs& g, int nt, int waves, bool main, hipStream_t stream);
-void launch_chunks_f32(const ChunkArgs& g, int nt, int waves, bool main, hipStream_t stream);
+// The kernels of one element type: launches the pieces' contributions or (main)
+// the outputs, or (g null) only tells how many blocks a CU holds.
+int chunks_f16(const ChunkArgs* g, int nt, int waves, bool main, hipStream_t stream);
+int chunks_bf16(const ChunkArgs* g, int nt, int waves, bool main, hipStream_t stream);
+int chunks_f32(const ChunkArgs* g, int nt, int waves, bool main, hipStream_t stream);
 
-template <typename E, int NT, int Q, int WAVES>
-void launch_chunks(const ChunkArgs& g, bool main, hipStream_t stream) {
-    if (main) {
-        const uint32_t blocks = g.blocks + (g.s.cu ? kScanTailBlocks : 0);
-        chunk_kernel<E, NT, Q, WAVES, true><<<blocks, 64 * WAVES, 0, stream>>>(g);
-    } else {
-        chunk_kernel<E, NT, Q, WAVES, false><<<g.blocks, 64 * WAVES, 0, stream>>>(g);
+template <typename E, int NT, int WAVES>
+int chunks(const ChunkArgs* g, bool main, hipStream_t stream) {
+    constexpr int Q = 32;
+    if (g && main) {
+        const uint32_t blocks = g->blocks + (g->s.cu ? kScanTailBlocks : 0);
+        chunk_kernel<E, NT, Q, WAVES, true><<<blocks, 64 * WAVES, 0, stream>>>(*g);
+    } else if (g) {
+        chunk_kernel<E, NT, Q, WAVES, false><<<g->blocks, 64 * WAVES, 0, stream>>>(*g);
     }
+    return ChunkShape<E, NT, Q, WAVES>::kResident;
 }
 
-template <typename E, int NT, int Q>
-void launch_chunks(const ChunkArgs& g, int waves, bool main, hipStream_t stream) {
+template <typename E, int NT>
+int chunks(const ChunkArgs* g, int waves, bool main, hipStream_t stream) {
     if constexpr (NT < 256) {
-        if (waves == 2) return launch_chunks<E, NT, Q, 2>(g, main, stream);
+        if (waves == 2) return chunks<E, NT, 2>(g, main, stream);
     }
-    if (waves == 8) return launch_chunks<E, NT, Q, 8>(g, main, stream);
-    launch_chunks<E, NT, Q, 4>(g, main, stream);
+    if (waves == 3) return chunks<E, NT, 3>(g, main, stream);
+    return chunks<E, NT, 4>(g, main, stream);
+}
+
+template <typename E>
+int chunks(const ChunkArgs* g, int nt, int waves, bool main, hipStream_t stream) {
+    switch (nt) {
+        case 32: return chunks<E, 32>(g, waves, main, stream);
+        case 64: return chunks<E, 64>(g, waves, main, stream);
+        case 128: return chunks<E, 128>(g, waves, main, stream);
+        default: return chunks<E, 256>(g, waves, main, stream);
+    }
 }
 
 }  // namespace ssm

@@ -4,13 +4,8 @@
 namespace pe {
 namespace ssm {
 
-void launch_chunks_bf16(const ChunkArgs& g, int nt, int waves, bool main, hipStream_t stream) {
-    switch (nt) {
-        case 32: return launch_chunks<BF16, 32, 64>(g, waves, main, stream);
-        case 64: return launch_chunks<BF16, 64, 64>(g, waves, main, stream);
-        case 128: return launch_chunks<BF16, 128, 64>(g, waves, main, stream);
-        default: return launch_chunks<BF16, 256, 32>(g, waves, main, stream);
-    }
+int chunks_bf16(const ChunkArgs* g, int nt, int waves, bool main, hipStream_t stream) {
+    return chunks<BF16>(g, nt, waves, main, stream);
 }
 
 }  // namespace ssm
