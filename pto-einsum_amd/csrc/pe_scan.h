@@ -21,8 +21,16 @@ struct ScanArgs {
 };
 
 template <typename E>
-__device__ __forceinline__ float load_dt(const ScanArgs& g, int64_t at) {
-    return g.dt_f32 ? static_cast<const float*>(g.dt)[at] : E::to_f32(static_cast<const typename E::T*>(g.dt)[at]);
+__device__ __forceinline__ uint32_t dt_bits(const ScanArgs& g, const void* dt, int64_t at) {
+    if (E::kBytes == 4 || g.dt_f32) return static_cast<const uint32_t*>(dt)[at];
+    return static_cast<const uint16_t*>(dt)[at];
+}
+template <typename E>
+__device__ __forceinline__ float dt_of(const ScanArgs& g, uint32_t bits) {
+    if constexpr (E::kBytes == 2) {
+        if (!g.dt_f32) return E::to_f32(__builtin_bit_cast(typename E::T, uint16_t(bits)));
+    }
+    return __uint_as_float(bits);
 }
 
 // The step size of head h for the raw value v.

@@ -68,7 +68,7 @@ Plan plan_of(const pe_scan_desc& d, bool packed) {
     if (d.T <= 16 || d.N < 8 || d.P < 8) return p;
     // Offsets within a chunk are 32 bits.
     constexpr int64_t kMostStride = int64_t(1) << 24;
-    for (const int64_t ts : {d.x_ts, d.z_ts, d.b_ts, d.c_ts, d.H * d.P})
+    for (const int64_t ts : {d.x_ts, d.z_ts, d.dt_ts, d.b_ts, d.c_ts, d.H * d.P})
         if (ts >= kMostStride) return p;
     p.chunks = true;
     p.nt = d.N <= 32 ? 32 : d.N <= 64 ? 64 : d.N <= 128 ? 128 : 256;

@@ -199,8 +199,12 @@ __device__ __forceinline__ float scale_for(float m, float& inverse) {
 
 // The largest of the four lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float max_of_groups(float m) {
-    m = fmaxf(m, __shfl_xor(m, 16));
-    return fmaxf(m, __shfl_xor(m, 32));
+    // Both halves of what the swap returns hold, in each lane, one of the pair.
+    const uint32_t u = __float_as_uint(m);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // x, which the compiler takes for another value: what is formed from it inside a
@@ -299,23 +303,26 @@ template <typename E, int Q, int COLS, int THREADS, int LC = COLS>
 struct Rows {
     static constexpr int kVecs = Q * COLS / 8, kEach = (kVecs + THREADS - 1) / THREADS;
     Raw<E> r[kEach];
-    int32_t at[kEach];   // of a whole chunk, in bytes
-    __device__ __forceinline__ int32_t offset(int i, int64_t ts, int tokens, int width) const {
+    // Offsets in bytes from eight elements before the rows, so that they are never
+    // negative and the loads take a scalar base; `at` those of a whole chunk.
+    uint32_t at[kEach];
+    __device__ __forceinline__ uint32_t offset(int i, int32_t ts, int tokens, int width) const {
         const int v = threadIdx.x + i * THREADS, row = min(v / (COLS / 8), min(tokens, Q) - 1), c = v % (COLS / 8) * 8;
-        return (row * int32_t(ts) + min(c, width - 8)) * E::kBytes;
+        return uint32_t(row * ts + min(c, width - 8) + 8) * E::kBytes;
     }
-    __device__ __forceinline__ void init(int64_t ts, int width) {
+    __device__ __forceinline__ void init(int32_t ts, int width) {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) at[i] = offset(i, ts, Q, width);
     }
     // Of a whole chunk whose first row lies at `base`, and of one of `tokens` rows.
     __device__ __forceinline__ void load(const typename E::T* base) {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) r[i].load(reinterpret_cast<const char*>(base) + at[i]);
+        for (int i = 0; i < kEach; ++i) r[i].load(reinterpret_cast<const char*>(base - 8) + at[i]);
     }
-    __device__ __forceinline__ void load(const typename E::T* base, int64_t ts, int tokens, int width) {
+    __device__ __forceinline__ void load(const typename E::T* base, int32_t ts, int tokens, int width) {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) r[i].load(reinterpret_cast<const char*>(base) + offset(i, ts, tokens, width));
+        for (int i = 0; i < kEach; ++i)
+            r[i].load(reinterpret_cast<const char*>(base - 8) + offset(i, ts, tokens, width));
     }
     __device__ __forceinline__ void trim(int tokens, int width) {
         if (width < COLS) {
@@ -342,7 +349,9 @@ struct Rows {
             if (kVecs % THREADS == 0 || v < kVecs) r[i].put(lds + v / (COLS / 8) * PITCH + v % (COLS / 8) * 8);
         }
     }
-    // To kIn planes.
+    // To kIn planes; SPLIT: columns c of each 32 in the order of frag_split, c = 16
+    // h + 4 g + j at 8 g + 4 h + j.
+    template <bool SPLIT = false>
     __device__ __forceinline__ void store(uint16_t* lds, int tokens, int width) {
         trim(tokens, width);
 #pragma unroll
@@ -352,8 +361,16 @@ struct Rows {
                 u32x4 t[Scheme<E>::kIn];
                 r[i].terms(t);
 #pragma unroll
-                for (int k = 0; k < Scheme<E>::kIn; ++k)
-                    *reinterpret_cast<u32x4*>(lds + k * Q * LC + place<LC>(v / (COLS / 8), v % (COLS / 8) * 8)) = t[k];
+                for (int k = 0; k < Scheme<E>::kIn; ++k) {
+                    const int row = v / (COLS / 8), u = v % (COLS / 8);
+                    if constexpr (SPLIT) {
+                        const int c = 8 * ((u & ~3) + 2 * (u & 1)) + 4 * ((u >> 1) & 1);
+                        *reinterpret_cast<u32x2*>(lds + k * Q * LC + place<LC>(row, c)) = u32x2{t[k][0], t[k][1]};
+                        *reinterpret_cast<u32x2*>(lds + k * Q * LC + place<LC>(row, c + 8)) = u32x2{t[k][2], t[k][3]};
+                    } else {
+                        *reinterpret_cast<u32x4*>(lds + k * Q * LC + place<LC>(row, 8 * u)) = t[k];
+                    }
+                }
             }
         }
     }
@@ -451,13 +468,21 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     const uint32_t ph = job / g.ptiles, pt = job - ph * g.ptiles;
     const uint32_t id = ph / uint32_t(a.H), h = ph - id * uint32_t(a.H);
     Piece piece;
-    if (!find_piece(g, id, piece)) return;
+    if (!__builtin_amdgcn_readfirstlane(find_piece(g, id, piece))) return;
+    // The same for the whole block: kept in scalar registers.
+    piece.t0 = __builtin_amdgcn_readfirstlane(int(piece.t0));
+    piece.t1 = __builtin_amdgcn_readfirstlane(int(piece.t1));
+    piece.seq = __builtin_amdgcn_readfirstlane(piece.seq);
+    piece.last = __builtin_amdgcn_readfirstlane(piece.last);
     if (!MAIN && piece.last) return;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 15, lg = lane >> 4;
     const int p0 = int(pt) * kPT, width = min(kPT, a.P - p0);  // columns of x
     const bool active = 16 * wave < width;
+    // The wave's turn at the scores: other waves from block to block, since a
+    // block's first wave is on the same SIMD in each.
+    const int scorer = int((uint32_t(wave) + job) % WAVES);
     const int p = p0 + 16 * wave + lr;
     const int64_t seq = a.cu ? 0 : piece.seq;
     const int group = int(h) / (a.H / a.G);
@@ -467,7 +492,11 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     const T* zb = static_cast<const T*>(a.z) + seq * a.z_bs + piece.t0 * a.z_ts + h * a.z_hs + p0;
     const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
     const double A2 = double(A) * 1.4426950408889634;  // exponents are of 2
-    const int64_t dt_at = seq * a.dt_bs + piece.t0 * a.dt_ts + h * a.dt_hs;
+    const char* dtp = static_cast<const char*>(a.dt) +
+                      (seq * a.dt_bs + piece.t0 * a.dt_ts + h * a.dt_hs) * (a.dt_f32 ? 4 : E::kBytes);
+    // Token strides: below 2^24 (the host sees to it).
+    const int32_t b_ts = int32_t(a.b_ts), c_ts = int32_t(a.c_ts), x_ts = int32_t(a.x_ts), z_ts = int32_t(a.z_ts);
+    const int32_t dt_ts = int32_t(a.dt_ts);
     const int tokens = int(piece.t1 - piece.t0);
 
     f32x4 S[kNN];  // lane: p = lr; n = 16 i + 4 lg + element
@@ -476,8 +505,8 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     bool have_state = false;
 #pragma unroll
     for (int i = 0; i < kNN; ++i) S[i] = f32x4{0, 0, 0, 0};
-    const int64_t ys = int64_t(a.H) * a.P;  // token stride of y
-    T* yb = static_cast<T*>(a.y) + ((a.cu ? 0 : int64_t(piece.seq) * a.T) + piece.t0) * ys + int64_t(h) * a.P + p0;
+    const int32_t ys = a.H * a.P;  // token stride of y
+    T* yb = static_cast<T*>(a.y) + ((a.cu ? 0 : int64_t(piece.seq) * a.T) + piece.t0) * int64_t(ys) + int64_t(h) * a.P + p0;
     const int64_t state_at = ((int64_t(piece.seq) * a.H + h) * a.P + p) * a.N;
     if (MAIN && (ws || a.state_in)) {
         have_state = true;
@@ -504,11 +533,11 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     Rows<E, Q, kPT, kThreads, kXC> rx;
     Rows<E, Q, kPT, kThreads> rz;
     const bool gated = MAIN && a.z;
-    rb.init(a.b_ts, a.N);
-    rx.init(a.x_ts, a.P - p0);
+    rb.init(b_ts, a.N);
+    rx.init(x_ts, a.P - p0);
     if constexpr (MAIN) {
-        rc.init(a.c_ts, a.N);
-        rz.init(a.z_ts, a.P - p0);
+        rc.init(c_ts, a.N);
+        rz.init(z_ts, a.P - p0);
     }
     // The next chunk's rows: `left` tokens from where the pointers stand.
     auto fetch = [&](int left) {
@@ -520,28 +549,29 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                 if (gated) rz.load(zb);
             }
         } else {
-            rb.load(bb, a.b_ts, left, a.N);
-            rx.load(xb, a.x_ts, left, a.P - p0);
+            rb.load(bb, b_ts, left, a.N);
+            rx.load(xb, x_ts, left, a.P - p0);
             if constexpr (MAIN) {
-                rc.load(cb, a.c_ts, left, a.N);
-                if (gated) rz.load(zb, a.z_ts, left, a.P - p0);
+                rc.load(cb, c_ts, left, a.N);
+                if (gated) rz.load(zb, z_ts, left, a.P - p0);
             }
         }
-        bb += Q * a.b_ts;
-        xb += Q * a.x_ts;
+        bb += Q * b_ts;
+        xb += Q * x_ts;
         if constexpr (MAIN) {
-            cb += Q * a.c_ts;
-            zb += Q * a.z_ts;
+            cb += Q * c_ts;
+            zb += Q * z_ts;
         }
     };
     fetch(tokens);
     // Raw step sizes of the next kTokens, a wave 64 of them at a time.
     constexpr int kParts = kTokens / 64, kOwn = (kParts + WAVES - 1) / WAVES;
-    float raw[kOwn];
+    uint32_t raw[kOwn];
     auto fetch_dt = [&](int t) {
 #pragma unroll
         for (int i = 0; i < kOwn; ++i)
-            raw[i] = load_dt<E>(a, dt_at + min(t + 64 * (wave + i * WAVES) + lane, tokens - 1) * a.dt_ts);
+            raw[i] = dt_bits<E>(a, dtp, min(64 * (wave + i * WAVES) + lane, tokens - t - 1) * dt_ts);
+        dtp += int64_t(kTokens) * dt_ts * (a.dt_f32 ? 4 : E::kBytes);
     };
     fetch_dt(0);
     double sum = 0.0;  // of this piece's exponents
@@ -553,7 +583,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
         rb.store(m.b, left, a.N);
         rx.store(m.x, left, a.P - p0);
         if constexpr (MAIN) {
-            rc.store(m.c, left, a.N);
+            rc.template store<true>(m.c, left, a.N);
             if (gated) rz.template store_raw<kZP>(m.z, left, a.P - p0);
         }
         if (at == 0) {
@@ -561,7 +591,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
             for (int i = 0; i < kOwn; ++i) {
                 const int part = wave + i * WAVES, tok = 64 * part + lane;
                 if (part < kParts) {
-                    const float d = t0 + tok < tokens ? step_size(a, raw[i], bias) : 0.0f;
+                    const float d = t0 + tok < tokens ? step_size(a, dt_of<E>(a, raw[i]), bias) : 0.0f;
                     // Decays below 2^-4096 are 0 all the same.
                     double e = A2 * double(d);
                     e = e < -4096.0 ? -4096.0 : e;
@@ -595,7 +625,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
         if constexpr (MAIN) {
 #pragma unroll
             for (int it = 0; it < (kTT + WAVES - 1) / WAVES; ++it) {
-                const int tt = it == 0 ? wave : kTT - 1 - wave;
+                const int tt = scorer + it * WAVES;
                 if (tt < kTT) {
                     const int t = 16 * tt + lr;
                     f32x4 w[kTT];
@@ -612,7 +642,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                                 V8 bf[kIn];
 #pragma unroll
                                 for (int k = 0; k < kIn; ++k)
-                                    bf[k] = frag_row<V8, NT>(m.b + k * Q * NT, 16 * s, 32 * kk, ln);
+                                    bf[k] = frag_split<V8, NT>(m.b + k * Q * NT, 16 * s, 32 * kk, ln);
                                 w[s] = mma(bf, cf, w[s]);
                             }
                     }
@@ -695,7 +725,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                             V8 cf[kIn];
 #pragma unroll
                             for (int k = 0; k < kIn; ++k)
-                                cf[k] = frag_split<V8, NT>(m.c + k * Q * NT, 16 * tt, 32 * kk, ln);
+                                cf[k] = frag_row<V8, NT>(m.c + k * Q * NT, 16 * tt, 32 * kk, ln);
                             y[tt] = mma(cf, sf, y[tt]);
                         }
                     }
@@ -758,6 +788,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                 } else {
                     S[i] = d;
                 }
+                if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);
             }
             have_state = true;
             if constexpr (MAIN) {
@@ -768,6 +799,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                 for (int ks = 0; ks < kKS; ++ks) some |= not_finite(xf[ks][0]);
                 any_bad = __any(some != 0);
                 if (any_bad) {
+                    bad = fresh(bad);  // keeps this from being computed always
 #pragma unroll
                     for (int ks = 0; ks < kKS; ++ks)
 #pragma unroll
@@ -802,10 +834,12 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) d[i] = __builtin_fmaf(d[i], r[i], y[tt][i]);
                     }
-                    if (any_bad)
+                    if (any_bad) {
+                        const int first = fresh(bad);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (16 * tt + 4 * lg + i >= bad) d[i] = __builtin_nanf("");
+                            if (16 * tt + 4 * lg + i >= first) d[i] = __builtin_nanf("");
+                    }
                     // x of the outputs' tokens, for the skip
                     float xv[4];
 #pragma unroll
@@ -839,7 +873,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                 constexpr int kV = 16 / E::kBytes, kL = 16 / kV, kR = 64 / kL;
                 const int pc = 16 * wave + kV * (lane % kL), have = width - pc;
                 char* yp = reinterpret_cast<char*>(yb);
-                const int32_t yo = ((lane / kL) * int32_t(ys) + pc) * E::kBytes, yr = kR * int32_t(ys) * E::kBytes;
+                const uint32_t yo = uint32_t((lane / kL) * ys + pc) * E::kBytes, yr = uint32_t(kR * ys) * E::kBytes;
 #pragma unroll
                 for (int i = 0; i < Q / kR; ++i) {
                     const int t = lane / kL + i * kR;

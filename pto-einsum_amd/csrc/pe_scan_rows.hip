@@ -88,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(ScanArgs g, uint32_t til
     }
     const float A = g.A[h], bias = g.dt_bias ? g.dt_bias[h] : 0.0f, skip = g.D ? g.D[h] : 0.0f;
     for (int64_t t = t0; t < t1; ++t) {
-        const float d = step_size(g, load_dt<E>(g, seq * g.dt_bs + t * g.dt_ts + h * g.dt_hs), bias);
+        const float d = step_size(g, dt_of<E>(g, dt_bits<E>(g, g.dt, seq * g.dt_bs + t * g.dt_ts + h * g.dt_hs)), bias);
         const float a = expf(A * d);
         float b[4], c[4];
         const int left = g.N - n0;
