@@ -927,7 +927,7 @@ int chunks(const ChunkArgs* g, bool main, hipStream_t stream) {
         const uint32_t blocks = g->blocks + (g->s.cu ? kScanTailBlocks : 0);
         chunk_kernel<E, NT, Q, WAVES, true><<<blocks, 64 * WAVES, 0, stream>>>(*g);
     } else if (g) {
-        chunk_kernel<E, NT, Q, WAVES, false><<<g->blocks, 64 * WAVES, 0, stream>>>(*g);
+        chunk_kernel<E, NT, E::kBytes == 2 && NT <= 128 ? 64 : 32, WAVES, false><<<g->blocks, 64 * WAVES, 0, stream>>>(*g);
     }
     return ChunkShape<E, NT, Q, WAVES>::kResident;
 }

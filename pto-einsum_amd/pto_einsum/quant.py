@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import abi, runtime
-from .ssm import DTYPES, _ptr, extent, inner, lib, no_grad, of_shape, of_type, same_gpu
+from .ssm import DTYPES, _plans, _ptr, check, dense, extent, inner, layout, lib, on, ready, remember
 
 
 def matvec_q4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
@@ -26,29 +26,39 @@ def matvec_q4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros
     k; scales and zeros (none: 8) [N, ceil(K / group)] of x's dtype.  Sums are
     float32; y has x's dtype.  The weights are read once for every 64 rows of x."""
     what = "matvec_q4"
-    if x.dtype not in DTYPES:
-        raise TypeError(f"{what}: unsupported dtype {x.dtype} for x")
-    if x.dim() < 1:
-        raise ValueError(f"{what}: x must have an axis")
-    if group not in (32, 64, 128):
-        raise ValueError(f"{what}: group must be 32, 64 or 128, got {group}")
-    K = x.shape[-1]
-    if packed.dtype != torch.uint8 or packed.dim() != 2:
-        raise TypeError(f"{what}: packed must be a 2-D uint8 tensor, got {packed.dtype} of shape {tuple(packed.shape)}")
-    N = packed.shape[0]
-    of_type(what, x.dtype, scales=scales, zeros=zeros)
-    of_shape(what, packed=(packed, (N, (K + 1) // 2)), scales=(scales, (N, -(-K // group))),
-             zeros=(zeros, (N, -(-K // group))))
-    no_grad(what, x, scales, zeros)
-    dev = same_gpu(what, x, packed=packed, scales=scales, zeros=zeros)
-    rows = inner(x if x.dim() == 2 else x.reshape(-1, K) if K else x.reshape(x.shape[:-1].numel(), 0))
-    packed, scales = packed.contiguous(), scales.contiguous()
-    zeros = None if zeros is None else zeros.contiguous()
-    d = abi.Q4Desc(dtype=DTYPES[x.dtype], group=group, M=rows.shape[0], N=N, K=K, x_ms=rows.stride(0),
-                   x_numel=extent(rows))
-    with torch.cuda.device(dev):
-        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
-        rc = lib().pe_matvec_q4(ctypes.byref(d), _ptr(rows), _ptr(packed), _ptr(scales), _ptr(zeros), _ptr(y),
-                                runtime.raw_stream(dev.index))
+    key = (what, layout(x), layout(packed), layout(scales), layout(zeros), group)
+    plan = _plans.get(key)
+    if plan is None:
+        if x.dtype not in DTYPES:
+            raise TypeError(f"{what}: unsupported dtype {x.dtype} for x")
+        if x.dim() < 1:
+            raise ValueError(f"{what}: x must have an axis")
+        if group not in (32, 64, 128):
+            raise ValueError(f"{what}: group must be 32, 64 or 128, got {group}")
+        K = x.shape[-1]
+        if packed.dtype is not torch.uint8 or packed.dim() != 2:
+            raise TypeError(f"{what}: packed must be a 2-D uint8 tensor, got {packed.dtype} of shape "
+                            f"{tuple(packed.shape)}")
+        N = packed.shape[0]
+        if packed.shape[1] != (K + 1) // 2:
+            raise ValueError(f"{what}: packed must have shape {(N, (K + 1) // 2)}, got {tuple(packed.shape)}")
+        groups = (N, -(-K // group))
+        check(what, "scales", scales, groups, x.dtype)
+        check(what, "zeros", zeros, groups, x.dtype)
+        ready(what, x, packed, scales, zeros)
+        if x.dim() != 2:
+            rows = x.reshape(-1, K) if K else x.reshape(x.shape[:-1].numel(), 0)
+            return matvec_q4(rows, packed, scales, zeros, group=group).reshape(*x.shape[:-1], N)
+        given, laid = (x, packed, scales, zeros), (inner(x), dense(packed), dense(scales), dense(zeros))
+        if any(g is not t for g, t in zip(given, laid)):
+            return matvec_q4(*laid, group=group)
+        d = abi.Q4Desc(DTYPES[x.dtype], group, x.shape[0], N, K, x.stride(0), extent(x))
+        plan = remember(key, (d, (x.shape[0], N)))
+    d, shape = plan
+    dev = ready(what, x, packed, scales, zeros)
+    with on(dev):
+        y = x.new_empty(shape)
+        rc = lib().pe_matvec_q4(ctypes.byref(d), x.data_ptr(), packed.data_ptr(), scales.data_ptr(), _ptr(zeros),
+                                y.data_ptr(), runtime.raw_stream(dev))
     runtime.check(rc, "pe_matvec_q4")
     return y

@@ -17,6 +17,7 @@ slots outside the cache mark rows without a sequence.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 
@@ -35,9 +36,30 @@ def lib():
     return abi.bind()
 
 
+# A call of single tokens lasts a few microseconds on the GPU, and checking ten
+# operands and filling a descriptor takes longer than that.  So the descriptor of
+# operands that passed is kept by their layouts -- shapes, strides, dtypes and
+# flags, nothing of the tensors themselves -- and a later call of the same layouts
+# only looks at devices and gradients.
+_plans: dict = {}
+
+
+def remember(key, plan):
+    """Keeps a plan; all are dropped when there are many (prompts of ever new
+    lengths)."""
+    if len(_plans) >= 4096:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def layout(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
 def extent(t: torch.Tensor) -> int:
-    """Elements addressable from t's first element to the end of its storage."""
-    return t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+    """Elements from t's first to its last, which torch keeps inside its storage."""
+    return 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else 0
 
 
 def inner(t: torch.Tensor) -> torch.Tensor:
@@ -46,31 +68,46 @@ def inner(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def same_gpu(what: str, x: torch.Tensor, **others) -> torch.device:
-    if x.device.type != "cuda":
-        raise ValueError(f"{what}: operands must live on a GPU, got {x.device}")
-    for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{what}: operands must all live on one GPU, {name} is on {t.device}, not {x.device}")
-    return x.device
+def dense(t):
+    return None if t is None else t.contiguous()
 
 
-def no_grad(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached operands")
-
-
-def of_type(what: str, dtype, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.dtype != dtype:
+def check(what: str, name: str, t, shape, dtype) -> None:
+    """t, where it is given, has that shape and dtype."""
+    if t is not None:
+        if t.shape != shape:
+            raise ValueError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+        if t.dtype is not dtype:
             raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
 
 
-def of_shape(what: str, **tensors) -> None:
-    """``name=(tensor, shape)``: each tensor that is given has that shape."""
-    for name, (t, shape) in tensors.items():
-        if t is not None and tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+def ready(what: str, x, *others) -> int:
+    """The index of the GPU that x and all others (None: not given) live on; no
+    gradient is asked of them."""
+    index = x.get_device()
+    grad = torch.is_grad_enabled()
+    if grad and x.requires_grad:
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached operands")
+    alike = True
+    for t in others:
+        if t is not None:
+            if grad and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached operands")
+            alike = alike and t.get_device() == index
+    if index < 0 or not x.is_cuda:
+        raise ValueError(f"{what}: operands must live on a GPU, got {x.device}")
+    if not alike:
+        where = sorted({str(t.device) for t in others if t is not None} | {str(x.device)})
+        raise ValueError(f"{what}: operands must all live on one GPU, got {', '.join(where)}")
+    return index
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on(index: int):
+    """A context in which GPU ``index`` is the current device."""
+    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def _ptr(t):
@@ -81,7 +118,7 @@ def _index(what: str, name: str, t, length: int | None):
     """An int32 index vector, contiguous."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.dim() != 1:
+    if t.dtype is not torch.int32 or t.dim() != 1:
         raise TypeError(f"{what}: {name} must be a 1-D int32 tensor, got {t.dtype} of shape {tuple(t.shape)}")
     if length is not None and t.shape[0] != length:
         raise ValueError(f"{what}: {name} must have {length} entries, got {t.shape[0]}")
@@ -113,16 +150,18 @@ def _lead(t, packed: bool):
 def _conv_operands(what, x, weight, bias, activation):
     if x.dtype not in DTYPES:
         raise TypeError(f"{what}: unsupported dtype {x.dtype} for x")
-    if activation not in (None, "silu"):
+    if activation is not None and activation != "silu":
         raise ValueError(f"{what}: activation must be None or 'silu', got {activation!r}")
-    if weight.dim() != 2 or weight.shape[0] != x.shape[-1]:
-        raise ValueError(f"{what}: weight must be [{x.shape[-1]}, width], got shape {tuple(weight.shape)}")
+    D = x.shape[-1]
+    if weight.dim() != 2 or weight.shape[0] != D:
+        raise ValueError(f"{what}: weight must be [{D}, width], got shape {tuple(weight.shape)}")
     width = weight.shape[1]
     if not 2 <= width <= MAX_WIDTH:
         raise ValueError(f"{what}: width must be 2 to {MAX_WIDTH}, got {width}")
-    of_type(what, x.dtype, weight=weight, bias=bias)
-    of_shape(what, bias=(bias, (x.shape[-1],)))
-    return width, weight.contiguous(), None if bias is None else bias.contiguous()
+    if weight.dtype is not x.dtype:
+        raise TypeError(f"{what}: weight must be {x.dtype}, got {weight.dtype}")
+    check(what, "bias", bias, (D,), x.dtype)
+    return width, weight.contiguous(), dense(bias)
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -139,23 +178,27 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     sequence's first token, oldest first (none: zeros).  Returns y of x's
     shape and the state after each sequence, both of x's dtype."""
     what = "causal_conv"
-    nseq, T, cu = _sequences(what, x, cu_seqlens, 3)
-    D = x.shape[-1]
-    width, weight, bias = _conv_operands(what, x, weight, bias, activation)
-    of_type(what, x.dtype, initial_state=initial_state)
-    of_shape(what, initial_state=(initial_state, (nseq, width - 1, D)))
-    no_grad(what, x, weight, bias, initial_state)
-    dev = same_gpu(what, x, weight=weight, bias=bias, initial_state=initial_state, cu_seqlens=cu)
-    x = inner(x)
-    first = None if initial_state is None else initial_state.contiguous()
-    d = abi.ConvDesc(dtype=DTYPES[x.dtype], width=width, silu=activation is not None, nseq=nseq, T=T, D=D,
-                     x_numel=extent(x))
-    d.x_bs, d.x_ts = _lead(x, cu is not None)
-    with torch.cuda.device(dev):
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        state = torch.empty((nseq, width - 1, D), dtype=x.dtype, device=dev)
-        rc = lib().pe_causal_conv(ctypes.byref(d), _ptr(x), _ptr(weight), _ptr(bias), _ptr(first), _ptr(cu), _ptr(y),
-                                  _ptr(state), runtime.raw_stream(dev.index))
+    key = (what, layout(x), layout(weight), layout(bias), activation, layout(initial_state), layout(cu_seqlens))
+    plan = _plans.get(key)
+    if plan is None:
+        nseq, T, cu = _sequences(what, x, cu_seqlens, 3)
+        D = x.shape[-1]
+        width, w, b = _conv_operands(what, x, weight, bias, activation)
+        check(what, "initial_state", initial_state, (nseq, width - 1, D), x.dtype)
+        ready(what, x, weight, bias, initial_state, cu)
+        given, laid = (x, weight, bias, initial_state, cu_seqlens), (inner(x), w, b, dense(initial_state), cu)
+        if any(g is not t for g, t in zip(given, laid)):
+            return causal_conv(*laid[:3], activation=activation, initial_state=laid[3], cu_seqlens=cu)
+        x_bs, x_ts = _lead(x, cu is not None)
+        plan = remember(key, (abi.ConvDesc(DTYPES[x.dtype], width, activation is not None, 0, nseq, T, D, x_bs, x_ts, 0,
+                                           extent(x)), (nseq, width - 1, D)))
+    d, state_shape = plan
+    dev = ready(what, x, weight, bias, initial_state, cu_seqlens)
+    with on(dev):
+        y = x.new_empty(x.shape)
+        state = x.new_empty(state_shape)
+        rc = lib().pe_causal_conv(ctypes.byref(d), x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(initial_state),
+                                  _ptr(cu_seqlens), y.data_ptr(), state.data_ptr(), runtime.raw_stream(dev))
     runtime.check(rc, "pe_causal_conv")
     return y, state
 
@@ -168,29 +211,35 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor,
     two rows the same; none: state b); a slot outside [0, S) marks a row
     without a sequence, whose output is zero.  Returns y [B, D]."""
     what = "causal_conv_step"
-    if x.dim() != 2:
-        raise ValueError(f"{what}: x must be [B, D], got shape {tuple(x.shape)}")
-    B, D = x.shape
-    width, weight, bias = _conv_operands(what, x, weight, bias, activation)
-    of_type(what, x.dtype, state=state)
-    S = _cache(what, state, (width - 1, D), B, slots)
-    slots = _index(what, "slots", slots, B)
-    no_grad(what, x, weight, bias, state)
-    dev = same_gpu(what, x, weight=weight, bias=bias, state=state, slots=slots)
-    x = inner(x)
-    d = abi.ConvDesc(dtype=DTYPES[x.dtype], width=width, silu=activation is not None, nseq=B, D=D, x_bs=x.stride(0),
-                     nslots=S, x_numel=extent(x))
-    with torch.cuda.device(dev):
-        y = torch.empty((B, D), dtype=x.dtype, device=dev)
-        rc = lib().pe_causal_conv_step(ctypes.byref(d), _ptr(x), _ptr(weight), _ptr(bias), _ptr(state), _ptr(slots),
-                                       _ptr(y), runtime.raw_stream(dev.index))
+    key = (what, layout(x), layout(weight), layout(state), layout(bias), activation, layout(slots))
+    d = _plans.get(key)
+    if d is None:
+        if x.dim() != 2:
+            raise ValueError(f"{what}: x must be [B, D], got shape {tuple(x.shape)}")
+        B, D = x.shape
+        width, w, b = _conv_operands(what, x, weight, bias, activation)
+        S = _cache(what, state, (width - 1, D), x.dtype, B, slots)
+        at = _index(what, "slots", slots, B)
+        ready(what, x, weight, bias, state, slots)
+        given, laid = (x, weight, bias, slots), (inner(x), w, b, at)
+        if any(g is not t for g, t in zip(given, laid)):
+            return causal_conv_step(laid[0], w, state, b, activation=activation, slots=at)
+        d = remember(key, abi.ConvDesc(DTYPES[x.dtype], width, activation is not None, 0, B, 0, D, x.stride(0), 0, S,
+                                       extent(x)))
+    dev = ready(what, x, weight, bias, state, slots)
+    with on(dev):
+        y = x.new_empty(x.shape)
+        rc = lib().pe_causal_conv_step(ctypes.byref(d), x.data_ptr(), weight.data_ptr(), _ptr(bias), state.data_ptr(),
+                                       _ptr(slots), y.data_ptr(), runtime.raw_stream(dev))
     runtime.check(rc, "pe_causal_conv_step")
     return y
 
 
-def _cache(what, state, shape, B, slots) -> int:
+def _cache(what, state, shape, dtype, B, slots) -> int:
     """The rows of a cache of states [S, *shape]."""
-    if state.dim() != 1 + len(shape) or tuple(state.shape[1:]) != tuple(shape) or not state.is_contiguous():
+    if state.dtype is not dtype:
+        raise TypeError(f"{what}: state must be {dtype}, got {state.dtype}")
+    if state.dim() != 1 + len(shape) or state.shape[1:] != shape or not state.is_contiguous():
         raise ValueError(f"{what}: state must be contiguous [S, {', '.join(map(str, shape))}], got shape "
                          f"{tuple(state.shape)}, strides {state.stride()}")
     if slots is None and state.shape[0] < B:
@@ -200,35 +249,41 @@ def _cache(what, state, shape, B, slots) -> int:
 
 # --------------------------------------------------------------------- scan --
 
-def _scan_desc(what, lead, x, dt, A, B, C, D, z, dt_bias, dt_softplus):
+def _scan_operands(what, lead, x, dt, A, B, C, D, z, dt_bias):
     """Checks the operands of a scan whose tensors start with the axes ``lead``;
-    its descriptor (extents without nseq and T), and the operands laid out."""
-    if x.dtype not in DTYPES:
-        raise TypeError(f"{what}: unsupported dtype {x.dtype} for x")
+    (H, P, G, N) and the operands laid out."""
+    dtype = x.dtype
+    if dtype not in DTYPES:
+        raise TypeError(f"{what}: unsupported dtype {dtype} for x")
     H, P = x.shape[-2:]
-    if B.dim() != len(lead) + 2 or tuple(B.shape[:-2]) != lead:
+    if B.dim() != len(lead) + 2 or B.shape[:-2] != lead:
         raise ValueError(f"{what}: B must be {list(lead)} + [groups, N], got shape {tuple(B.shape)}")
     G, N = B.shape[-2:]
     if G < 1 or H % G:
         raise ValueError(f"{what}: {H} heads do not share {G} groups of B and C evenly")
     if N > MAX_N:
         raise ValueError(f"{what}: N must be at most {MAX_N}, got {N}")
-    of_shape(what, C=(C, B.shape), dt=(dt, (*lead, H)), z=(z, x.shape), A=(A, (H,)), D=(D, (H,)),
-             dt_bias=(dt_bias, (H,)))
-    of_type(what, x.dtype, B=B, C=C, z=z)
-    of_type(what, torch.float32, A=A, D=D, dt_bias=dt_bias)
-    if dt.dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"{what}: dt must be {x.dtype} or float32, got {dt.dtype}")
-    no_grad(what, x, dt, A, B, C, D, z, dt_bias)
-    x, B, C = inner(x), inner(B), inner(C)
-    z = None if z is None else inner(z)
-    A, D, dt_bias = (None if t is None else t.contiguous() for t in (A, D, dt_bias))
-    d = abi.ScanDesc(dtype=DTYPES[x.dtype], dt_dtype=DTYPES[dt.dtype], softplus=bool(dt_softplus), H=H, P=P, G=G, N=N,
-                     x_hs=x.stride(-2), dt_hs=dt.stride(-1), b_gs=B.stride(-2), c_gs=C.stride(-2),
-                     x_numel=extent(x), dt_numel=extent(dt), b_numel=extent(B), c_numel=extent(C))
-    if z is not None:
-        d.z_hs, d.z_numel = z.stride(-2), extent(z)
-    return d, x, dt, A, B, C, D, z, dt_bias
+    if B.dtype is not dtype:
+        raise TypeError(f"{what}: B must be {dtype}, got {B.dtype}")
+    check(what, "C", C, B.shape, dtype)
+    check(what, "dt", dt, (*lead, H), dtype if dt.dtype is dtype else torch.float32)
+    check(what, "z", z, x.shape, dtype)
+    heads, f32 = (H,), torch.float32
+    check(what, "A", A, heads, f32)
+    check(what, "D", D, heads, f32)
+    check(what, "dt_bias", dt_bias, heads, f32)
+    return (H, P, G, N), (inner(x), dt, A.contiguous(), inner(B), inner(C), dense(D), None if z is None else inner(z),
+                          dense(dt_bias))
+
+
+def _scan_desc(x, dt, B, C, z, softplus, nseq, T, H, P, G, N, slots, lead):
+    """The descriptor; ``lead`` gives a tensor's (sequence stride, token stride)."""
+    xs, dts, bs, cs = lead(x), lead(dt), lead(B), lead(C)
+    zs = (0, 0) if z is None else lead(z)
+    z_hs, z_numel = (0, 0) if z is None else (z.stride(-2), extent(z))
+    return abi.ScanDesc(DTYPES[x.dtype], DTYPES[dt.dtype], softplus, 0, nseq, T, H, P, G, N, *xs, x.stride(-2), *zs,
+                        z_hs, *dts, dt.stride(-1), *bs, B.stride(-2), *cs, C.stride(-2), slots, extent(x), z_numel,
+                        extent(dt), extent(B), extent(C))
 
 
 def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
@@ -250,32 +305,34 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     Returns y (x's shape and dtype) and the float32 states after each
     sequence."""
     what = "selective_scan"
-    nseq, T, cu = _sequences(what, x, cu_seqlens, 4)
-    packed = cu is not None
-    lead = (T,) if packed else (nseq, T)
-    d, x, dt, A, B, C, D, z, dt_bias = _scan_desc(what, lead, x, dt, A, B, C, D, z, dt_bias, dt_softplus)
-    of_type(what, torch.float32, initial_state=initial_state)
-    of_shape(what, initial_state=(initial_state, (nseq, d.H, d.P, d.N)))
-    no_grad(what, initial_state)
-    dev = same_gpu(what, x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, initial_state=initial_state,
-                   cu_seqlens=cu)
-    first = None if initial_state is None else initial_state.contiguous()
-    d.nseq, d.T = nseq, T
-    d.x_bs, d.x_ts = _lead(x, packed)
-    d.dt_bs, d.dt_ts = _lead(dt, packed)
-    d.b_bs, d.b_ts = _lead(B, packed)
-    d.c_bs, d.c_ts = _lead(C, packed)
-    if z is not None:
-        d.z_bs, d.z_ts = _lead(z, packed)
-    core = lib()
-    with torch.cuda.device(dev):
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        state = torch.empty((nseq, d.H, d.P, d.N), dtype=torch.float32, device=dev)
-        ws_bytes = core.pe_selective_scan_workspace_bytes(ctypes.byref(d), packed)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        rc = core.pe_selective_scan(ctypes.byref(d), _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z),
-                                    _ptr(dt_bias), _ptr(first), _ptr(cu), _ptr(y), _ptr(state), _ptr(ws), ws_bytes,
-                                    runtime.raw_stream(dev.index))
+    key = (what, layout(x), layout(dt), layout(A), layout(B), layout(C), layout(D), layout(z), layout(dt_bias),
+           bool(dt_softplus), layout(initial_state), layout(cu_seqlens))
+    plan = _plans.get(key)
+    if plan is None:
+        nseq, T, cu = _sequences(what, x, cu_seqlens, 4)
+        packed = cu is not None
+        given = (x, dt, A, B, C, D, z, dt_bias)
+        (H, P, G, N), laid = _scan_operands(what, (T,) if packed else (nseq, T), *given)
+        check(what, "initial_state", initial_state, (nseq, H, P, N), torch.float32)
+        ready(what, *given, initial_state, cu)
+        first = dense(initial_state)
+        if any(g is not t for g, t in zip((*given, initial_state, cu_seqlens), (*laid, first, cu))):
+            x, dt, A, B, C, D, z, dt_bias = laid
+            return selective_scan(x, dt, A, B, C, D=D, z=z, dt_bias=dt_bias, dt_softplus=dt_softplus,
+                                  initial_state=first, cu_seqlens=cu)
+        d = _scan_desc(x, dt, B, C, z, bool(dt_softplus), nseq, T, H, P, G, N, 0,
+                       (lambda t: (0, t.stride(0))) if packed else (lambda t: t.stride()[:2]))
+        plan = remember(key, (d, (nseq, H, P, N), lib().pe_selective_scan_workspace_bytes(ctypes.byref(d), packed)))
+    d, state_shape, ws_bytes = plan
+    dev = ready(what, x, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens)
+    with on(dev):
+        y = x.new_empty(x.shape)
+        state = A.new_empty(state_shape)
+        ws = A.new_empty(ws_bytes // 4) if ws_bytes else None
+        rc = lib().pe_selective_scan(ctypes.byref(d), x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(),
+                                     C.data_ptr(), _ptr(D), _ptr(z), _ptr(dt_bias), _ptr(initial_state),
+                                     _ptr(cu_seqlens), y.data_ptr(), state.data_ptr(), _ptr(ws), ws_bytes,
+                                     runtime.raw_stream(dev))
     runtime.check(rc, "pe_selective_scan")
     return y, state
 
@@ -291,23 +348,29 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     slot outside [0, S) marks a row without a sequence, whose output is zero.
     Returns y [n, H, P] of x's dtype."""
     what = "selective_scan_step"
-    if x.dim() != 3:
-        raise ValueError(f"{what}: x must be [n, H, P], got shape {tuple(x.shape)}")
-    n = x.shape[0]
-    d, x, dt, A, B, C, D, z, dt_bias = _scan_desc(what, (n,), x, dt, A, B, C, D, z, dt_bias, dt_softplus)
-    of_type(what, torch.float32, state=state)
-    d.nslots = _cache(what, state, (d.H, d.P, d.N), n, slots)
-    slots = _index(what, "slots", slots, n)
-    no_grad(what, state)
-    dev = same_gpu(what, x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, state=state, slots=slots)
-    d.nseq = n
-    d.x_bs, d.dt_bs, d.b_bs, d.c_bs = x.stride(0), dt.stride(0), B.stride(0), C.stride(0)
-    if z is not None:
-        d.z_bs = z.stride(0)
-    with torch.cuda.device(dev):
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        rc = lib().pe_selective_scan_step(ctypes.byref(d), _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D),
-                                          _ptr(z), _ptr(dt_bias), _ptr(state), _ptr(slots), _ptr(y),
-                                          runtime.raw_stream(dev.index))
+    key = (what, layout(x), layout(dt), layout(A), layout(B), layout(C), layout(state), layout(D), layout(z),
+           layout(dt_bias), bool(dt_softplus), layout(slots))
+    d = _plans.get(key)
+    if d is None:
+        if x.dim() != 3:
+            raise ValueError(f"{what}: x must be [n, H, P], got shape {tuple(x.shape)}")
+        n = x.shape[0]
+        given = (x, dt, A, B, C, D, z, dt_bias)
+        (H, P, G, N), laid = _scan_operands(what, (n,), *given)
+        S = _cache(what, state, (H, P, N), torch.float32, n, slots)
+        at = _index(what, "slots", slots, n)
+        ready(what, *given, state, slots)
+        if any(g is not t for g, t in zip((*given, slots), (*laid, at))):
+            x, dt, A, B, C, D, z, dt_bias = laid
+            return selective_scan_step(x, dt, A, B, C, state, D=D, z=z, dt_bias=dt_bias, dt_softplus=dt_softplus,
+                                       slots=at)
+        d = remember(key, _scan_desc(x, dt, B, C, z, bool(dt_softplus), n, 0, H, P, G, N, S,
+                                     lambda t: (t.stride(0), 0)))
+    dev = ready(what, x, dt, A, B, C, D, z, dt_bias, state, slots)
+    with on(dev):
+        y = x.new_empty(x.shape)
+        rc = lib().pe_selective_scan_step(ctypes.byref(d), x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(),
+                                          C.data_ptr(), _ptr(D), _ptr(z), _ptr(dt_bias), state.data_ptr(), _ptr(slots),
+                                          y.data_ptr(), runtime.raw_stream(dev))
     runtime.check(rc, "pe_selective_scan_step")
     return y
