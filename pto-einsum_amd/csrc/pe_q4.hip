@@ -4,10 +4,12 @@
 //
 // Reading the weights once bounds it, half a byte each.  A wave owns 16 NT weight
 // rows and a range of K; the block's waves split K and add their parts in LDS in
-// a fixed order.  A step covers 256 k: a lane loads a quarter of each group of
-// one row (4, 8 or 16 bytes) for all of them at once, so that a step's weights,
-// scales and x are in flight together and matrix-core operands are whole words of
-// what was loaded; the order of k inside a group is the same for x.
+// a fixed order.  A step covers 128 k: its weights, scales and x are loaded as they
+// lie, 16 bytes a lane and rows contiguous over lanes, while the step before is
+// worked on, and pass through LDS of the wave's own to the lanes that feed them to
+// the matrix cores.  (Loaded straight in that order, where neighbouring lanes have
+// different rows, every lane's 8 bytes cost a look-up of their own: 16 tokens
+// 16384 x 8192 took 34 us.)
 //
 // Weights become operands without an inexact step: q is a whole number, exact in
 // 16 bits, so a group's sum Q = sum q x and X = sum x (a product with ones, once
@@ -28,18 +30,10 @@ namespace pe {
 namespace ssm {
 namespace {
 
-// Waves of a block: 16 where a wave's registers (128 then) hold a step.
-// Whether registers hold two steps.
+constexpr int kStep = 128;
+// Waves of a block: what its LDS holds.
 template <typename E, int MT, int NT>
-constexpr bool kPairs = E::kBytes == 2 && MT * NT >= 2 && MT < 4;
-template <typename E, int MT, int NT>
-constexpr int kWaves = MT * NT == 1 ? 16 : 8;
-// k of a step: a float32 step of 256 would be twice the code and registers.
-template <typename E>
-constexpr int kStep = E::kBytes == 4 ? 128 : 256;
-#ifndef PE_Q4_TILES
-#define PE_Q4_TILES 4
-#endif
+constexpr int kWaves = E::kBytes == 4 ? (MT == 1 ? 8 : 4) : MT * NT == 1 ? 16 : 8;
 
 struct Q4Args {
     const void* x;
@@ -107,184 +101,163 @@ __device__ __forceinline__ bf16x8 weights(F32, uint32_t w) {
     return __builtin_bit_cast(bf16x8, t);
 }
 
-// Eight elements of x as loaded, and as operand terms in the weights' order.
-template <typename E>
-struct XVec {
-    u32x4 v;
-    __device__ __forceinline__ void load(const typename E::T* p) {
-        typedef u32x4 uv __attribute__((aligned(2)));
-        v = *reinterpret_cast<const uv*>(p);
-    }
-    // The first `by` elements dropped, zeros moved in.
-    __device__ __forceinline__ void drop(int by) {
-        if (by & 1)
+// Eight elements of x as operand terms in the weights' order.
+__device__ __forceinline__ void operand(const _Float16* p, f16x8 (&o)[1]) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+    u32x4 t;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = (v[i] >> 16) | (i < 3 ? v[(i + 1) & 3] << 16 : 0u);
-        if (by & 2) v = u32x4{v[1], v[2], v[3], 0};
-        if (by & 4) v = u32x4{v[2], v[3], 0, 0};
-        if (by & 8) v = u32x4{0, 0, 0, 0};
-    }
-    __device__ __forceinline__ void set(int i, typename E::T x) {
-        const uint32_t b = __builtin_bit_cast(uint16_t, x);
-        v[i / 2] = (i & 1) ? (v[i / 2] & 0xffffu) | (b << 16) : (v[i / 2] & 0xffff0000u) | b;
-    }
-    __device__ __forceinline__ void operand(typename Mma<E>::V8 (&o)[1]) const {
-        u32x4 t;
+    for (int i = 0; i < 4; ++i)   // elements i and i + 4
+        t[i] = __builtin_amdgcn_perm(v[2 + i / 2], v[i / 2], (i & 1) ? 0x07060302u : 0x05040100u);
+    o[0] = __builtin_bit_cast(f16x8, t);
+}
+__device__ __forceinline__ void operand(const __bf16* p, bf16x8 (&o)[1]) {
+    f16x8 t[1];
+    operand(reinterpret_cast<const _Float16*>(p), t);
+    o[0] = __builtin_bit_cast(bf16x8, t[0]);
+}
+__device__ __forceinline__ void operand(const float* p, bf16x8 (&o)[3]) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)   // elements i and i + 4
-            t[i] = __builtin_amdgcn_perm(v[2 + i / 2], v[i / 2], (i & 1) ? 0x07060302u : 0x05040100u);
-        o[0] = __builtin_bit_cast(typename Mma<E>::V8, t);
+    for (int i = 0; i < 8; ++i) {
+        float r = i < 4 ? a[i & 3] : b[i & 3];
+        o[0][i] = (__bf16)r;
+        r -= (float)o[0][i];
+        o[1][i] = (__bf16)r;
+        r -= (float)o[1][i];
+        o[2][i] = (__bf16)r;
     }
-};
-template <>
-struct XVec<F32> {
-    float v[8];
-    __device__ __forceinline__ void load(const float* p) {
-        typedef f32x4 uv __attribute__((aligned(4)));
-        const f32x4 a = *reinterpret_cast<const uv*>(p), b = *reinterpret_cast<const uv*>(p + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = a[i];
-            v[4 + i] = b[i];
-        }
-    }
-    __device__ __forceinline__ void drop(int by) {
-#pragma unroll
-        for (int s = 1; s <= 8; s *= 2)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = (by & s) ? (i + s < 8 ? v[(i + s) & 7] : 0.0f) : v[i];
-    }
-    __device__ __forceinline__ void set(int i, float x) { v[i] = x; }
-    __device__ __forceinline__ void operand(bf16x8 (&o)[3]) const {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float r = v[i];
-            o[0][i] = (__bf16)r;
-            r -= (float)o[0][i];
-            o[1][i] = (__bf16)r;
-            r -= (float)o[1][i];
-            o[2][i] = (__bf16)r;
-        }
-    }
-};
+}
 
-// The word at byte `at` of a row; bytes past its end are anything.
-__device__ __forceinline__ uint32_t last_word(const uint8_t* row, int at, int bytes) {
-    typedef uint32_t u1 __attribute__((aligned(1)));
-    if (bytes >= 4) {
-        const int from = min(at, bytes - 4);
-        return *reinterpret_cast<const u1*>(row + from) >> (8 * min(3, at - from));
-    }
-    uint32_t v = 0;
+// 16 bytes of a row at byte `at`, those past its end 0.
+typedef u32x4 LooseVec __attribute__((aligned(1)));
+__device__ __forceinline__ u32x4 last_vec(const uint8_t* row, int64_t at, int64_t bytes) {
+    u32x4 v = {0, 0, 0, 0};
+    if (bytes >= 16) {
+        // a vector that starts earlier, moved into place
+        const int64_t from = min(at, bytes - 16);
+        const int by = int(min(int64_t(16), at - from));
+        v = *reinterpret_cast<const LooseVec*>(row + from);
+        if (by & 16) v = u32x4{0, 0, 0, 0};
+        if (by & 8) v = u32x4{v[2], v[3], 0, 0};
+        if (by & 4) v = u32x4{v[1], v[2], v[3], 0};
+        const int bits = 8 * (by & 3);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) v |= uint32_t(row[min(at + b, bytes - 1)]) << (8 * b);
+        for (int i = 0; i < 4; ++i)
+            v[i] = uint32_t((uint64_t(v[i]) | (i < 3 ? uint64_t(v[(i + 1) & 3]) << 32 : 0)) >> bits);
+        return v;
+    }
+    for (int b = 0; b < 16; ++b)
+        if (at + b < bytes) v[b / 4] |= uint32_t(row[at + b]) << (8 * (b & 3));
     return v;
 }
 
-// One step's operands.  GW words of a row's group belong to a lane.
 template <typename E, int GROUP, int MT, int NT>
-struct Step {
+struct Wave {
     using T = typename E::T;
-    static constexpr int kGroups = kStep<E> / GROUP, GW = GROUP / 32;
-    typedef uint32_t Words __attribute__((ext_vector_type(GW)));
-    typedef uint32_t LooseWords __attribute__((ext_vector_type(GW), aligned(1)));
-    Words w[NT][kGroups];
-    // Scales and zero points, packed as they lie in memory.
-    static constexpr int kSW = kGroups * E::kBytes / 4;
-    typedef uint32_t Pack __attribute__((ext_vector_type(kSW)));
-    typedef uint32_t LoosePack __attribute__((ext_vector_type(kSW), aligned(E::kBytes)));
-    Pack scale[NT], zero[NT];
-    __device__ __forceinline__ static float value(const Pack& p, int j) {
-        if constexpr (E::kBytes == 4) return __uint_as_float(p[j]);
-        else return E::to_f32(__builtin_bit_cast(T, uint16_t(p[j / 2] >> (16 * (j & 1)))));
-    }
-    __device__ __forceinline__ static Pack gather(const T* p, int64_t row, int g0, int groups) {
-        Pack o = {};
-#pragma unroll
-        for (int j = 0; j < kGroups; ++j) {
-            const T v = p[row + min(g0 + j, groups - 1)];
-            if constexpr (E::kBytes == 4) o[j] = __float_as_uint(v);
-            else o[j / 2] |= uint32_t(__builtin_bit_cast(uint16_t, v)) << (16 * (j & 1));
-        }
-        return o;
-    }
-    // x of one tile comes with the weights; of several, a vector at a time as it
-    // is used (the registers would not hold it).
-    static constexpr bool kAhead = MT == 1;
-    XVec<E> x[kAhead ? kGroups : 1][kAhead ? GW : 1];
+    static constexpr int kGroups = kStep / GROUP, GW = GROUP / 32, kRows = 16 * NT, kXRows = 16 * MT;
+    static constexpr int kWP = kStep / 2 + 16, kXP = kStep + 16 / E::kBytes;   // pitches: bytes, elements
+    static constexpr int kXVecs = kStep * E::kBytes / 16;                      // of a row of x
+    static constexpr int kXEach = kXRows * kXVecs / 64;
+    // Scales and zero points of a row: kGroups of each.
+    typedef typename Vec<E, kGroups>::utype LooseScales;
 
-    // FULL: all of the step's k are there.  Loads take clamped addresses else,
-    // and x is 0 past K (a weight there does not count then, nor does a scale).
+    struct Lds {
+        alignas(16) uint8_t w[kRows * kWP];
+        alignas(16) T x[kXRows * kXP];
+        float scale[kGroups][kRows], zero[kGroups][kRows];
+    };
+
+    // A step's weights and scales in registers.  Lane l: weight rows l / 4 + 16 t,
+    // 16 bytes each; scales and zero points of row l.
+    struct Weights {
+        u32x4 w[NT];
+        typename Vec<E, kGroups>::type scale, zero;
+    };
+    u32x4 x[kXEach];
+
     template <bool FULL>
-    __device__ __forceinline__ void load(const Q4Args& g, const uint8_t* const (&wrow)[NT], const int64_t (&srow)[NT],
-                                         const T* const (&xrow)[MT], const bool (&there)[MT], int k0, int lg) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int j = 0; j < kGroups; ++j) {
-                const int at = (k0 + j * GROUP) / 2 + lg * (GROUP / 8);
-                if constexpr (FULL) {
-                    w[t][j] = *reinterpret_cast<const LooseWords*>(wrow[t] + at);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < GW; ++i) w[t][j][i] = last_word(wrow[t], at + 4 * i, g.row_bytes);
-                }
-            }
-        const int g0 = k0 / GROUP;
-        const T *sp = static_cast<const T*>(g.scales), *zp = static_cast<const T*>(g.zeros);
+    __device__ __forceinline__ static void load(Weights& o, const Q4Args& g, int n0, int k0, int lane) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            zero[t] = Pack{};
+            const uint8_t* row = g.packed + int64_t(min(n0 + 16 * t + lane / 4, g.N - 1)) * g.row_bytes;
+            const int at = k0 / 2 + 16 * (lane & 3);
+            if constexpr (FULL) o.w[t] = *reinterpret_cast<const LooseVec*>(row + at);
+            else o.w[t] = last_vec(row, at, g.row_bytes);
+        }
+        if (lane < kRows) {
+            const int64_t at = int64_t(min(n0 + lane, g.N - 1)) * g.groups + k0 / GROUP;
+            const T *sp = static_cast<const T*>(g.scales) + at, *zp = static_cast<const T*>(g.zeros) + at;
             if constexpr (FULL) {
-                scale[t] = *reinterpret_cast<const LoosePack*>(sp + srow[t] + g0);
-                if (zp) zero[t] = *reinterpret_cast<const LoosePack*>(zp + srow[t] + g0);
+                o.scale = *reinterpret_cast<const LooseScales*>(sp);
+                if (g.zeros) o.zero = *reinterpret_cast<const LooseScales*>(zp);
             } else {
-                scale[t] = gather(sp, srow[t], g0, g.groups);
-                if (zp) zero[t] = gather(zp, srow[t], g0, g.groups);
+#pragma unroll
+                for (int j = 0; j < kGroups; ++j) {
+                    const int i = min(j, g.groups - 1 - k0 / GROUP);
+                    o.scale[j] = sp[i];
+                    if (g.zeros) o.zero[j] = zp[i];
+                }
             }
         }
-        if constexpr (kAhead)
-#pragma unroll
-            for (int j = 0; j < kGroups; ++j)
-#pragma unroll
-                for (int i = 0; i < GW; ++i) load_x<FULL>(g, x[j][i], xrow[0], there[0], k0, j, i, lg);
     }
 
     template <bool FULL>
-    __device__ __forceinline__ static void load_x(const Q4Args& g, XVec<E>& v, const T* row, bool there, int k0, int j,
-                                                  int i, int lg) {
-        const int k = k0 + j * GROUP + lg * (GROUP / 4) + 8 * i;
-        if constexpr (FULL) {
-            v.load(row + k);
-        } else {
-            // A vector that starts earlier, moved into place; or element by element.
-            if (g.K >= 8) {
-                const int from = min(k, g.K - 8);
-                v.load(row + from);
-                v.drop(there ? min(8, k - from) : 8);
-            } else {
+    __device__ __forceinline__ void load_x(const Q4Args& g, int m0, int k0, int lane) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const T u = row[min(k + e, g.K - 1)];
-                    v.set(e, there && k + e < g.K ? u : T(0.0f));
-                }
+        for (int i = 0; i < kXEach; ++i) {
+            const int v = lane + 64 * i, m = m0 + v / kXVecs, vec = v % kXVecs;
+            const int64_t at = int64_t(k0) * E::kBytes + vec * 16;
+            if (m0 + 64 * i / kXVecs < g.M) {
+                const uint8_t* row = reinterpret_cast<const uint8_t*>(static_cast<const T*>(g.x) +
+                                                                      int64_t(min(m, g.M - 1)) * g.x_ms);
+                if constexpr (FULL) x[i] = *reinterpret_cast<const LooseVec*>(row + at);
+                else x[i] = last_vec(row, at, int64_t(g.K) * E::kBytes);
             }
+        }
+    }
+
+    // Rows of x past M stay 0.
+    __device__ __forceinline__ static void clear(const Q4Args& g, Lds& m, int m0, int lane) {
+        constexpr int kVecs = kXRows * kXP * E::kBytes / 16;
+        if (m0 + kXRows > g.M)
+            for (int i = lane; i < kVecs; i += 64) reinterpret_cast<u32x4*>(m.x)[i] = u32x4{0, 0, 0, 0};
+    }
+
+    __device__ __forceinline__ void store(const Weights& o, const Q4Args& g, Lds& m, int m0, int lane) const {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            *reinterpret_cast<u32x4*>(m.w + (16 * t + lane / 4) * kWP + 16 * (lane & 3)) = o.w[t];
+        if (lane < kRows)
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j) {
+                m.scale[j][lane] = E::to_f32(o.scale[j]);
+                m.zero[j][lane] = (g.zeros ? E::to_f32(o.zero[j]) : 8.0f) + Mma<E>::kOffset;
+            }
+#pragma unroll
+        for (int i = 0; i < kXEach; ++i) {
+            const int v = lane + 64 * i;
+            if (m0 + v / kXVecs < g.M)
+                *reinterpret_cast<u32x4*>(m.x + v / kXVecs * kXP + v % kXVecs * (16 / E::kBytes)) = x[i];
         }
     }
 
     // acc[m][t]: rows m = 4 lg + element, column n = lr.
-    template <bool FULL>
-    __device__ __forceinline__ void apply(const Q4Args& g, const T* const (&xrow)[MT], const bool (&there)[MT], int k0,
-                                          int lg, f32x4 (&acc)[MT][NT]) const {
+    __device__ __forceinline__ static void apply(const Q4Args& g, const Lds& l, int lane, f32x4 (&acc)[MT][NT]) {
         using V8 = typename Mma<E>::V8;
         constexpr int kTerms = Mma<E>::kTerms;
+        const int lr = lane & 15, lg = lane >> 4;
         V8 ones;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ones[i] = (typename std::remove_reference<decltype(ones[0])>::type)1.0f;
         const bool with_x = g.zeros || Mma<E>::kOffset != -8.0f;
 #pragma unroll
         for (int j = 0; j < kGroups; ++j) {
+            typedef uint32_t Words __attribute__((ext_vector_type(GW)));
             f32x4 q[MT][NT], xs[MT];
+            Words w[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                w[t] = *reinterpret_cast<const Words*>(l.w + (16 * t + lr) * kWP + j * (GROUP / 2) + lg * (GROUP / 8));
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 xs[m] = f32x4{0, 0, 0, 0};
@@ -296,20 +269,14 @@ struct Step {
                 V8 o[MT][kTerms];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    if constexpr (kAhead) {
-                        x[j][i].operand(o[m]);
-                    } else {
-                        XVec<E> v;
-                        load_x<FULL>(g, v, xrow[m], there[m], k0, j, i, lg);
-                        v.operand(o[m]);
-                    }
+                    operand(l.x + (16 * m + lr) * kXP + j * GROUP + lg * (GROUP / 4) + 8 * i, o[m]);
                     if (with_x)
 #pragma unroll
                         for (int c = kTerms - 1; c >= 0; --c) xs[m] = mma(o[m][c], ones, xs[m]);
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const V8 wv = weights(E{}, w[t][j][i]);
+                    const V8 wv = weights(E{}, w[t][i]);
 #pragma unroll
                     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -318,8 +285,7 @@ struct Step {
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const float s = value(scale[t], j);
-                const float z = (g.zeros ? value(zero[t], j) : 8.0f) + Mma<E>::kOffset;
+                const float s = l.scale[j][16 * t + lr], z = l.zero[j][16 * t + lr];
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -328,8 +294,6 @@ struct Step {
                         acc[m][t][e] = __builtin_fmaf(s, v, acc[m][t][e]);
                     }
             }
-            // One group's operands at a time: unpacked ahead, they do not fit.
-            if constexpr (MT * NT > 1) __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
@@ -337,68 +301,65 @@ struct Step {
 template <typename E, int GROUP, int MT, int NT>
 __global__ __launch_bounds__(64 * (kWaves<E, MT, NT>)) void q4_kernel(Q4Args g) {
     using T = typename E::T;
+    using W = Wave<E, GROUP, MT, NT>;
     constexpr int kPitch = 16 * NT + 1;
-    __shared__ float part[kWaves<E, MT, NT>][16 * MT][kPitch];
+    __shared__ union {
+        typename W::Lds wave[kWaves<E, MT, NT>];
+        float part[kWaves<E, MT, NT>][16 * MT][kPitch];
+    } m;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = int(blockDim.x) >> 6, lr = lane & 15, lg = lane >> 4;
     const int n0 = int(blockIdx.x) * 16 * NT, m0 = int(blockIdx.y) * 16 * MT;
-    const uint8_t* wrow[NT];
-    int64_t srow[NT];
-    const T* xrow[MT];
-    bool there[MT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int64_t n = min(n0 + 16 * t + lr, g.N - 1);
-        wrow[t] = g.packed + n * g.row_bytes;
-        srow[t] = n * g.groups;
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        there[m] = m0 + 16 * m + lr < g.M;
-        xrow[m] = static_cast<const T*>(g.x) + int64_t(min(m0 + 16 * m + lr, g.M - 1)) * g.x_ms;
-    }
     f32x4 acc[MT][NT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0, 0, 0, 0};
+        for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
 
-    const int first = wave * g.steps, all = (g.K + kStep<E> - 1) / kStep<E>, last = min(first + g.steps, all);
-    const int full = min(last, g.K / kStep<E>);
-    Step<E, GROUP, MT, NT> s;
-    if constexpr (kPairs<E, MT, NT>) {
-        // While a step is worked on, the next one's operands are on their way.
-        Step<E, GROUP, MT, NT> u;
-        if (first < full) s.template load<true>(g, wrow, srow, xrow, there, first * kStep<E>, lg);
-        for (int i = first; i < full; i += 2) {
-            if (i + 1 < full) u.template load<true>(g, wrow, srow, xrow, there, (i + 1) * kStep<E>, lg);
-            s.template apply<true>(g, xrow, there, i * kStep<E>, lg, acc);
-            if (i + 1 >= full) break;
-            if (i + 2 < full) s.template load<true>(g, wrow, srow, xrow, there, (i + 2) * kStep<E>, lg);
-            u.template apply<true>(g, xrow, there, (i + 1) * kStep<E>, lg, acc);
-        }
-    } else {
-        for (int i = first; i < full; ++i) {
-            s.template load<true>(g, wrow, srow, xrow, there, i * kStep<E>, lg);
-            s.template apply<true>(g, xrow, there, i * kStep<E>, lg, acc);
-        }
+    // Steps of this wave; the last of all may be one of less than kStep.
+    const int first = wave * g.steps, last = min(first + g.steps, (g.K + kStep - 1) / kStep);
+    W s;
+    typename W::Weights even, odd;
+    auto load = [&](typename W::Weights& o, int i) __attribute__((always_inline)) {
+        if (i >= last) return;
+        if ((i + 1) * int64_t(kStep) <= g.K) W::template load<true>(o, g, n0, i * kStep, lane);
+        else W::template load<false>(o, g, n0, i * kStep, lane);
+    };
+    auto load_x = [&](int i) __attribute__((always_inline)) {
+        if (i >= last) return;
+        if ((i + 1) * int64_t(kStep) <= g.K) s.template load_x<true>(g, m0, i * kStep, lane);
+        else s.template load_x<false>(g, m0, i * kStep, lane);
+    };
+    // Weights are loaded two steps ahead (memory answers later than a step takes),
+    // x, which comes from a cache, one.
+    auto step = [&](typename W::Weights& o, int i) __attribute__((always_inline)) {
+        s.store(o, g, m.wave[wave], m0, lane);
+        load_x(i + 1);
+        load(o, i + 2);
+        // The wave's own LDS: its operations are carried out in order.
+        W::apply(g, m.wave[wave], lane, acc);
+    };
+    load(even, first);
+    load_x(first);
+    load(odd, first + 1);
+    W::clear(g, m.wave[wave], m0, lane);
+    for (int i = first; i < last; i += 2) {
+        step(even, i);
+        if (i + 1 < last) step(odd, i + 1);
     }
-    if (full < last && full >= first) {
-        s.template load<false>(g, wrow, srow, xrow, there, full * kStep<E>, lg);
-        s.template apply<false>(g, xrow, there, full * kStep<E>, lg, acc);
-    }
+    __syncthreads();
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) part[wave][16 * m + 4 * lg + e][16 * t + lr] = acc[m][t][e];
+            for (int e = 0; e < 4; ++e) m.part[wave][16 * i + 4 * lg + e][16 * t + lr] = acc[i][t][e];
     __syncthreads();
     for (int at = threadIdx.x; at < 256 * MT * NT; at += blockDim.x) {
-        const int m = at / (16 * NT), n = at % (16 * NT);
+        const int row = at / (16 * NT), n = at % (16 * NT);
         float v = 0.0f;
-        for (int w = 0; w < waves; ++w) v += part[w][m][n];
-        if (m0 + m < g.M && n0 + n < g.N) static_cast<T*>(g.y)[int64_t(m0 + m) * g.N + n0 + n] = (T)v;
+        for (int w = 0; w < waves; ++w) v += m.part[w][row][n];
+        if (m0 + row < g.M && n0 + n < g.N) static_cast<T*>(g.y)[int64_t(m0 + row) * g.N + n0 + n] = (T)v;
     }
 }
 
@@ -409,10 +370,10 @@ int launch(Q4Args g, hipStream_t stream) {
     const int mt = g.M <= 16 ? 1 : g.M <= 32 ? 2 : 4;
     const int64_t tall = ceil_div(g.M, 16 * mt);
     int nt = 1;
-    while (2 * nt * mt <= PE_Q4_TILES && ceil_div(g.N, 32 * nt) * tall >= cu_count()) nt *= 2;
+    while (2 * nt * mt <= 4 && ceil_div(g.N, 32 * nt) * tall >= cu_count()) nt *= 2;
     auto run = [&](auto m, auto n) {
         constexpr int MT = m(), NT = n();
-        const int steps = int(ceil_div(g.K, kStep<E>));
+        const int steps = int(ceil_div(g.K, kStep));
         g.steps = std::max(1, int(ceil_div(steps, kWaves<E, MT, NT>)));
         const int waves = std::max(1, int(ceil_div(steps, g.steps)));
         const int64_t cols = ceil_div(g.N, 16 * NT);
