@@ -6,8 +6,8 @@
 // Reading x and writing y bound it: 2 W flops for two elements moved.  A thread
 // owns V channels (16 bytes) and walks a run of consecutive tokens with the
 // last W - 1 inputs in registers, so x is read once but for W - 1 tokens at the
-// run's start; the loads of a group of tokens are issued together.  Sums are
-// float32 in the order of j after the bias; the output is rounded once.
+// run's start.  A group of tokens is loaded while the one before is worked on.
+// Sums are float32 in the order of j after the bias; the output is rounded once.
 #include "pe_ssm.h"
 
 #include <algorithm>
@@ -37,7 +37,25 @@ template <typename E, int W, int V>
 struct Taps {
     float w[W][V], b[V];
     __device__ __forceinline__ void load(const ConvArgs& g, int64_t d, int n) {
-        const typename E::T* wp = static_cast<const typename E::T*>(g.w) + d * W;
+        using T = typename E::T;
+        const T* wp = static_cast<const T*>(g.w) + d * W;
+        if (n >= V) {
+            T all[W * V];
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const typename Vec<E, V>::utype v = *reinterpret_cast<const typename Vec<E, V>::utype*>(wp + j * V);
+#pragma unroll
+                for (int i = 0; i < V; ++i) all[j * V + i] = v[i];
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                b[i] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < W; ++j) w[j][i] = E::to_f32(all[i * W + j]);
+            }
+            if (g.bias) load_f32<E, V>(static_cast<const T*>(g.bias) + d, n, b);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
 #pragma unroll
@@ -102,7 +120,9 @@ __global__ __launch_bounds__(kThreads) void conv_kernel(ConvArgs g) {
     const uint32_t at = blockIdx.x * kThreads + threadIdx.x;
     const uint32_t row = at / g.vecs, vec = at - row * g.vecs;
     if (row >= g.rows) return;
-    const int64_t d = int64_t(vec) * V;
+    // The last channels' thread takes V of them all the same, some of which its
+    // neighbour computes too (and both write the same).
+    const int64_t d = g.D < V ? 0 : min(int64_t(vec) * V, g.D - V);
     const int n = int(g.D - d < V ? g.D - d : V);
     const T* x = static_cast<const T*>(g.x) + d;
     T* y = static_cast<T*>(g.y) + d;
@@ -161,15 +181,33 @@ __global__ __launch_bounds__(kThreads) void conv_kernel(ConvArgs g) {
         const T* xs = x + first * g.x_ts;
         history<E, W, V>(g, xs, s, t - first, d, n, h);
         const int64_t stop = last < end ? last : end;
-        for (; t + U <= stop; t += U) {
-            float v[U][V], o[V];
+        if (n >= V) {
+            typename Vec<E, V>::type even[U], odd[U];
+            auto load = [&](typename Vec<E, V>::type (&v)[U], int64_t at) __attribute__((always_inline)) {
+                if (at + U <= stop)
 #pragma unroll
-            for (int u = 0; u < U; ++u) load_f32<E, V>(x + (t + u) * g.x_ts, n, v[u]);
+                    for (int u = 0; u < U; ++u)
+                        v[u] = *reinterpret_cast<const typename Vec<E, V>::utype*>(x + (at + u) * g.x_ts);
+            };
+            auto work = [&](const typename Vec<E, V>::type (&r)[U]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                taps.apply(h, v[u], g.silu, o);
-                push<W, V>(h, v[u]);
-                store_f32<E, V>(y + (t + u) * g.D, n, o);
+                for (int u = 0; u < U; ++u) {
+                    float v[V], o[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[i] = E::to_f32(r[u][i]);
+                    taps.apply(h, v, g.silu, o);
+                    push<W, V>(h, v);
+                    store_f32<E, V>(y + (t + u) * g.D, V, o);
+                }
+                t += U;
+            };
+            load(even, t);
+            while (t + U <= stop) {
+                load(odd, t + U);
+                work(even);
+                if (t + U > stop) break;
+                load(even, t + U);
+                work(odd);
             }
         }
         for (; t < stop; ++t) {
@@ -261,9 +299,12 @@ extern "C" int pe_causal_conv(const pe_conv_desc* d, const void* x, const void* 
     return with_type(d->dtype, [&](auto e) {
         using E = decltype(e);
         return with_width(d->width, [&](auto w) {
-            constexpr int W = w(), V = 16 / E::kBytes, U = 8;
+            constexpr int W = w(), V = 16 / E::kBytes, U = 4;
             g.vecs = uint32_t(ceil_div(d->D, V));
+            // Tokens a thread walks: of longer runs fewer inputs are read twice,
+            // shorter ones make more threads (some four waves for each SIMD).
             g.run = 32;
+            while (g.run > 8 && __int128(ceil_div(d->T, g.run)) * (cu ? 1 : d->nseq) * g.vecs < 1 << 18) g.run /= 2;
             g.runs = uint32_t(ceil_div(d->T, g.run));
             const int64_t rows = (cu ? int64_t(g.runs) : int64_t(g.runs) * d->nseq) +
                                  (cu || d->T == 0 ? d->nseq : 0);
