@@ -75,19 +75,24 @@ Plan plan_of(const pe_scan_desc& d, bool packed) {
     // Tiles of up to 64 rows p, as even as waves of 16 allow.
     p.ptiles = ceil_div(d.P, 64);
     p.waves = int(std::max<int64_t>(p.nt == 256 ? 3 : 2, ceil_div(ceil_div(d.P, 16), p.ptiles)));
-    // Pieces of a sequence (packed: of the whole buffer).  What a choice costs, in
-    // chunks of 32 tokens that a block walks: those of a piece and one for its
-    // start, in as many rounds as the blocks need; half of that again for the
-    // pieces' contributions, and 6 for the states of 1000 blocks of 64 x 128.
+    // Pieces of a sequence (packed: of the whole buffer), of 64 tokens at least.
+    // What a choice costs, in chunks of 32 tokens that a block walks: those of a
+    // piece and one for its start, in as many rounds as the blocks need; with
+    // several pieces half of that again for their contributions, 6 for the states
+    // of 1000 blocks of 64 x 128, and 2 for two launches more.  Measured, us for 1, 2,
+    // 4, 8, 16 pieces (chosen: *): 1 x 128 tokens, 32 heads 17* 20 20; 2 x 256, 16
+    // heads 28 27 22* 25; 1 x 1024, 32 heads 105 76 47 39 38*; 2 x 4096, 64 heads 404
+    // 270 182 179 184, 161 for 6*; 1 x 16384, 24 heads 1400 920 468 243 162, 121 for
+    // 32* (64 x 128 a head, 16-bit types).
     const int64_t seqs = packed ? 1 : d.nseq, across = d.H * p.ptiles, chunks = ceil_div(d.T, 32);
     const double slots = 256.0 * chunks_of(d.dtype)(nullptr, p.nt, p.waves, true, nullptr);
     double best = 0.0;
-    for (int64_t k = 1; k <= std::min<int64_t>(chunks, 96); ++k) {
+    for (int64_t k = 1; k <= std::max<int64_t>(1, std::min<int64_t>(chunks / 2, 96)); ++k) {
         const int64_t piece = ceil_div(chunks, k);
         if (k > 1 && ceil_div(chunks, k - 1) == piece) continue;
         const double blocks = double(seqs) * double(across) * double(ceil_div(chunks, piece));
         double cost = std::ceil(blocks / slots) * double(piece + 1);
-        if (k > 1) cost = 1.5 * cost + 0.006 * blocks * (p.waves * p.nt / 512.0);
+        if (k > 1) cost = 2.0 + 1.5 * cost + 0.006 * blocks * (p.waves * p.nt / 512.0);
         if (k == 1 || cost < best) {
             best = cost;
             p.piece = 32 * piece;
@@ -117,6 +122,7 @@ __global__ __launch_bounds__(kCarryThreads) void carry_kernel(ChunkArgs g, uint3
     const uint32_t pt = at / vecs, v = at - pt * vecs, lane = v & 63, frag = v >> 6;
     const uint32_t wave = frag / frags, i = frag - wave * frags;
     const int64_t p = int64_t(pt) * 16 * wave_rows + 16 * wave + (lane & 15), n = 16 * i + 4 * (lane >> 4);
+    if (p - (lane & 15) >= a.P || int(16 * i) >= a.N) return;  // beside the state
     int64_t id, count;
     if (a.cu) {
         const int64_t from = offset_of(a.cu, s, a.T), to = offset_of(a.cu, s + 1, a.T);

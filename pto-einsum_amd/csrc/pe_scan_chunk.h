@@ -136,6 +136,21 @@ __device__ __forceinline__ f32x4 mma(const V8 (&a)[NA], const V8 (&b)[NB], f32x4
     return c;
 }
 
+// The same for T tiles at a time: their sums take turns, so that none waits for
+// its own last product.
+template <int T, int NA, int NB, typename V8>
+__device__ __forceinline__ void mma(const V8 (&a)[T][NA], const V8 (&b)[NB], f32x4 (&c)[T]) {
+#pragma unroll
+    for (int o = NA + NB - 2; o >= 0; --o) {
+        if (o > 2) continue;
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (o - i >= 0 && o - i < NB)
+#pragma unroll
+                for (int t = 0; t < T; ++t) c[t] = mfma(a[t][i], b[o - i], c[t]);
+    }
+}
+
 // The two 16-bit values nearest to x (float16: toward zero, what is left over is
 // whole in float32 either way), and x less those.
 __device__ __forceinline__ uint32_t take_term(const bf16x8*, f32x2& x) {
@@ -343,9 +358,10 @@ struct Rows {
     template <int PITCH>
     __device__ __forceinline__ void store_raw(typename E::T* lds, int tokens, int width) {
         trim(tokens, width);
+        const int first = fresh(threadIdx.x);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int v = threadIdx.x + i * THREADS;
+            const int v = first + i * THREADS;
             if (kVecs % THREADS == 0 || v < kVecs) r[i].put(lds + v / (COLS / 8) * PITCH + v % (COLS / 8) * 8);
         }
     }
@@ -354,9 +370,10 @@ struct Rows {
     template <bool SPLIT = false>
     __device__ __forceinline__ void store(uint16_t* lds, int tokens, int width) {
         trim(tokens, width);
+        const int first = fresh(threadIdx.x);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int v = threadIdx.x + i * THREADS;
+            const int v = first + i * THREADS;
             if (kVecs % THREADS == 0 || v < kVecs) {
                 u32x4 t[Scheme<E>::kIn];
                 r[i].terms(t);
@@ -512,7 +529,8 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
         have_state = true;
         if (ws) {
 #pragma unroll
-            for (int i = 0; i < kNN; ++i) S[i] = *reinterpret_cast<const f32x4*>(ws + i * 256);
+            for (int i = 0; i < kNN; ++i)
+                if (16 * i < a.N && active) S[i] = *reinterpret_cast<const f32x4*>(ws + i * 256);
         } else if (p < a.P) {
 #pragma unroll
             for (int i = 0; i < kNN; ++i) {
@@ -619,99 +637,129 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
         if (left > Q) fetch(left - Q);
         __syncthreads();
 
-        int ln = fresh(lane);
-        __builtin_amdgcn_sched_barrier(0);
-        // G^T, weighted: P[t][s] = G_ts exp(run_t - run_s) d_s, s <= t.
-        if constexpr (MAIN) {
+        // Fragments are read a step ahead of the products that take them; the
+        // barriers to the scheduler keep it from moving the reads back (to save
+        // registers, it waited for each right after its read: chunks of one
+        // block alone took 1.5 times as long).
+        int ln = fresh(lane), lr = ln & 15, lg = ln >> 4;
+        auto read_c = [&](V8 (&f)[kTT][kIn], int kk) __attribute__((always_inline)) {
 #pragma unroll
-            for (int it = 0; it < (kTT + WAVES - 1) / WAVES; ++it) {
-                const int tt = scorer + it * WAVES;
-                if (tt < kTT) {
-                    const int t = 16 * tt + lr;
-                    f32x4 w[kTT];
+            for (int tt = 0; tt < kTT; ++tt)
 #pragma unroll
-                    for (int s = 0; s < kTT; ++s) w[s] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int kk = 0; kk < kKN; ++kk) {
-                        V8 cf[kIn];
-#pragma unroll
-                        for (int k = 0; k < kIn; ++k) cf[k] = frag_row<V8, NT>(m.c + k * Q * NT, 16 * tt, 32 * kk, ln);
-#pragma unroll
-                        for (int s = 0; s < kTT; ++s)
-                            if (s <= tt) {
-                                V8 bf[kIn];
-#pragma unroll
-                                for (int k = 0; k < kIn; ++k)
-                                    bf[k] = frag_split<V8, NT>(m.b + k * Q * NT, 16 * s, 32 * kk, ln);
-                                w[s] = mma(bf, cf, w[s]);
-                            }
-                    }
-                    const float hi = m.hi[at + t], lo = m.lo[at + t];
-                    float top = 0.0f;
-#pragma unroll
-                    for (int s = 0; s < kTT; ++s)
-                        if (s <= tt) {
-                            const int s0 = 16 * s + 4 * lg;
-                            const f32x4 sh = *reinterpret_cast<const f32x4*>(m.hi + at + s0);
-                            const f32x4 sl = *reinterpret_cast<const f32x4*>(m.lo + at + s0);
-                            const f32x4 sd = *reinterpret_cast<const f32x4*>(m.step + at + s0);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float e = __builtin_amdgcn_exp2f((hi - sh[i]) + (lo - sl[i]));
-                                w[s][i] *= e * sd[i];
-                                if (s == tt) w[s][i] = s0 + i <= t ? w[s][i] : 0.0f;
-                                if constexpr (Sch::kScaled) top = fmaxf(top, fabsf(w[s][i]));
-                            }
-                        }
-                    float factor = 1.0f;
-                    if constexpr (Sch::kScaled) {
-                        float inverse;
-                        factor = scale_for(max_of_groups(top), inverse);
-                        if (lg == 0) m.row[t] = inverse;
-                    }
-#pragma unroll
-                    for (int s = 0; s < kTT; ++s)
-                        if (s <= (tt | 1)) {
-                            f32x2 u = {w[s][0] * factor, w[s][1] * factor}, v = {w[s][2] * factor, w[s][3] * factor};
-#pragma unroll
-                            for (int k = 0; k < kOut; ++k)
-                                *reinterpret_cast<u32x2*>(m.p + k * Q * Q + place<Q>(t, 16 * s + 4 * lg)) =
-                                    u32x2{take_term((const V8*)nullptr, u), take_term((const V8*)nullptr, v)};
-                        }
+                for (int k = 0; k < kIn; ++k) {
+                    if constexpr (MAIN) f[tt][k] = frag_row<V8, NT>(m.c + k * Q * NT, 16 * tt, 32 * kk, ln);
                 }
-            }
-        }
-
-        __builtin_amdgcn_sched_barrier(0);
-        ln = fresh(ln);
-        // x^T: lane p, s = 32 ks + 4 lg .. + 3 and those 16 further on, the order of
-        // all products over s.
-        V8 xf[kKS][kIn];
-        int bad = Q;  // the first token whose x is not finite
-        bool any_bad = false;
-        f32x4 y[MAIN ? kTT : 1];
-        if (active) {
+        };
+        auto read_bt = [&](V8 (&f)[kKS][2][kIn], int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int ks = 0; ks < kKS; ++ks)
 #pragma unroll
-                for (int k = 0; k < kIn; ++k)
-                    xf[ks][k] = frag_tr<V8, kXC>(m.x + k * Q * kXC, 32 * ks, 16 * wave, ln);
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int k = 0; k < kIn; ++k)
+                        f[ks][u][k] = frag_tr<V8, NT>(m.b + k * Q * NT, 32 * ks, 16 * (2 * i + u), ln);
+        };
+        // G^T, weighted: P[t][s] = G_ts exp(run_t - run_s) d_s, s <= t, tiles s of
+        // 16 up to tile t.
+        if constexpr (MAIN) {
+            auto scores = [&](auto tiles) __attribute__((always_inline)) {
+                constexpr int kS = tiles(), tt = kS - 1;
+                const int t = 16 * tt + lr;
+                f32x4 w[kS];
+#pragma unroll
+                for (int s = 0; s < kS; ++s) w[s] = f32x4{0, 0, 0, 0};
+                V8 cf[2][kIn], bf[2][kS][kIn];
+                auto read = [&](int kk) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int k = 0; k < kIn; ++k) {
+                        cf[kk & 1][k] = frag_row<V8, NT>(m.c + k * Q * NT, 16 * tt, 32 * kk, ln);
+#pragma unroll
+                        for (int s = 0; s < kS; ++s)
+                            bf[kk & 1][s][k] = frag_split<V8, NT>(m.b + k * Q * NT, 16 * s, 32 * kk, ln);
+                    }
+                };
+                read(0);
+#pragma unroll
+                for (int kk = 0; kk < kKN; ++kk) {
+                    if (kk + 1 < kKN) read(kk + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    mma(bf[kk & 1], cf[kk & 1], w);
+                }
+                const float hi = m.hi[at + t], lo = m.lo[at + t];
+                f32x4 e[kS], sd[kS];
+#pragma unroll
+                for (int s = 0; s < kS; ++s) {
+                    const int s0 = 16 * s + 4 * lg;
+                    const f32x4 sh = *reinterpret_cast<const f32x4*>(m.hi + at + s0);
+                    const f32x4 sl = *reinterpret_cast<const f32x4*>(m.lo + at + s0);
+                    sd[s] = *reinterpret_cast<const f32x4*>(m.step + at + s0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) e[s][i] = (hi - sh[i]) + (lo - sl[i]);
+                }
+                float top = 0.0f;
+#pragma unroll
+                for (int s = 0; s < kS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        w[s][i] *= __builtin_amdgcn_exp2f(e[s][i]) * sd[s][i];
+                        if (s == tt) w[s][i] = 4 * lg + i <= lr ? w[s][i] : 0.0f;
+                        if constexpr (Sch::kScaled) top = fmaxf(top, fabsf(w[s][i]));
+                    }
+                float factor = 1.0f;
+                if constexpr (Sch::kScaled) {
+                    float inverse;
+                    factor = scale_for(max_of_groups(top), inverse);
+                    if (lg == 0) m.row[t] = inverse;
+                }
+                // In the order of the products over s: s = 16 h + 4 g + j at 8 g + 4 h + j.
+#pragma unroll
+                for (int s = 0; s < kTT; ++s) {
+                    f32x2 u = {0, 0}, v = {0, 0};
+                    if (s < kS) {
+                        u = f32x2{w[s < kS ? s : 0][0] * factor, w[s < kS ? s : 0][1] * factor};
+                        v = f32x2{w[s < kS ? s : 0][2] * factor, w[s < kS ? s : 0][3] * factor};
+                    }
+#pragma unroll
+                    for (int k = 0; k < kOut; ++k)
+                        *reinterpret_cast<u32x2*>(m.p + k * Q * Q + place<Q>(t, 8 * lg + 4 * s)) =
+                            u32x2{take_term((const V8*)nullptr, u), take_term((const V8*)nullptr, v)};
+                }
+            };
+            static_assert(kTT == 2, "two tiles of tokens");
+            if (scorer == 0) scores(std::integral_constant<int, 1>{});
+            if (scorer == 1) scores(std::integral_constant<int, 2>{});
+        }
+
+        __builtin_amdgcn_sched_barrier(0);
+        ln = fresh(ln), lr = ln & 15, lg = ln >> 4;
+        // x^T: lane p, s = 32 ks + 4 lg .. + 3 and those 16 further on, the order of
+        // all products over s.  In the outputs' layout, x of token tile tt is half of
+        // it.
+        V8 xf[kKS][kIn];
+        int bad = Q;  // the first token whose x is not finite
+        bool any_bad = false;
+        f32x4 y[MAIN ? kTT : 1], gate[MAIN ? kTT : 1];
+        if (active) {
             if constexpr (MAIN) {
                 // exp(run_t) C S
 #pragma unroll
                 for (int tt = 0; tt < kTT; ++tt) y[tt] = f32x4{0, 0, 0, 0};
                 if (have_state) {
+                    V8 cf[2][kTT][kIn];
+                    read_c(cf[0], 0);
                     float factor = 1.0f, inverse = 1.0f;
                     if constexpr (Sch::kScaled) {
-                        float top = 0.0f;
+                        float top[4] = {0, 0, 0, 0};
 #pragma unroll
                         for (int i = 0; i < kNN; ++i)
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) top = fmaxf(top, fabsf(S[i][k]));
-                        factor = scale_for(max_of_groups(top), inverse);
+                            for (int k = 0; k < 4; ++k) top[i & 3] = fmaxf(top[i & 3], fabsf(S[i][k]));
+                        factor = scale_for(max_of_groups(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), inverse);
                     }
 #pragma unroll
                     for (int kk = 0; kk < kKN; ++kk) {
+                        if (kk + 1 < kKN) read_c(cf[(kk + 1) & 1], kk + 1);
+                        __builtin_amdgcn_sched_barrier(0);
                         float v[8];
                         V8 sf[kOut];
 #pragma unroll
@@ -720,14 +768,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                             if constexpr (Sch::kScaled) v[i] *= factor;
                         }
                         split8(v, sf);
-#pragma unroll
-                        for (int tt = 0; tt < kTT; ++tt) {
-                            V8 cf[kIn];
-#pragma unroll
-                            for (int k = 0; k < kIn; ++k)
-                                cf[k] = frag_row<V8, NT>(m.c + k * Q * NT, 16 * tt, 32 * kk, ln);
-                            y[tt] = mma(cf, sf, y[tt]);
-                        }
+                        mma(cf[kk & 1], sf, y);
                     }
 #pragma unroll
                     for (int tt = 0; tt < kTT; ++tt) {
@@ -738,15 +779,22 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            ln = fresh(ln);
+            ln = fresh(ln), lr = ln & 15, lg = ln >> 4;
             // S' = exp(run_Q) S + B^T (w x)
+            V8 bf[2][kKS][2][kIn];
+#pragma unroll
+            for (int ks = 0; ks < kKS; ++ks)
+#pragma unroll
+                for (int k = 0; k < kIn; ++k)
+                    xf[ks][k] = frag_tr<V8, kXC>(m.x + k * Q * kXC, 32 * ks, 16 * wave, ln);
             float whole = m.whole[at / Q];
+            read_bt(bf[0], 0);
             if constexpr (!MAIN) {
                 sum += double(whole);
                 whole = __builtin_amdgcn_exp2f(whole);
             }
             V8 wx[kKS][kState];
-            float wv[kKS][8], top = 0.0f, factor = 1.0f, inverse = 1.0f;
+            float xv[kKS][8], wv[kKS][8], top = 0.0f, factor = 1.0f, inverse = 1.0f;
 #pragma unroll
             for (int ks = 0; ks < kKS; ++ks) {
                 const f32x4 w0 = *reinterpret_cast<const f32x4*>(m.weight + at + 32 * ks + 4 * lg);
@@ -756,9 +804,17 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                     float v = elem_f32(xf[ks][0], i);
 #pragma unroll
                     for (int k = 1; k < kIn; ++k) v += elem_f32(xf[ks][k], i);
+                    xv[ks][i] = v;
                     wv[ks][i] = v * (i < 4 ? w0[i & 3] : w1[i & 3]);
                     if constexpr (Sch::kScaled) top = fmaxf(top, fabsf(wv[ks][i]));
                 }
+            }
+            if constexpr (MAIN) {
+                // the skip
+#pragma unroll
+                for (int tt = 0; tt < kTT; ++tt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[tt][i] = __builtin_fmaf(skip, xv[tt / 2][4 * (tt & 1) + i], y[tt][i]);
             }
             if constexpr (Sch::kScaled) factor = scale_for(max_of_groups(top), inverse);
 #pragma unroll
@@ -769,29 +825,41 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                 split8(wv[ks], wx[ks]);
             }
 #pragma unroll
-            for (int i = 0; i < kNN; ++i) {
-                f32x4 d = f32x4{0, 0, 0, 0};
-                if constexpr (!Sch::kScaled)
+            for (int i = 0; i < kNN / 2; ++i) {
+                if (i + 1 < kNN / 2) read_bt(bf[(i + 1) & 1], i + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                f32x4 d[2];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) d[k] = S[i][k] * whole;
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int ks = 0; ks < kKS; ++ks) {
-                    V8 bf[kIn];
+                    for (int k = 0; k < 4; ++k) d[u][k] = Sch::kScaled ? 0.0f : S[2 * i + u][k] * whole;
 #pragma unroll
-                    for (int k = 0; k < kIn; ++k)
-                        bf[k] = frag_tr<V8, NT>(m.b + k * Q * NT, 32 * ks, 16 * i, ln);
-                    d = mma(bf, wx[ks], d);
-                }
-                if constexpr (Sch::kScaled) {
+                for (int ks = 0; ks < kKS; ++ks) mma(bf[i & 1][ks], wx[ks], d);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) S[i][k] = __builtin_fmaf(d[k], inverse, S[i][k] * whole);
-                } else {
-                    S[i] = d;
-                }
-                if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        S[2 * i + u][k] = Sch::kScaled ? __builtin_fmaf(d[u][k], inverse, S[2 * i + u][k] * whole) : d[u][k];
             }
             have_state = true;
             if constexpr (MAIN) {
+                // The gate's inputs, in the outputs' layout.
+                if (gated) {
+#pragma unroll
+                    for (int tt = 0; tt < kTT; ++tt) {
+                        if constexpr (E::kBytes == 2) {
+                            const u32x2 v = read_tr(reinterpret_cast<const uint16_t*>(m.z) +
+                                                    (16 * tt + 4 * lg + (lr >> 2)) * kZP + 16 * wave + 4 * (lr & 3));
+                            const V8 v8 = __builtin_bit_cast(V8, u32x4{v[0], v[1], 0, 0});
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) gate[tt][i] = silu(elem_f32(v8, i));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                gate[tt][i] = silu(E::to_f32(m.z[(16 * tt + 4 * lg + i) * kZP + 16 * wave + lr]));
+                        }
+                    }
+                }
                 // Tokens before one whose x is an infinity or NaN must not see
                 // it times their weight of 0: it is taken out and put back below.
                 uint32_t some = 0;
@@ -816,67 +884,45 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
         }
         if constexpr (MAIN) {
             __syncthreads();
-            ln = fresh(ln);
+            ln = fresh(ln), lr = ln & 15, lg = ln >> 4;
             if (active) {
+                V8 pf[kTT][kOut];
+#pragma unroll
+                for (int tt = 0; tt < kTT; ++tt)
+#pragma unroll
+                    for (int k = 0; k < kOut; ++k) pf[tt][k] = frag_row<V8, Q>(m.p + k * Q * Q, 16 * tt, 0, ln);
+                f32x4 d[kTT], r[kTT];
 #pragma unroll
                 for (int tt = 0; tt < kTT; ++tt) {
-                    f32x4 d = Sch::kScaled ? f32x4{0, 0, 0, 0} : y[tt];
+                    d[tt] = Sch::kScaled ? f32x4{0, 0, 0, 0} : y[tt];
+                    if constexpr (Sch::kScaled) r[tt] = *reinterpret_cast<const f32x4*>(m.row + 16 * tt + 4 * lg);
+                }
+                mma(pf, xf[0], d);
 #pragma unroll
-                    for (int ks = 0; ks <= tt / 2; ++ks) {
-                        V8 pf[kOut];
+                for (int tt = 0; tt < kTT; ++tt) {
+                    if constexpr (Sch::kScaled)
 #pragma unroll
-                        for (int k = 0; k < kOut; ++k)
-                            pf[k] = frag_split<V8, Q>(m.p + k * Q * Q, 16 * tt, 32 * ks, ln);
-                        d = mma(pf, xf[ks], d);
-                    }
-                    if constexpr (Sch::kScaled) {
-                        const f32x4 r = *reinterpret_cast<const f32x4*>(m.row + 16 * tt + 4 * lg);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) d[i] = __builtin_fmaf(d[i], r[i], y[tt][i]);
-                    }
+                        for (int i = 0; i < 4; ++i) d[tt][i] = __builtin_fmaf(d[tt][i], r[tt][i], y[tt][i]);
                     if (any_bad) {
                         const int first = fresh(bad);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (16 * tt + 4 * lg + i >= first) d[i] = __builtin_nanf("");
+                            if (16 * tt + 4 * lg + i >= first) d[tt][i] = __builtin_nanf("");
                     }
-                    // x of the outputs' tokens, for the skip
-                    float xv[4];
-#pragma unroll
-                    for (int k = 0; k < kIn; ++k) {
-                        const u32x2 v = read_tr<kXC>(m.x + k * Q * kXC, 16 * tt, 16 * wave, ln);
-                        const V8 v8 = __builtin_bit_cast(V8, u32x4{v[0], v[1], 0, 0});
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) xv[i] = k ? xv[i] + elem_f32(v8, i) : elem_f32(v8, i);
-                    }
-                    float zv[4];
-                    T* zt = m.z + (16 * tt + 4 * lg) * kZP + 16 * wave + lr;
-                    if constexpr (E::kBytes == 2) {
-                        const u32x2 v = read_tr(reinterpret_cast<const uint16_t*>(m.z) +
-                                                (16 * tt + 4 * lg + (lr >> 2)) * kZP + 16 * wave + 4 * (lr & 3));
-                        const V8 v8 = __builtin_bit_cast(V8, u32x4{v[0], v[1], 0, 0});
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) zv[i] = elem_f32(v8, i);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) zv[i] = E::to_f32(zt[i * kZP]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) d[i] = __builtin_fmaf(skip, xv[i], d[i]);
                     if (gated)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) d[i] *= silu(zv[i]);
+                        for (int i = 0; i < 4; ++i) d[tt][i] *= gate[tt][i];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) zt[i * kZP] = T(d[i]);
+                    for (int i = 0; i < 4; ++i) m.z[(16 * tt + 4 * lg + i) * kZP + 16 * wave + lr] = T(d[tt][i]);
                 }
                 // The wave's columns of y, 16 bytes a lane.
                 constexpr int kV = 16 / E::kBytes, kL = 16 / kV, kR = 64 / kL;
-                const int pc = 16 * wave + kV * (lane % kL), have = width - pc;
+                const int pc = 16 * wave + kV * (ln % kL), have = width - pc;
                 char* yp = reinterpret_cast<char*>(yb);
-                const uint32_t yo = uint32_t((lane / kL) * ys + pc) * E::kBytes, yr = uint32_t(kR * ys) * E::kBytes;
+                const uint32_t yo = uint32_t((ln / kL) * ys + pc) * E::kBytes, yr = uint32_t(kR * ys) * E::kBytes;
 #pragma unroll
                 for (int i = 0; i < Q / kR; ++i) {
-                    const int t = lane / kL + i * kR;
+                    const int t = ln / kL + i * kR;
                     const T* from = m.z + t * kZP + pc;
                     if (t < left) {
                         if (have >= kV) {
@@ -897,7 +943,8 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     if (!active) return;
     if constexpr (!MAIN) {
 #pragma unroll
-        for (int i = 0; i < kNN; ++i) *reinterpret_cast<f32x4*>(ws + i * 256) = S[i];
+        for (int i = 0; i < kNN; ++i)
+            if (16 * i < a.N) *reinterpret_cast<f32x4*>(ws + i * 256) = S[i];
         if (pt == 0 && threadIdx.x == 0) g.ws_decay[int64_t(id) * a.H + h] = __builtin_amdgcn_exp2f(float(sum));
     } else if (piece.last && a.state_out && p < a.P) {
 #pragma unroll
