@@ -467,6 +467,8 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     using Shape = ChunkShape<E, NT, Q, WAVES>;
     constexpr int kThreads = Shape::kThreads, kPT = Shape::kPT, kIn = Sch::kIn, kState = Sch::kState, kOut = Sch::kOut;
     constexpr int kZP = Shape::kZP, kXC = Shape::kXC, kTokens = Shape::kTokens;
+    // Tiles of n whose sums take turns; registers hold one of a float16 main kernel.
+    constexpr int kTurn = MAIN && Sch::kScaled ? 1 : 2;
     constexpr int kTT = Q / 16, kNN = NT / 16, kKS = Q / 32, kKN = NT / 32;
     __shared__ std::conditional_t<MAIN, typename Shape::Lds, typename Shape::LdsStates> m;
     const ScanArgs& a = g.s;
@@ -650,14 +652,14 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                     if constexpr (MAIN) f[tt][k] = frag_row<V8, NT>(m.c + k * Q * NT, 16 * tt, 32 * kk, ln);
                 }
         };
-        auto read_bt = [&](V8 (&f)[kKS][2][kIn], int i) __attribute__((always_inline)) {
+        auto read_bt = [&](V8 (&f)[kKS][kTurn][kIn], int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int ks = 0; ks < kKS; ++ks)
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < kTurn; ++u)
 #pragma unroll
                     for (int k = 0; k < kIn; ++k)
-                        f[ks][u][k] = frag_tr<V8, NT>(m.b + k * Q * NT, 32 * ks, 16 * (2 * i + u), ln);
+                        f[ks][u][k] = frag_tr<V8, NT>(m.b + k * Q * NT, 32 * ks, 16 * (kTurn * i + u), ln);
         };
         // G^T, weighted: P[t][s] = G_ts exp(run_t - run_s) d_s, s <= t, tiles s of
         // 16 up to tile t.
@@ -781,7 +783,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
             __builtin_amdgcn_sched_barrier(0);
             ln = fresh(ln), lr = ln & 15, lg = ln >> 4;
             // S' = exp(run_Q) S + B^T (w x)
-            V8 bf[2][kKS][2][kIn];
+            V8 bf[2][kKS][kTurn][kIn];
 #pragma unroll
             for (int ks = 0; ks < kKS; ++ks)
 #pragma unroll
@@ -825,21 +827,21 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                 split8(wv[ks], wx[ks]);
             }
 #pragma unroll
-            for (int i = 0; i < kNN / 2; ++i) {
-                if (i + 1 < kNN / 2) read_bt(bf[(i + 1) & 1], i + 1);
+            for (int i = 0; i < kNN / kTurn; ++i) {
+                if (i + 1 < kNN / kTurn) read_bt(bf[(i + 1) & 1], i + 1);
                 __builtin_amdgcn_sched_barrier(0);
-                f32x4 d[2];
+                f32x4 d[kTurn];
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < kTurn; ++u)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) d[u][k] = Sch::kScaled ? 0.0f : S[2 * i + u][k] * whole;
+                    for (int k = 0; k < 4; ++k) d[u][k] = Sch::kScaled ? 0.0f : S[kTurn * i + u][k] * whole;
 #pragma unroll
                 for (int ks = 0; ks < kKS; ++ks) mma(bf[i & 1][ks], wx[ks], d);
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < kTurn; ++u)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        S[2 * i + u][k] = Sch::kScaled ? __builtin_fmaf(d[u][k], inverse, S[2 * i + u][k] * whole) : d[u][k];
+                        S[kTurn * i + u][k] = Sch::kScaled ? __builtin_fmaf(d[u][k], inverse, S[kTurn * i + u][k] * whole) : d[u][k];
             }
             have_state = true;
             if constexpr (MAIN) {
