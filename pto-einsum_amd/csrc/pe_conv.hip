@@ -8,6 +8,11 @@
 // last W - 1 inputs in registers, so x is read once but for W - 1 tokens at the
 // run's start.  A group of tokens is loaded while the one before is worked on.
 // Sums are float32 in the order of j after the bias; the output is rounded once.
+//
+// Four prompts of 4096 x 4352 float16: 65 us a call, 4.4 TB/s (without the loads
+// ahead and with the library's exp and divide 142); 3993 x 1283 bfloat16 in packed
+// prompts 13 us; one token of 64 x 4352 4 us of a call of 10.5.  Stores that pass
+// the caches by made the large call 62 us back to back but 82 instead of 76 alone.
 #include "pe_ssm.h"
 
 #include <algorithm>

@@ -1,5 +1,6 @@
 // Selective scan token by token: the recurrence itself, for single tokens
-// (state in the cache's slots) and for prompts.
+// (state in the cache's slots) and for prompts of up to 16 tokens (and any whose
+// rows or strides the chunks do not take).
 //
 //   S[p, n] = exp(A d) S[p, n] + d x[p] B[n],    y[p] = sum_n C[n] S[p, n] + D x[p]
 //
@@ -8,6 +9,10 @@
 // bytes) each; a wave holds R x 64 / LPR rows, so a lane has R loads in flight
 // and B, C serve R rows.  The R sums over n are reduced together: log2 R halving
 // exchanges, each lane keeping half the rows it held, then butterflies.
+//
+// One token of 128 sequences, 64 heads of 64 x 128: 537 MB of states read and
+// written in 106 us, 5.1 TB/s (a large copy moves 5.1 to 6.5 here).  Of one
+// sequence, 32 heads: 6.7 us, of a call of 13.
 #include "pe_scan.h"
 
 namespace pe {
