@@ -271,6 +271,8 @@ typedef struct pe_scan_desc {
 } pe_scan_desc;
 #define PE_SCAN_MAX_N 256
 
+/* Bytes of the workspace (16-byte aligned) that pe_selective_scan needs for the
+ * descriptor, with packed set if offsets (cu) will be given; 0: none. */
 int64_t pe_selective_scan_workspace_bytes(const pe_scan_desc* d, int packed);
 int pe_selective_scan(const pe_scan_desc* d, const void* x, const void* dt, const float* A, const void* B,
                       const void* C, const float* D, const void* z, const float* dt_bias,
