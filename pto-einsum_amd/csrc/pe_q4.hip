@@ -340,13 +340,15 @@ __global__ __launch_bounds__(64 * (kWaves<E, MT, NT>)) void q4_kernel(Q4Args g) 
         s.store(o, g, m.wave[wave], m0, lane);
         load_x(i + 1);
         load(o, i + 2);
-        // The wave's own LDS: its operations are carried out in order.
+        wave_sync();
         W::apply(g, m.wave[wave], lane, acc);
+        wave_sync();
     };
     load(even, first);
     load_x(first);
     load(odd, first + 1);
     W::clear(g, m.wave[wave], m0, lane);
+    wave_sync();
     for (int i = first; i < last; i += 2) {
         step(even, i);
         if (i + 1 < last) step(odd, i + 1);

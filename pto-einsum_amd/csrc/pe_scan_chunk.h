@@ -927,6 +927,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                     for (int i = 0; i < 4; ++i) m.z[(16 * tt + 4 * lg + i) * kZP + 16 * wave + lr] = T(d[tt][i]);
                 }
                 // The wave's columns of y, 16 bytes a lane.
+                wave_sync();
                 constexpr int kV = 16 / E::kBytes, kL = 16 / kV, kR = 64 / kL;
                 const int pc = 16 * wave + kV * (ln % kL), have = width - pc;
                 char* yp = reinterpret_cast<char*>(yb);

@@ -66,6 +66,13 @@ __device__ __forceinline__ float silu(float v) {
 // log(1 + exp(v)) without overflow; exp(-|v|) below 2^-24 leaves max(v, 0).
 __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))); }
 
+// Between LDS writes and reads of other lanes of the same wave: a wave's LDS
+// operations are carried out in order, and the compiler must keep them so.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Offset i of packed sequences, clamped to the buffer's tokens.
 __device__ __forceinline__ int64_t offset_of(const int32_t* cu, int64_t i, int64_t total) {
     const int64_t v = cu[i];
