@@ -23,9 +23,12 @@
 //   float32:  q through float32, whose upper half is q in bfloat16; x is cut into
 //             three bfloat16 terms, exactly.
 //
-// 16 tokens, 16384 x 8192 bfloat16 in groups of 64: 24 us, 3.2 TB/s (75 with 4-byte
-// loads and no step ahead; 35 with weights that pass the caches by); one token,
-// 4096 x 4096: 6.4 us of a call of 9.5, which the host's part bounds.
+// 16 tokens, 16384 x 8192 bfloat16 in groups of 64, three sets of weights in turn:
+// 20.7 us, 3.7 TB/s (75 with 4-byte loads and no step ahead; 24 with a branch
+// around the loads ahead and a stretch of K for each wave); eight sets, which no
+// cache holds: 29 us, 2.3 TB/s, one token 27.  One block of eight waves a CU has
+// too little on its way for more.  One token, 4096 x 4096: 6.4 us of a call of
+// 9.4, which the host's part bounds.
 #include "pe_ssm.h"
 
 #include <algorithm>
@@ -46,7 +49,6 @@ struct Q4Args {
     void* y;
     int64_t x_ms;
     int32_t M, N, K, groups, row_bytes;
-    int32_t steps;       // of a wave
 };
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -188,19 +190,19 @@ struct Wave {
             if constexpr (FULL) o.w[t] = *reinterpret_cast<const LooseVec*>(row + at);
             else o.w[t] = last_vec(row, at, g.row_bytes);
         }
-        if (lane < kRows) {
-            const int64_t at = int64_t(min(n0 + lane, g.N - 1)) * g.groups + k0 / GROUP;
-            const T *sp = static_cast<const T*>(g.scales) + at, *zp = static_cast<const T*>(g.zeros) + at;
-            if constexpr (FULL) {
-                o.scale = *reinterpret_cast<const LooseScales*>(sp);
-                if (g.zeros) o.zero = *reinterpret_cast<const LooseScales*>(zp);
-            } else {
+        // (Without zero points the scales are read in their place, so that there is
+        // no branch around a load.)
+        const int64_t at = int64_t(min(n0 + min(lane, kRows - 1), g.N - 1)) * g.groups + k0 / GROUP;
+        const T *sp = static_cast<const T*>(g.scales) + at, *zp = static_cast<const T*>(g.zeros ? g.zeros : g.scales) + at;
+        if constexpr (FULL) {
+            o.scale = *reinterpret_cast<const LooseScales*>(sp);
+            o.zero = *reinterpret_cast<const LooseScales*>(zp);
+        } else {
 #pragma unroll
-                for (int j = 0; j < kGroups; ++j) {
-                    const int i = min(j, g.groups - 1 - k0 / GROUP);
-                    o.scale[j] = sp[i];
-                    if (g.zeros) o.zero[j] = zp[i];
-                }
+            for (int j = 0; j < kGroups; ++j) {
+                const int i = min(j, g.groups - 1 - k0 / GROUP);
+                o.scale[j] = sp[i];
+                o.zero[j] = zp[i];
             }
         }
     }
@@ -211,12 +213,10 @@ struct Wave {
         for (int i = 0; i < kXEach; ++i) {
             const int v = lane + 64 * i, m = m0 + v / kXVecs, vec = v % kXVecs;
             const int64_t at = int64_t(k0) * E::kBytes + vec * 16;
-            if (m0 + 64 * i / kXVecs < g.M) {
-                const uint8_t* row = reinterpret_cast<const uint8_t*>(static_cast<const T*>(g.x) +
-                                                                      int64_t(min(m, g.M - 1)) * g.x_ms);
-                if constexpr (FULL) x[i] = *reinterpret_cast<const LooseVec*>(row + at);
-                else x[i] = last_vec(row, at, int64_t(g.K) * E::kBytes);
-            }
+            const uint8_t* row = reinterpret_cast<const uint8_t*>(static_cast<const T*>(g.x) +
+                                                                  int64_t(min(m, g.M - 1)) * g.x_ms);
+            if constexpr (FULL) x[i] = *reinterpret_cast<const LooseVec*>(row + at);
+            else x[i] = last_vec(row, at, int64_t(g.K) * E::kBytes);
         }
     }
 
@@ -246,14 +246,13 @@ struct Wave {
     }
 
     // acc[m][t]: rows m = 4 lg + element, column n = lr.
-    __device__ __forceinline__ static void apply(const Q4Args& g, const Lds& l, int lane, f32x4 (&acc)[MT][NT]) {
+    __device__ __forceinline__ static void apply(const Lds& l, int lane, f32x4 (&acc)[MT][NT]) {
         using V8 = typename Mma<E>::V8;
         constexpr int kTerms = Mma<E>::kTerms;
         const int lr = lane & 15, lg = lane >> 4;
         V8 ones;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ones[i] = (typename std::remove_reference<decltype(ones[0])>::type)1.0f;
-        const bool with_x = g.zeros || Mma<E>::kOffset != -8.0f;
 #pragma unroll
         for (int j = 0; j < kGroups; ++j) {
             typedef uint32_t Words __attribute__((ext_vector_type(GW)));
@@ -274,9 +273,8 @@ struct Wave {
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     operand(l.x + (16 * m + lr) * kXP + j * GROUP + lg * (GROUP / 4) + 8 * i, o[m]);
-                    if (with_x)
 #pragma unroll
-                        for (int c = kTerms - 1; c >= 0; --c) xs[m] = mma(o[m][c], ones, xs[m]);
+                    for (int c = kTerms - 1; c >= 0; --c) xs[m] = mma(o[m][c], ones, xs[m]);
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
@@ -293,11 +291,11 @@ struct Wave {
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float v = with_x ? __builtin_fmaf(-z, xs[m][e], q[m][t][e]) : q[m][t][e];
-                        acc[m][t][e] = __builtin_fmaf(s, v, acc[m][t][e]);
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        acc[m][t][e] = __builtin_fmaf(s, __builtin_fmaf(-z, xs[m][e], q[m][t][e]), acc[m][t][e]);
             }
+            // One group's operands at a time: unpacked ahead, they do not fit.
+            if constexpr (kGroups > 1) __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
@@ -320,8 +318,9 @@ __global__ __launch_bounds__(64 * (kWaves<E, MT, NT>)) void q4_kernel(Q4Args g) 
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
 
-    // Steps of this wave; the last of all may be one of less than kStep.
-    const int first = wave * g.steps, last = min(first + g.steps, (g.K + kStep - 1) / kStep);
+    // This wave's steps: every waves-th, so that the block reads whole stretches of
+    // its rows at a time.  The last of all may be one of less than kStep.
+    const int last = (g.K + kStep - 1) / kStep;
     W s;
     typename W::Weights even, odd;
     auto load = [&](typename W::Weights& o, int i) __attribute__((always_inline)) {
@@ -336,22 +335,36 @@ __global__ __launch_bounds__(64 * (kWaves<E, MT, NT>)) void q4_kernel(Q4Args g) 
     };
     // Weights are loaded two steps ahead (memory answers later than a step takes),
     // x, which comes from a cache, one.
-    auto step = [&](typename W::Weights& o, int i) __attribute__((always_inline)) {
+    // One step, with what comes after it loaded: weights two steps ahead (memory
+    // answers later than a step takes), x, which comes from a cache, one.  AHEAD: both
+    // are there, whole; the loads then lie on one path, and what they are waited for
+    // by can be counted (on several, a step waited for the weights of the next two).
+    auto step = [&](typename W::Weights& o, int i, auto ahead) __attribute__((always_inline)) {
         s.store(o, g, m.wave[wave], m0, lane);
-        load_x(i + 1);
-        load(o, i + 2);
+        if constexpr (ahead()) {
+            s.template load_x<true>(g, m0, (i + waves) * kStep, lane);
+            W::template load<true>(o, g, n0, (i + 2 * waves) * kStep, lane);
+        } else {
+            load_x(i + waves);
+            load(o, i + 2 * waves);
+        }
         wave_sync();
-        W::apply(g, m.wave[wave], lane, acc);
+        W::apply(m.wave[wave], lane, acc);
         wave_sync();
     };
-    load(even, first);
-    load_x(first);
-    load(odd, first + 1);
+    load(even, wave);
+    load_x(wave);
+    load(odd, wave + waves);
     W::clear(g, m.wave[wave], m0, lane);
     wave_sync();
-    for (int i = first; i < last; i += 2) {
-        step(even, i);
-        if (i + 1 < last) step(odd, i + 1);
+    int i = wave;
+    for (; i + 3 * waves < g.K / kStep; i += 2 * waves) {
+        step(even, i, std::true_type{});
+        step(odd, i + waves, std::true_type{});
+    }
+    for (; i < last; i += 2 * waves) {
+        step(even, i, std::false_type{});
+        if (i + waves < last) step(odd, i + waves, std::false_type{});
     }
     __syncthreads();
 #pragma unroll
@@ -370,7 +383,7 @@ __global__ __launch_bounds__(64 * (kWaves<E, MT, NT>)) void q4_kernel(Q4Args g) 
 }
 
 template <typename E, int GROUP>
-int launch(Q4Args g, hipStream_t stream) {
+int launch(const Q4Args& g, hipStream_t stream) {
     // Tiles of 16 rows of x, and weight rows for each x that is loaded: as many as
     // leave a block for each CU.
     const int mt = g.M <= 16 ? 1 : g.M <= 32 ? 2 : 4;
@@ -380,8 +393,8 @@ int launch(Q4Args g, hipStream_t stream) {
     auto run = [&](auto m, auto n) {
         constexpr int MT = m(), NT = n();
         const int steps = int(ceil_div(g.K, kStep));
-        g.steps = std::max(1, int(ceil_div(steps, kWaves<E, MT, NT>)));
-        const int waves = std::max(1, int(ceil_div(steps, g.steps)));
+        const int each = std::max(1, int(ceil_div(steps, kWaves<E, MT, NT>)));   // of a wave
+        const int waves = std::max(1, int(ceil_div(steps, each)));
         const int64_t cols = ceil_div(g.N, 16 * NT);
         if (tall > 65535 || tall * cols * 64 * waves >= (int64_t(1) << 32))
             return fail(PE_ERR_UNSUPPORTED, "matvec_q4: too many rows");
