@@ -53,4 +53,13 @@ constexpr int64_t product_tile_blocks(int64_t P, int64_t Q, int64_t batches) {
     return 16 * P * Q >= 64 * 64 * tiles && tiles * batches <= kMaxBlocks ? tiles * batches : 0;
 }
 
+// Token strides that the chunked scan takes are below this: a chunk's rows (64 of
+// 16-bit elements, 32 of float32) then lie within 2^32 bytes of its first.
+constexpr int64_t kScanStrideEnd = int64_t(1) << 24;
+
+// Elements from a piece's first step size to that of token i.  Step sizes are
+// read 256 tokens at a time, and up to index 383 where three waves share them, so
+// unlike a chunk's rows they pass 2^31 elements at strides below kScanStrideEnd.
+constexpr int64_t step_offset(int32_t i, int32_t stride) { return int64_t(i) * stride; }
+
 }  // namespace pe

@@ -66,10 +66,9 @@ Plan plan_of(const pe_scan_desc& d, bool packed) {
     // Up to 16 tokens the recurrence is as quick; rows of less than eight
     // elements cannot be loaded as whole vectors.
     if (d.T <= 16 || d.N < 8 || d.P < 8) return p;
-    // Offsets within a chunk are 32 bits.
-    constexpr int64_t kMostStride = int64_t(1) << 24;
+    // Offsets of rows within a chunk are 32 bits.
     for (const int64_t ts : {d.x_ts, d.z_ts, d.dt_ts, d.b_ts, d.c_ts, d.H * d.P})
-        if (ts >= kMostStride) return p;
+        if (ts >= kScanStrideEnd) return p;
     p.chunks = true;
     p.nt = d.N <= 32 ? 32 : d.N <= 64 ? 64 : d.N <= 128 ? 128 : 256;
     // Tiles of up to 64 rows p, as even as waves of 16 allow.

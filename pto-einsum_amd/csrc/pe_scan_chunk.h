@@ -522,7 +522,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     const double A2 = double(A) * 1.4426950408889634;  // exponents are of 2
     const char* dtp = static_cast<const char*>(a.dt) +
                       (seq * a.dt_bs + piece.t0 * a.dt_ts + h * a.dt_hs) * (a.dt_f32 ? 4 : E::kBytes);
-    // Token strides: below 2^24 (the host sees to it).
+    // Token strides: below kScanStrideEnd (the host sees to it).
     const int32_t b_ts = int32_t(a.b_ts), c_ts = int32_t(a.c_ts), x_ts = int32_t(a.x_ts), z_ts = int32_t(a.z_ts);
     const int32_t dt_ts = int32_t(a.dt_ts);
     const int tokens = int(piece.t1 - piece.t0);
@@ -599,7 +599,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     auto fetch_dt = [&](int t) {
 #pragma unroll
         for (int i = 0; i < kOwn; ++i)
-            raw[i] = dt_bits<E>(a, dtp, min(64 * (wave + i * WAVES) + lane, tokens - t - 1) * dt_ts);
+            raw[i] = dt_bits<E>(a, dtp, step_offset(min(64 * (wave + i * WAVES) + lane, tokens - t - 1), dt_ts));
         dtp += int64_t(kTokens) * dt_ts * (a.dt_f32 ? 4 : E::kBytes);
     };
     fetch_dt(0);
