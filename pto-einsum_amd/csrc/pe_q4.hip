@@ -23,6 +23,9 @@
 //   float32:  q through float32, whose upper half is q in bfloat16; x is cut into
 //             three bfloat16 terms, exactly.
 //
+// Outputs that end as an infinity or NaN are formed again one by one, whole weights
+// times x (whole_weights).
+//
 // 16 tokens, 16384 x 8192 bfloat16 in groups of 64, three sets of weights in turn:
 // 20.7 us, 3.7 TB/s (75 with 4-byte loads and no step ahead; 24 with a branch
 // around the loads ahead and a stretch of K for each wave); eight sets, which no
@@ -300,6 +303,34 @@ struct Wave {
     }
 };
 
+// One output by its definition, whole weights times x.  Sums of q x and of x apart
+// are not it where x is infinite (inf - inf, 0 inf) or so large that one of them
+// passes float32's range while s (q - z) x does not, and such sums never end
+// finite: outputs that are not finite are formed again this way, ends included.
+template <typename E, int GROUP>
+__device__ __forceinline__ float whole_weights(const Q4Args& g, int64_t m, int64_t n) {
+    using T = typename E::T;
+    const T* x = static_cast<const T*>(g.x) + m * g.x_ms;
+    const uint8_t* w = g.packed + n * g.row_bytes;
+    float v = 0.0f;
+    for (int64_t k = 0; k < g.K && v == v; k += 32) {   // a NaN stays one
+        const int64_t at = n * g.groups + k / GROUP;
+        const float s = E::to_f32(static_cast<const T*>(g.scales)[at]);
+        const float z = g.zeros ? E::to_f32(static_cast<const T*>(g.zeros)[at]) : 8.0f;
+        const u32x4 q = last_vec(w, k / 2, g.row_bytes);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float o[8];
+            const int left = int(min(int64_t(8), g.K - k - 8 * i));
+            load_f32<E, 8>(x + k + 8 * i, left, o);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v = j < left ? __builtin_fmaf(o[j], s * (float((q[i] >> (4 * j)) & 15) - z), v) : v;
+        }
+    }
+    return v;
+}
+
 template <typename E, int GROUP, int MT, int NT>
 __global__ __launch_bounds__(64 * (kWaves<E, MT, NT>)) void q4_kernel(Q4Args g) {
     using T = typename E::T;
@@ -333,8 +364,6 @@ __global__ __launch_bounds__(64 * (kWaves<E, MT, NT>)) void q4_kernel(Q4Args g) 
         if ((i + 1) * int64_t(kStep) <= g.K) s.template load_x<true>(g, m0, i * kStep, lane);
         else s.template load_x<false>(g, m0, i * kStep, lane);
     };
-    // Weights are loaded two steps ahead (memory answers later than a step takes),
-    // x, which comes from a cache, one.
     // One step, with what comes after it loaded: weights two steps ahead (memory
     // answers later than a step takes), x, which comes from a cache, one.  AHEAD: both
     // are there, whole; the loads then lie on one path, and what they are waited for
@@ -378,7 +407,10 @@ __global__ __launch_bounds__(64 * (kWaves<E, MT, NT>)) void q4_kernel(Q4Args g) 
         const int row = at / (16 * NT), n = at % (16 * NT);
         float v = 0.0f;
         for (int w = 0; w < waves; ++w) v += m.part[w][row][n];
-        if (m0 + row < g.M && n0 + n < g.N) static_cast<T*>(g.y)[int64_t(m0 + row) * g.N + n0 + n] = (T)v;
+        if (m0 + row < g.M && n0 + n < g.N) {
+            if (!(fabsf(v) <= 3.4028235e38f)) v = whole_weights<E, GROUP>(g, m0 + row, n0 + n);
+            static_cast<T*>(g.y)[int64_t(m0 + row) * g.N + n0 + n] = (T)v;
+        }
     }
 }
 
