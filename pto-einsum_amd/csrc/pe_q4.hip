@@ -21,7 +21,9 @@
 //             sums lose by it, 2^-24 of 136 |x| a product, is far below the
 //             result's own rounding.
 //   float32:  q through float32, whose upper half is q in bfloat16; x is cut into
-//             three bfloat16 terms, exactly.
+//             three bfloat16 terms, exactly: of 2^24 x, since bfloat16 has no bits below
+//             2^-133 and the matrix cores lose subnormals (x of 2^-124: 6e-4 of the
+//             result as it is).
 //
 // Outputs that end as an infinity or NaN are formed again one by one, whole weights
 // times x (whole_weights).
@@ -56,24 +58,25 @@ struct Q4Args {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-// Operand vectors and terms of a type, and what its weights are: q + kOffset.
+// Operand vectors and terms of a type, what its weights are, q + kOffset, and what
+// x enters the products times.
 template <typename E>
 struct Mma {  // BF16
     using V8 = bf16x8;
     static constexpr int kTerms = 1;
-    static constexpr float kOffset = 128.0f;
+    static constexpr float kOffset = 128.0f, kScale = 1.0f;
 };
 template <>
 struct Mma<F16> {
     using V8 = f16x8;
     static constexpr int kTerms = 1;
-    static constexpr float kOffset = -8.0f;
+    static constexpr float kOffset = -8.0f, kScale = 1.0f;
 };
 template <>
 struct Mma<F32> {
     using V8 = bf16x8;
     static constexpr int kTerms = 3;
-    static constexpr float kOffset = 0.0f;
+    static constexpr float kOffset = 0.0f, kScale = 0x1p24f;
 };
 
 __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
@@ -243,8 +246,12 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < kXEach; ++i) {
             const int v = lane + 64 * i;
+            u32x4 xv = x[i];
+            if constexpr (Mma<E>::kScale != 1.0f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) xv[e] = __float_as_uint(__uint_as_float(xv[e]) * Mma<E>::kScale);
             if (m0 + v / kXVecs < g.M)
-                *reinterpret_cast<u32x4*>(m.x + v / kXVecs * kXP + v % kXVecs * (16 / E::kBytes)) = x[i];
+                *reinterpret_cast<u32x4*>(m.x + v / kXVecs * kXP + v % kXVecs * (16 / E::kBytes)) = xv;
         }
     }
 
@@ -407,6 +414,7 @@ __global__ __launch_bounds__(64 * (kWaves<E, MT, NT>)) void q4_kernel(Q4Args g) 
         const int row = at / (16 * NT), n = at % (16 * NT);
         float v = 0.0f;
         for (int w = 0; w < waves; ++w) v += m.part[w][row][n];
+        v *= 1.0f / Mma<E>::kScale;
         if (m0 + row < g.M && n0 + n < g.N) {
             if (!(fabsf(v) <= 3.4028235e38f)) v = whole_weights<E, GROUP>(g, m0 + row, n0 + n);
             static_cast<T*>(g.y)[int64_t(m0 + row) * g.N + n0 + n] = (T)v;

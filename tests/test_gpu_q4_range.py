@@ -58,3 +58,13 @@ def test_x_near_the_largest(dtype, zeros, K):
     size = (x.double().abs()[:, None] * w.abs()).sum(-1)
     assert bool((size < 3e38).all())
     assert bool(((y[:3] - ref[:3]).abs() <= u.HALF[dtype] * ref[:3].abs() + 2.0 ** -24 * (K + 3) * size[:3]).all())
+
+
+@pytest.mark.parametrize("e", [-100, -112, -124, -130, -140])
+def test_small_float32_x(e):
+    """x down to float32's subnormals."""
+    x, packed, scales, z = _case(torch.float32, 2, 40, 300, 32, True, seed=1)
+    x = (x.double() * 2.0 ** e).float()
+    y = _run(x, packed, scales, z, 32).double().cpu()
+    ref, size = u.q4(x, packed, scales, z, 32, 300)
+    assert bool(((y - ref).abs() <= u.q4_bound(ref, size, 300, torch.float32)).all())
