@@ -216,11 +216,13 @@ int pe_reduce_order(const pe_reduce_desc* d, const void* src, int64_t* order);
 /* ---- state-space layer: short causal convolution, selective scan ----
  * No counterpart in the reference.  Sequences are either dense (cu == NULL:
  * nseq sequences of T tokens, `bs` apart) or packed one after another along
- * the token axis (cu: nseq + 1 int32 offsets on the device, cu[0] = 0, T the
- * tokens of the buffer; sequences may be empty; outputs of tokens past
- * cu[nseq] are zero).  cu and slots are read on the device: offsets are
- * clamped to the buffer there, and a slot outside [0, nslots) marks a row
- * without a sequence, whose output is zero and which touches no state.
+ * the token axis (cu: nseq + 1 int32 offsets on the device that do not fall, T
+ * the tokens of the buffer; sequences may be empty; outputs of tokens before
+ * cu[0] and from cu[nseq] on are zero).  cu and slots are read on the device:
+ * offsets are clamped to the buffer there (where they fall, outputs and new
+ * states are unspecified, but nothing beside them is written), and a slot
+ * outside [0, nslots) marks a row without a sequence, whose output is zero and
+ * which touches no state.  Outputs overlap no operand, nor state_out state_in.
  * Strides are in elements; the innermost axis of every tensor is contiguous. */
 
 /* y[t, d] = act(bias[d] + sum_{j < W} weight[d, j] * x[t - W + 1 + j, d]), sums

@@ -39,6 +39,15 @@ __device__ __forceinline__ float step_size(const ScanArgs& g, float v, float bia
     return g.softplus ? softplus(v) : v;
 }
 
+// Outputs of tokens before the first packed sequence and after the last: zeros.
+template <typename E>
+__device__ __forceinline__ void clear_outside(const ScanArgs& g, int64_t thread, int64_t threads) {
+    typename E::T* y = static_cast<typename E::T*>(g.y);
+    const int64_t row = int64_t(g.H) * g.P, first = offset_of(g.cu, 0, g.T) * row;
+    for (int64_t i = thread; i < first; i += threads) y[i] = typename E::T(0.0f);
+    for (int64_t i = offset_of(g.cu, g.nseq, g.T) * row + thread; i < g.T * row; i += threads) y[i] = typename E::T(0.0f);
+}
+
 // One wave holds whole rows of the state and walks its sequence token by token:
 // single tokens (slots), and prompts (rows_kernel in pe_scan_rows.hip).
 int launch_rows(int dtype, const ScanArgs& g, hipStream_t stream);

@@ -482,11 +482,8 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     __shared__ std::conditional_t<MAIN, typename Shape::Lds, typename Shape::LdsStates> m;
     const ScanArgs& a = g.s;
 
-    if (blockIdx.x >= g.blocks) {  // tokens past the packed sequences
-        const int64_t row = int64_t(a.H) * a.P, from = offset_of(a.cu, a.nseq, a.T) * row, to = a.T * row;
-        for (int64_t i = from + int64_t(blockIdx.x - g.blocks) * kThreads + threadIdx.x; i < to;
-             i += kScanTailBlocks * kThreads)
-            static_cast<T*>(a.y)[i] = T(0.0f);
+    if (blockIdx.x >= g.blocks) {
+        clear_outside<E>(a, int64_t(blockIdx.x - g.blocks) * kThreads + threadIdx.x, kScanTailBlocks * kThreads);
         return;
     }
     // Blocks go round the eight XCDs in turn; each XCD gets a run of work, whose

@@ -28,10 +28,8 @@ template <typename E, int LPR, int R, bool N4, bool NT>
 __global__ __launch_bounds__(kThreads) void rows_kernel(ScanArgs g, uint32_t tiles, uint32_t main_blocks) {
     using T = typename E::T;
     constexpr int G = 64 / LPR, TR = G * R;
-    if (blockIdx.x >= main_blocks) {  // tokens past the packed sequences
-        const int64_t row = int64_t(g.H) * g.P, from = offset_of(g.cu, g.nseq, g.T) * row, to = g.T * row;
-        for (int64_t i = from + (blockIdx.x - main_blocks) * kThreads + threadIdx.x; i < to; i += kTailBlocks * kThreads)
-            static_cast<T*>(g.y)[i] = T(0.0f);
+    if (blockIdx.x >= main_blocks) {
+        clear_outside<E>(g, int64_t(blockIdx.x - main_blocks) * kThreads + threadIdx.x, kTailBlocks * kThreads);
         return;
     }
     const int lane = threadIdx.x & 63, l = lane % LPR, grp = lane / LPR;

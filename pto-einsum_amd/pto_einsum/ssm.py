@@ -12,8 +12,9 @@ has too: it is the next operator's operand, unlike a contraction's float32
 result.  Sums and scan states are float32.  Calls enqueue on the current
 stream, allocate through torch only and neither synchronise nor clear memory
 with a memset, so they can be captured in a ``StageGraph``.  ``cu_seqlens`` and
-``slots`` are read on the GPU; offsets outside the buffer are clamped to it and
-slots outside the cache mark rows without a sequence.
+``slots`` are read on the GPU; offsets outside the buffer are clamped to it (where
+they fall, the outputs and new states mean nothing), and slots outside the cache
+mark rows without a sequence.
 """
 from __future__ import annotations
 
@@ -172,8 +173,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
         y[t, d] = act(bias[d] + sum_j weight[d, j] * x[t - width + 1 + j, d])
 
     x [nseq, T, D], or packed [T, D] with ``cu_seqlens`` (int32 offsets on the
-    GPU, nseq + 1 of them, from 0 up; tokens past the last get y = 0); weight
-    [D, width] with 2 <= width <= 8; ``activation`` None or "silu".
+    GPU, nseq + 1 of them that do not fall; tokens before the first and from the
+    last on get y = 0); weight [D, width] with 2 <= width <= 8; ``activation`` None or "silu".
     ``initial_state`` [nseq, width - 1, D] holds the inputs before each
     sequence's first token, oldest first (none: zeros).  Returns y of x's
     shape and the state after each sequence, both of x's dtype."""
@@ -300,8 +301,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     x, z [nseq, T, H, P], dt [nseq, T, H] (x's dtype or float32), B, C [nseq,
     T, G, N] with N <= 256, any strides but along the last axis; or packed,
     without the first axis, with ``cu_seqlens`` (int32 offsets on the GPU, nseq +
-    1 of them, from 0 up; tokens past the last get y = 0).  A, D, dt_bias are
-    float32 [H]; ``initial_state`` float32 [nseq, H, P, N] (none: zeros).
+    1 of them that do not fall; tokens before the first and from the last on get
+    y = 0).  A, D, dt_bias are float32 [H]; ``initial_state`` float32 [nseq, H, P, N] (none: zeros).
     Returns y (x's shape and dtype) and the float32 states after each
     sequence."""
     what = "selective_scan"
