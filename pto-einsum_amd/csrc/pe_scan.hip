@@ -59,6 +59,10 @@ struct Plan {
     int64_t state_floats = 0, decay_floats = 0;   // workspace
 };
 
+// Blocks of carry_kernel for a sequence and head.
+constexpr int kCarryThreads = 256, kAhead = 8;
+int64_t carry_blocks(const Plan& p) { return ceil_div(p.ptiles * p.waves * (p.nt / 16) * 64, kCarryThreads); }
+
 auto chunks_of(int dtype) { return dtype == PE_F16 ? chunks_f16 : dtype == PE_BF16 ? chunks_bf16 : chunks_f32; }
 
 Plan plan_of(const pe_scan_desc& d, bool packed) {
@@ -99,7 +103,14 @@ Plan plan_of(const pe_scan_desc& d, bool packed) {
     }
     p.per_seq = ceil_div(d.T, p.piece);
     p.pieces = packed ? p.per_seq + d.nseq : p.per_seq * d.nseq;
-    if (packed || p.per_seq > 1) {
+    // What passes a launch's threads goes token by token: so many sequences and
+    // heads fill the card that way too.
+    const __int128 most = (int64_t(1) << 32) - 1;
+    const bool several = packed || p.per_seq > 1;
+    if ((__int128(p.pieces) * across + kScanTailBlocks) * 64 * p.waves > most ||
+        (several && __int128(d.nseq) * d.H * carry_blocks(p) * kCarryThreads > most))
+        return Plan{};
+    if (several) {
         p.decay_floats = ceil_div(p.pieces * d.H, 4) * 4;
         p.state_floats = p.pieces * d.H * p.ptiles * p.waves * (p.nt / 16) * 256;
     }
@@ -109,8 +120,6 @@ Plan plan_of(const pe_scan_desc& d, bool packed) {
 // From the pieces' contributions to the states at their starts, in place, and
 // the final states.  A thread follows four n of a row p through its sequence;
 // the next kAhead contributions are on their way.
-constexpr int kCarryThreads = 256, kAhead = 8;
-
 __global__ __launch_bounds__(kCarryThreads) void carry_kernel(ChunkArgs g, uint32_t vecs, uint32_t frags, uint32_t wave_rows,
                                                               uint32_t head_blocks) {
     const ScanArgs& a = g.s;
@@ -166,15 +175,10 @@ __global__ __launch_bounds__(kCarryThreads) void carry_kernel(ChunkArgs g, uint3
 }
 
 int launch_plan(const pe_scan_desc& d, const Plan& p, const ScanArgs& a, void* ws, hipStream_t stream) {
-    const __int128 blocks = __int128(p.pieces) * d.H * p.ptiles;
-    // Fewer than 2^32 threads in each launch (a head has at least as many pieces
-    // as sequences, and 16 NT WAVES / 4 threads of the carry to 64 WAVES).
-    if ((blocks + kScanTailBlocks) * 64 * p.waves * (p.nt / 16) >= int64_t(1) << 32)
-        return fail(PE_ERR_UNSUPPORTED, "selective_scan: too many rows");
     ChunkArgs g{};
     g.s = a;
     g.piece = uint32_t(p.piece); g.pieces = uint32_t(p.pieces); g.per_seq = uint32_t(p.per_seq);
-    g.ptiles = uint32_t(p.ptiles); g.blocks = uint32_t(blocks);
+    g.ptiles = uint32_t(p.ptiles); g.blocks = uint32_t(p.pieces * d.H * p.ptiles);
     g.state4 = a.N % 4 == 0 && aligned(a.state_in, 16) && aligned(a.state_out, 16);
     if (p.state_floats) {
         g.ws_decay = static_cast<float*>(ws);
@@ -184,7 +188,7 @@ int launch_plan(const pe_scan_desc& d, const Plan& p, const ScanArgs& a, void* w
     if (p.state_floats) {
         run(&g, p.nt, p.waves, false, stream);
         const uint32_t frags = uint32_t(p.nt / 16), vecs = uint32_t(p.waves) * frags * 64;
-        const uint32_t head_blocks = uint32_t(ceil_div(p.ptiles * vecs, kCarryThreads));
+        const uint32_t head_blocks = uint32_t(carry_blocks(p));
         carry_kernel<<<uint32_t(d.nseq * d.H) * head_blocks, kCarryThreads, 0, stream>>>(g, vecs, frags,
                                                                                          uint32_t(p.waves), head_blocks);
     }

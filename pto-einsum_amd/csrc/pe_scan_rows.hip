@@ -161,7 +161,8 @@ int launch(const ScanArgs& g, hipStream_t stream) {
     constexpr int TR = 64 / LPR * R;
     const uint32_t tiles = uint32_t(ceil_div(g.P, TR));
     const __int128 waves = __int128(g.nseq) * g.H * tiles;
-    if (waves >= (1 << 24)) return fail(PE_ERR_UNSUPPORTED, "selective_scan: too many rows");
+    // Fewer than 2^32 threads.
+    if (waves >= (1 << 26) - 4 * kTailBlocks) return fail(PE_ERR_UNSUPPORTED, "selective_scan: too many rows");
     const uint32_t blocks = uint32_t(ceil_div(int64_t(waves), kThreads / 64));
     const uint32_t all = blocks + (g.cu ? kTailBlocks : 0);
     // States of 32 MB and more pass the caches by: with states of several calls in
