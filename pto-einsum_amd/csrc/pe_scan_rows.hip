@@ -91,10 +91,12 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(ScanArgs g, uint32_t til
             }
         }
     }
+    // Lanes past N keep a state of 0: an infinite x times their B of 0 would be NaN.
+    const bool mine = n0 < g.N;
     const float A = g.A[h], bias = g.dt_bias ? g.dt_bias[h] : 0.0f, skip = g.D ? g.D[h] : 0.0f;
     for (int64_t t = t0; t < t1; ++t) {
-        const float d = step_size(g, dt_of<E>(g, dt_bits<E>(g, g.dt, seq * g.dt_bs + t * g.dt_ts + h * g.dt_hs)), bias);
-        const float a = expf(A * d);
+        const float step = step_size(g, dt_of<E>(g, dt_bits<E>(g, g.dt, seq * g.dt_bs + t * g.dt_ts + h * g.dt_hs)), bias);
+        const float d = mine ? step : 0.0f, a = mine ? expf(A * step) : 0.0f;
         float b[4], c[4];
         const int left = g.N - n0;
         load_f32<E, 4>(static_cast<const T*>(g.B) + seq * g.b_bs + t * g.b_ts + group * g.b_gs + n0, left, b);
@@ -104,11 +106,11 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(ScanArgs g, uint32_t til
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int p = p0 + r * G + grp;
-            const float dx = d * (p < g.P ? E::to_f32(x[p]) : 0.0f);
+            const float dx = d * (p < g.P && mine ? E::to_f32(x[p]) : 0.0f);
             float v = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                st[r][i] = __builtin_fmaf(a, st[r][i], dx * b[i]);
+                st[r][i] = N4 || i < left ? __builtin_fmaf(a, st[r][i], dx * b[i]) : 0.0f;
                 v = __builtin_fmaf(c[i], st[r][i], v);
             }
             sum[r] = v;
