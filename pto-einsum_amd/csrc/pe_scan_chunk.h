@@ -28,8 +28,17 @@
 //             puts a column's (row's) largest at 2^14: float16's range is not
 //             met, and what is lost is below 2^-38 of the largest
 //   float32   three bfloat16 terms of everything, products of terms i + j <= 2
-// Operands of 16 bits enter as they are.  Sums are float32; run_t is summed in 64
+// Operands of 16 bits enter as they are.  So a float16 scan's new states are good to
+// 2^-21 of their inputs (their sums are float32), and float32 values below 2^-110
+// lose bits: the last term of 2^-120 lies under what the matrix cores keep, 6e-4.
+// Sums are float32; run_t is summed in 64
 // bits and kept as two float32, since differences of large sums count.
+//
+// Infinities and NaN spread through terms and through weights of 0 to tokens and
+// elements that the recurrence keeps clear of them, and C B^T can pass float32's
+// range where the recurrence does not; nothing of the kind ends in finite outputs.  So
+// a wave that finds an output (before its gate), or a piece's contribution, not finite
+// runs its piece again by the recurrence.
 //
 // What bounds it is vector work, not memory or the matrix cores: a wave spends some
 // 600 vector instructions on a chunk (splitting S and the weighted x into terms,
@@ -196,26 +205,11 @@ __device__ __forceinline__ float elem_f32(bf16x8 v, int i) {
     return __builtin_bit_cast(float, (i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
 }
 
-// Nonzero if an element is an infinity or NaN: the exponent of each half of a
-// word plus 1 reaches the half's top bit just when it was all ones.
-__device__ __forceinline__ uint32_t not_finite(u32x4 w, uint32_t exponent, uint32_t one) {
-    uint32_t r = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r |= (w[i] & exponent) + one;
-    return r & 0x80008000u;
-}
-__device__ __forceinline__ uint32_t not_finite(f16x8 v) {
-    return not_finite(__builtin_bit_cast(u32x4, v), 0x7c007c00u, 0x04000400u);
-}
-__device__ __forceinline__ uint32_t not_finite(bf16x8 v) {
-    return not_finite(__builtin_bit_cast(u32x4, v), 0x7f807f80u, 0x00800080u);
-}
-
-// A power of two that takes m > 0 into [2^14, 2^15) (clamped; any for 0, for
-// infinities and NaN), and its inverse.
+// A power of two that takes m > 0 into [2^14, 2^15) (below, where m is under
+// 2^-112; any for 0, for infinities and NaN), and its inverse.
 __device__ __forceinline__ float scale_for(float m, float& inverse) {
     int e = int((__float_as_uint(m) >> 23) & 0xff) - 127;
-    e = min(max(e, -100), 100);
+    e = min(max(e, -112), 127);
     inverse = __uint_as_float(uint32_t(e - 14 + 127) << 23);
     return __uint_as_float(uint32_t(14 - e + 127) << 23);
 }
@@ -234,6 +228,12 @@ __device__ __forceinline__ float max_of_groups(float m) {
 // loop is not kept in registers across it (some 40 LDS
 // addresses and 40 lane masks otherwise).
 __device__ __forceinline__ int fresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// The same of a tile: four registers in a row and not four values.
+__device__ __forceinline__ f32x4 fresh(f32x4 x) {
     asm volatile("" : "+v"(x));
     return x;
 }
@@ -525,34 +525,42 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     const int tokens = int(piece.t1 - piece.t0);
 
     f32x4 S[kNN];  // lane: p = lr; n = 16 i + 4 lg + element
-    float* ws = g.ws_state ? g.ws_state + ((((int64_t(id) * a.H + h) * g.ptiles + pt) * WAVES + wave) * kNN * 64 + lane) * 4
-                           : nullptr;
-    bool have_state = false;
-#pragma unroll
-    for (int i = 0; i < kNN; ++i) S[i] = f32x4{0, 0, 0, 0};
+    // Where a lane's part of the piece's state lies in the workspace.
+    auto place_of = [&](int ln) __attribute__((always_inline)) {
+        return g.ws_state + ((((int64_t(id) * a.H + h) * g.ptiles + pt) * WAVES + wave) * kNN * 64 + ln) * 4;
+    };
     const int32_t ys = a.H * a.P;  // token stride of y
     T* yb = static_cast<T*>(a.y) + ((a.cu ? 0 : int64_t(piece.seq) * a.T) + piece.t0) * int64_t(ys) + int64_t(h) * a.P + p0;
     const int64_t state_at = ((int64_t(piece.seq) * a.H + h) * a.P + p) * a.N;
-    if (MAIN && (ws || a.state_in)) {
-        have_state = true;
-        if (ws) {
+    // Lane ln's part of the state at the piece's start (contributions: 0).
+    auto load_state = [&](int ln) __attribute__((always_inline)) {
+        const int lg = ln >> 4, p = p0 + 16 * wave + (ln & 15);
+        const int64_t state_at = ((int64_t(piece.seq) * a.H + h) * a.P + p) * a.N;
 #pragma unroll
-            for (int i = 0; i < kNN; ++i)
-                if (16 * i < a.N && active) S[i] = *reinterpret_cast<const f32x4*>(ws + i * 256);
-        } else if (p < a.P) {
+        for (int i = 0; i < kNN; ++i) S[i] = f32x4{0, 0, 0, 0};
+        if constexpr (MAIN) {
+            if (g.ws_state) {
+                const float* ws = place_of(ln);
 #pragma unroll
-            for (int i = 0; i < kNN; ++i) {
-                const int n = 16 * i + 4 * lg;
-                if (g.state4) {
-                    if (n < a.N) S[i] = *reinterpret_cast<const f32x4*>(a.state_in + state_at + n);
-                } else {
+                for (int i = 0; i < kNN; ++i)
+                    if (16 * i < a.N && active) S[i] = *reinterpret_cast<const f32x4*>(ws + i * 256);
+            } else if (a.state_in && p < a.P) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (n + k < a.N) S[i][k] = a.state_in[state_at + n + k];
+                for (int i = 0; i < kNN; ++i) {
+                    const int n = 16 * i + 4 * lg;
+                    if (g.state4) {
+                        if (n < a.N) S[i] = *reinterpret_cast<const f32x4*>(a.state_in + state_at + n);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (n + k < a.N) S[i][k] = a.state_in[state_at + n + k];
+                    }
                 }
             }
         }
-    }
+    };
+    load_state(lane);
+    bool have_state = MAIN && (g.ws_state || a.state_in);
 
     Rows<E, Q, NT, kThreads> rb;
     Rows<E, Q, MAIN ? NT : 32, kThreads> rc;
@@ -601,6 +609,7 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     };
     fetch_dt(0);
     double sum = 0.0;  // of this piece's exponents
+    float wild[MAIN ? 1 : 4] = {};  // NaN once an output (contributions: the state) was not finite
     const float skip = a.D ? a.D[h] : 0.0f;
 
     for (int t0 = 0; t0 < tokens; t0 += Q) {
@@ -744,14 +753,14 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
         // all products over s.  In the outputs' layout, x of token tile tt is half of
         // it.
         V8 xf[kKS][kIn];
-        int bad = Q;  // the first token whose x is not finite
-        bool any_bad = false;
         f32x4 y[MAIN ? kTT : 1], gate[MAIN ? kTT : 1];
+        if constexpr (MAIN) {
+#pragma unroll
+            for (int tt = 0; tt < kTT; ++tt) y[tt] = f32x4{0, 0, 0, 0};
+        }
         if (active) {
             if constexpr (MAIN) {
                 // exp(run_t) C S
-#pragma unroll
-                for (int tt = 0; tt < kTT; ++tt) y[tt] = f32x4{0, 0, 0, 0};
                 if (have_state) {
                     V8 cf[2][kTT][kIn];
                     read_c(cf[0], 0);
@@ -850,43 +859,23 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                         S[kTurn * i + u][k] = Sch::kScaled ? __builtin_fmaf(d[u][k], inverse, S[kTurn * i + u][k] * whole) : d[u][k];
             }
             have_state = true;
-            if constexpr (MAIN) {
-                // The gate's inputs, in the outputs' layout.
-                if (gated) {
+        }
+        if constexpr (MAIN) {
+            // The gate's inputs, in the outputs' layout.
+            if (active && gated) {
 #pragma unroll
-                    for (int tt = 0; tt < kTT; ++tt) {
-                        if constexpr (E::kBytes == 2) {
-                            const u32x2 v = read_tr(reinterpret_cast<const uint16_t*>(m.z) +
-                                                    (16 * tt + 4 * lg + (lr >> 2)) * kZP + 16 * wave + 4 * (lr & 3));
-                            const V8 v8 = __builtin_bit_cast(V8, u32x4{v[0], v[1], 0, 0});
+                for (int tt = 0; tt < kTT; ++tt) {
+                    if constexpr (E::kBytes == 2) {
+                        const u32x2 v = read_tr(reinterpret_cast<const uint16_t*>(m.z) +
+                                                (16 * tt + 4 * lg + (lr >> 2)) * kZP + 16 * wave + 4 * (lr & 3));
+                        const V8 v8 = __builtin_bit_cast(V8, u32x4{v[0], v[1], 0, 0});
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) gate[tt][i] = silu(elem_f32(v8, i));
-                        } else {
+                        for (int i = 0; i < 4; ++i) gate[tt][i] = silu(elem_f32(v8, i));
+                    } else {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                gate[tt][i] = silu(E::to_f32(m.z[(16 * tt + 4 * lg + i) * kZP + 16 * wave + lr]));
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            gate[tt][i] = silu(E::to_f32(m.z[(16 * tt + 4 * lg + i) * kZP + 16 * wave + lr]));
                     }
-                }
-                // Tokens before one whose x is an infinity or NaN must not see
-                // it times their weight of 0: it is taken out and put back below.
-                uint32_t some = 0;
-#pragma unroll
-                for (int ks = 0; ks < kKS; ++ks) some |= not_finite(xf[ks][0]);
-                any_bad = __any(some != 0);
-                if (any_bad) {
-                    bad = fresh(bad);  // keeps this from being computed always
-#pragma unroll
-                    for (int ks = 0; ks < kKS; ++ks)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (!(fabsf(elem_f32(xf[ks][0], i)) <= 3.4028235e38f)) {
-                                bad = min(bad, 32 * ks + 16 * (i / 4) + 4 * lg + i % 4);
-#pragma unroll
-                                for (int k = 0; k < kIn; ++k) xf[ks][k][i] = {};
-                            }
-                    bad = min(bad, __shfl_xor(bad, 16));
-                    bad = min(bad, __shfl_xor(bad, 32));
                 }
             }
         }
@@ -911,12 +900,8 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
                     if constexpr (Sch::kScaled)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) d[tt][i] = __builtin_fmaf(d[tt][i], r[tt][i], y[tt][i]);
-                    if (any_bad) {
-                        const int first = fresh(bad);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (16 * tt + 4 * lg + i >= first) d[tt][i] = __builtin_nanf("");
-                    }
+                    for (int i = 0; i < 4; ++i) wild[0] = __builtin_fmaf(d[tt][i], 0.0f, wild[0]);
                     if (gated)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) d[tt][i] *= gate[tt][i];
@@ -950,11 +935,78 @@ __global__ __launch_bounds__(64 * WAVES, (ChunkShape<E, NT, Q, WAVES>::kPerSimd)
     }
 
     if (!active) return;
+    // What is not finite has spread (above): the piece again, by the recurrence as
+    // rows_kernel has it.  Lanes l ^ 16 and l ^ 32 hold other n of one p.  (What a lane
+    // needs for it is formed here: kept through the chunks it spilled registers.)
     if constexpr (!MAIN) {
 #pragma unroll
         for (int i = 0; i < kNN; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) wild[k] = __builtin_fmaf(S[i][k], 0.0f, wild[k]);
+        wild[0] = (wild[0] + wild[MAIN ? 0 : 1]) + (wild[MAIN ? 0 : 2] + wild[MAIN ? 0 : 3]);
+    }
+    if (__any(wild[0] != wild[0])) {
+        __threadfence();  // outputs are written a second time, by other lanes
+        const int ln = fresh(lane), p = p0 + 16 * wave + (ln & 15);
+        const int64_t row = min(p, a.P - 1);
+        load_state(ln);
+#pragma unroll 1
+        for (int64_t t = piece.t0; t < piece.t1; ++t) {
+            const float d = step_size(a, dt_of<E>(a, dt_bits<E>(a, a.dt, seq * a.dt_bs + t * a.dt_ts + h * a.dt_hs)), bias);
+            const float fade = expf(A * d);
+            const T* bt = static_cast<const T*>(a.B) + seq * a.b_bs + t * a.b_ts + group * a.b_gs;
+            const T* ct = static_cast<const T*>(a.C) + seq * a.c_bs + t * a.c_ts + group * a.c_gs;
+            const T x = static_cast<const T*>(a.x)[seq * a.x_bs + t * a.x_ts + h * a.x_hs + row];
+            const int n0 = 4 * fresh(ln >> 4);
+            // A token's loads at once; a vector that would pass the row's end starts
+            // earlier.
+            typename Vec<E, 4>::type b[kNN], c[MAIN ? kNN : 1];
+#pragma unroll
+            for (int i = 0; i < kNN; ++i) {
+                const int at = min(16 * i + n0, a.N - 4);
+                b[i] = *reinterpret_cast<const typename Vec<E, 4>::utype*>(bt + at);
+                if constexpr (MAIN) c[i] = *reinterpret_cast<const typename Vec<E, 4>::utype*>(ct + at);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const float xv = p < a.P ? E::to_f32(x) : 0.0f, dx = d * xv;
+            float v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kNN; ++i) {
+                const int n = 16 * i + n0, by = n - min(n, a.N - 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    T bk = b[i][k], ck = c[MAIN ? i : 0][k];
+#pragma unroll
+                    for (int j = k + 1; j < 4; ++j) {
+                        bk = by == j - k ? b[i][j] : bk;
+                        ck = by == j - k ? c[MAIN ? i : 0][j] : ck;
+                    }
+                    S[i][k] = n + k < a.N ? __builtin_fmaf(fade, S[i][k], dx * E::to_f32(bk)) : 0.0f;
+                    if constexpr (MAIN) v = n + k < a.N ? __builtin_fmaf(E::to_f32(ck), S[i][k], v) : v;
+                }
+                S[i] = fresh(S[i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (MAIN) {
+                v += __shfl_xor(v, 16);
+                v += __shfl_xor(v, 32);
+                v = __builtin_fmaf(skip, xv, v);
+                if (gated) v *= silu(E::to_f32(static_cast<const T*>(a.z)[seq * a.z_bs + t * a.z_ts + h * a.z_hs + row]));
+                if (ln < 16 && p < a.P)
+                    static_cast<T*>(a.y)[((a.cu ? 0 : int64_t(piece.seq) * a.T) + t) * ys + int64_t(h) * a.P + p] = T(v);
+            }
+        }
+    }
+    if constexpr (!MAIN) {
+        float* ws = place_of(lane);
+#pragma unroll
+        for (int i = 0; i < kNN; ++i)
             if (16 * i < a.N) *reinterpret_cast<f32x4*>(ws + i * 256) = S[i];
-        if (pt == 0 && threadIdx.x == 0) g.ws_decay[int64_t(id) * a.H + h] = __builtin_amdgcn_exp2f(float(sum));
+        if (pt == 0 && threadIdx.x == 0) {
+            // Not 0, but the least above it: an infinite state stays one.
+            const float decay = __builtin_amdgcn_exp2f(float(sum));
+            g.ws_decay[int64_t(id) * a.H + h] = decay == 0.0f ? 0x1p-149f : decay;
+        }
     } else if (piece.last && a.state_out && p < a.P) {
 #pragma unroll
         for (int i = 0; i < kNN; ++i) {
