@@ -86,9 +86,10 @@ Plan plan_of(const pe_scan_desc& d, bool packed) {
     // 4, 8, 16 pieces (chosen: *): 1 x 128 tokens, 32 heads 17* 20 20; 2 x 256, 16
     // heads 28 27 22* 25; 1 x 1024, 32 heads 105 76 47 39 38*; 2 x 4096, 64 heads 404
     // 270 182 179 184, 161 for 6*; 1 x 16384, 24 heads 1400 920 468 243 162, 121 for
-    // 32* (64 x 128 a head, 16-bit types).
+    // 32* (64 x 128 a head, 16-bit types; float32 and other heads take the same
+    // constants, of which only the hand-over's is scaled to their size).
     const int64_t seqs = packed ? 1 : d.nseq, across = d.H * p.ptiles, chunks = ceil_div(d.T, 32);
-    const double slots = 256.0 * chunks_of(d.dtype)(nullptr, p.nt, p.waves, true, nullptr);
+    const double slots = double(cu_count()) * chunks_of(d.dtype)(nullptr, p.nt, p.waves, true, nullptr);
     double best = 0.0;
     for (int64_t k = 1; k <= std::max<int64_t>(1, std::min<int64_t>(chunks / 2, 96)); ++k) {
         const int64_t piece = ceil_div(chunks, k);

@@ -74,7 +74,7 @@ constexpr int kScanTailBlocks = 64;
 struct Piece {
     int64_t t0, t1;
     int32_t seq;
-    bool first, last;
+    bool last;
 };
 
 // Piece `id`.  Packed pieces end at multiples of g.piece of the buffer and at
@@ -87,7 +87,6 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs& g, uint32_t id, Piec
         const uint32_t j = id - uint32_t(o.seq) * g.per_seq;
         o.t0 = int64_t(j) * g.piece;
         o.t1 = min(a.T, o.t0 + int64_t(g.piece));
-        o.first = j == 0;
         o.last = j + 1 == g.per_seq;
         return true;
     }
@@ -103,7 +102,6 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs& g, uint32_t id, Piec
     o.seq = lo;
     o.t0 = max(from, int64_t(j) * g.piece);
     o.t1 = min(to, (int64_t(j) + 1) * g.piece);
-    o.first = j == j0;
     o.last = to <= (int64_t(j) + 1) * g.piece;
     return o.t0 < o.t1;
 }
@@ -140,21 +138,9 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-// Sum of a_i b_j, the small ones first; of three terms each, those with i + j <= 2.
-template <int NA, int NB, typename V8>
-__device__ __forceinline__ f32x4 mma(const V8 (&a)[NA], const V8 (&b)[NB], f32x4 c) {
-#pragma unroll
-    for (int o = NA + NB - 2; o >= 0; --o) {
-        if (o > 2) continue;
-#pragma unroll
-        for (int i = 0; i < NA; ++i)
-            if (o - i >= 0 && o - i < NB) c = mfma(a[i], b[o - i], c);
-    }
-    return c;
-}
-
-// The same for T tiles at a time: their sums take turns, so that none waits for
-// its own last product.
+// Sums of a_i b_j for T tiles, the small ones first; of three terms each, those
+// with i + j <= 2.  The tiles take turns, so that none waits for its own last
+// product.
 template <int T, int NA, int NB, typename V8>
 __device__ __forceinline__ void mma(const V8 (&a)[T][NA], const V8 (&b)[NB], f32x4 (&c)[T]) {
 #pragma unroll
@@ -448,8 +434,8 @@ struct ChunkShape {
     static constexpr int kXC = WAVES == 3 ? 64 : kPT;          // columns of x's planes: a power of two
     static constexpr int kZP = kPT + 16 / E::kBytes;
     static constexpr int kTokens = 256;  // whose step sizes are prepared at a time
-    // Waves of a SIMD that the registers are held to: three hide more of the chain
-    // from LDS read to product than a few spilled registers cost.
+    // Waves of a SIMD that the registers are held to: three, which hide more of the
+    // chain from LDS read to product, where 16-bit types run without a spill then.
     static constexpr int kPerSimd = E::kBytes == 2 && NT <= 128 && (NT < 128 || WAVES > 2) ? 3 : 2;
     struct Lds {
         alignas(16) uint16_t b[kIn * Q * NT], c[kIn * Q * NT], x[kIn * Q * kXC], p[kOut * Q * Q];
