@@ -18,8 +18,9 @@
 //
 //   float16:  0x6400 | q is 1024 + q; minus 1032, q - 8 exactly.
 //   bfloat16: 0x4300 | q is 128 + q, used as it is, with z + 128: what the float32
-//             sums lose by it, 2^-24 of 136 |x| a product, is far below the
-//             result's own rounding.
+//             sums lose by it, 2^-24 of (128 + q) |s x| a product, is far below the
+//             result's own rounding, except where a row's weights are all 0: then
+//             the result is that small, not 0.
 //   float32:  q through float32, whose upper half is q in bfloat16; x is cut into
 //             three bfloat16 terms, exactly: of 2^24 x, since bfloat16 has no bits below
 //             2^-133 and the matrix cores lose subnormals (x of 2^-124: 6e-4 of the
@@ -29,11 +30,11 @@
 // times x (whole_weights).
 //
 // 16 tokens, 16384 x 8192 bfloat16 in groups of 64, three sets of weights in turn:
-// 20.7 us, 3.7 TB/s (75 with 4-byte loads and no step ahead; 24 with a branch
+// 20.8 us, 3.7 TB/s (75 with 4-byte loads and no step ahead; 24 with a branch
 // around the loads ahead and a stretch of K for each wave); eight sets, which no
-// cache holds: 29 us, 2.3 TB/s, one token 27.  One block of eight waves a CU has
-// too little on its way for more.  One token, 4096 x 4096: 6.4 us of a call of
-// 9.4, which the host's part bounds.
+// cache holds: 30 us, 2.2 TB/s, one token 27.  One block of eight waves a CU has
+// too little on its way for more.  One token, 4096 x 4096: 6.6 us of a call of
+// 9.5, which the host's part bounds.
 #include "pe_ssm.h"
 
 #include <algorithm>

@@ -44,8 +44,8 @@
 // 600 vector instructions on a chunk (splitting S and the weighted x into terms,
 // fading S, weights, gates) beside 40 matrix instructions, three waves a SIMD.  Two
 // prompts of 4096 tokens, 64 heads of 64 x 128, float16: contributions 40 us, states
-// 9, outputs 122, a call of 155; 1 x 16384, 24 heads, bfloat16: 31, 10, 88, a call
-// of 118 to 130 (token by token 15.2 and 55.6 ms).  Chunks of 64 tokens halve what is done
+// 9, outputs 126, a call of 155; 1 x 16384, 24 heads, bfloat16: 32, 11, 88, a call
+// of 119 to 129 (token by token 15.2 and 55.6 ms).  Chunks of 64 tokens halve what is done
 // once a chunk but leave two waves a SIMD: 17 % longer.
 #pragma once
 

@@ -12,7 +12,7 @@
 //
 // One token of 128 sequences, 64 heads of 64 x 128: 537 MB of states read and
 // written in 106 us, 5.1 TB/s (a large copy moves 5.1 to 6.5 here).  Of one
-// sequence, 32 heads: 6.7 us, of a call of 13.
+// sequence, 32 heads: 6.6 to 7 us, of a call of 13.
 #include "pe_scan.h"
 
 namespace pe {
