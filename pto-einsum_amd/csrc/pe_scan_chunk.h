@@ -31,8 +31,8 @@
 // Operands of 16 bits enter as they are.  So a float16 scan's new states are good to
 // 2^-21 of their inputs (their sums are float32), and float32 values below 2^-110
 // lose bits: the last term of 2^-120 lies under what the matrix cores keep, 6e-4.
-// Sums are float32; run_t is summed in 64
-// bits and kept as two float32, since differences of large sums count.
+// Sums are float32; run_t is summed in 64 bits and kept as two float32, since
+// differences of large sums count.
 //
 // Infinities and NaN spread through terms and through weights of 0 to tokens and
 // elements that the recurrence keeps clear of them, and C B^T can pass float32's
