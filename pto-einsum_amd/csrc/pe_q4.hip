@@ -129,16 +129,22 @@ __device__ __forceinline__ void operand(const __bf16* p, bf16x8 (&o)[1]) {
     o[0] = __builtin_bit_cast(bf16x8, t[0]);
 }
 __device__ __forceinline__ void operand(const float* p, bf16x8 (&o)[3]) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+    u32x4 t[3];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float r = i < 4 ? a[i & 3] : b[i & 3];
-        o[0][i] = (__bf16)r;
-        r -= (float)o[0][i];
-        o[1][i] = (__bf16)r;
-        r -= (float)o[1][i];
-        o[2][i] = (__bf16)r;
+    for (int i = 0; i < 4; ++i) {   // two at a time: one conversion
+        f32x2 r = i < 2 ? f32x2{a[(2 * i) & 3], a[(2 * i + 1) & 3]} : f32x2{b[(2 * i) & 3], b[(2 * i + 1) & 3]};
+#pragma unroll
+        for (int c = 0; c < 3; ++c) {
+            t[c][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+            r[0] -= __uint_as_float(t[c][i] << 16);
+            r[1] -= __uint_as_float(t[c][i] & 0xffff0000u);
+        }
     }
+#pragma unroll
+    for (int c = 0; c < 3; ++c) o[c] = __builtin_bit_cast(bf16x8, t[c]);
 }
 
 // 16 bytes of a row at byte `at`, those past its end 0.
