@@ -443,9 +443,17 @@ int launch(const Q4Args& g, hipStream_t stream) {
         const int each = std::max(1, int(ceil_div(steps, kWaves<E, MT, NT>)));   // of a wave
         const int waves = std::max(1, int(ceil_div(steps, each)));
         const int64_t cols = ceil_div(g.N, 16 * NT);
-        if (tall > 65535 || tall * cols * 64 * waves >= (int64_t(1) << 32))
-            return fail(PE_ERR_UNSUPPORTED, "matvec_q4: too many rows");
-        q4_kernel<E, GROUP, MT, NT><<<dim3{uint32_t(cols), uint32_t(tall)}, 64 * waves, 0, stream>>>(g);
+        // Rows of x that a launch holds (65535 tiles along an axis, fewer than 2^32
+        // threads), and as many launches as they need.
+        const int64_t tiles = std::min<int64_t>(65535, ((int64_t(1) << 32) - 1) / (cols * 64 * waves));
+        if (tiles < 1) return fail(PE_ERR_UNSUPPORTED, "matvec_q4: too many weight rows");
+        for (int64_t m = 0; m < g.M; m += tiles * 16 * MT) {
+            Q4Args part = g;
+            part.x = static_cast<const typename E::T*>(g.x) + m * g.x_ms;
+            part.y = static_cast<typename E::T*>(g.y) + m * g.N;
+            part.M = int32_t(std::min<int64_t>(g.M - m, tiles * 16 * MT));
+            q4_kernel<E, GROUP, MT, NT><<<dim3{uint32_t(cols), uint32_t(ceil_div(part.M, 16 * MT))}, 64 * waves, 0, stream>>>(part);
+        }
         return hip_status_of_launch("matvec_q4");
     };
     using std::integral_constant;
