@@ -38,8 +38,9 @@ enum pe_status {
     PE_ERR_WORKSPACE = -4    /* workspace missing or too small */
 };
 
-/* PE_BF16: the state-space operators and the 4-bit product only. */
-enum pe_dtype { PE_F32 = 0, PE_F16 = 1, PE_BF16 = 2 };
+/* PE_BF16: the state-space operators, the norms and the products with weights of
+ * few bits only.  PE_I8: x of the 8-bit product only. */
+enum pe_dtype { PE_F32 = 0, PE_F16 = 1, PE_BF16 = 2, PE_I8 = 3 };
 
 /* Contraction-free product over a row-major float32 output:
  *   out[o] = (add_zero ? 0.0f + a*b : a*b),  a = (float)in0[sum_d o_d*a_stride[d]],
@@ -303,6 +304,65 @@ typedef struct pe_q4_desc {
 
 int pe_matvec_q4(const pe_q4_desc* d, const void* x, const void* packed, const void* scales, const void* zeros,
                  void* y, void* stream);
+
+/* ---- between two blocks: norms with gate and residual, rows in 8 bits ----
+ * No counterpart in the reference.  Rows of D contiguous elements lie at
+ * rows0 x rows1 places (a tensor's leading axes, collapsed to two; strides in
+ * elements, 0 where a gate or residual is shared by them).  Sums, norms and
+ * gates are float32; each output is rounded once.  Outputs are contiguous,
+ * [rows][D], and overlap no operand.
+ *
+ * A row in 8 bits: a = max |v|, scale = a / 127 (float32), q = the whole number
+ * nearest to 127 v / a, ties to even, as the exact quotient decides; a = 0 gives
+ * scale 0 and zeros, a row with an infinity or NaN the scale NaN and zeros.  Rows
+ * in 8 bits lie q_ms bytes apart, D rounded up to 16, the bytes between zero. */
+typedef struct pe_rows_desc {
+    int32_t dtype;                      /* of x, weights, gate and y */
+    int32_t res_dtype;                  /* of the residual: dtype or PE_F32 */
+    int32_t norm_first;                 /* gated_norm: the gate multiplies the norm's result */
+    int32_t gate_row;                   /* residual_norm: one gate for a row */
+    int64_t rows0, rows1, D;
+    int64_t groups;                     /* gated_norm: norms of D / groups elements each (others: 1) */
+    int64_t x_s0, x_s1, g_s0, g_s1, r_s0, r_s1;
+    int64_t q_ms;                       /* rows in 8 bits */
+    int64_t x_numel, g_numel, r_numel;
+    float eps, scale;                   /* scale: of the residual sum */
+} pe_rows_desc;
+
+int pe_quantize_q8(const pe_rows_desc* d, const void* x, int8_t* q, float* scales, void* stream);
+/* u = x * silu(z), y = u / sqrt(mean(u^2) + eps) * weight, or with norm_first
+ * y = x / sqrt(mean(x^2) + eps) * weight * silu(z); weight [D] and z may be NULL.
+ * With scales, y goes to rows in 8 bits (q, scales) instead; at most 8192 groups. */
+int pe_gated_norm(const pe_rows_desc* d, const void* x, const void* weight, const void* z, void* y, int8_t* q,
+                  float* scales, void* stream);
+/* u = x, or x / sqrt(mean(x^2) + eps) * post_weight if that is given;
+ * r = residual + scale * (gate * u); y = r / sqrt(mean(r^2) + eps) * weight, from r
+ * before it is rounded to new_residual (res_dtype).  weight [D], post_weight [D]
+ * and gate may be NULL; with scales, y goes to rows in 8 bits instead. */
+int pe_residual_norm(const pe_rows_desc* d, const void* x, const void* residual, const void* weight,
+                     const void* post_weight, const void* gate, void* y, void* new_residual, int8_t* q,
+                     float* scales, void* stream);
+
+/* y[m, n] = x_scales[m] * w_scales[n] * sum_k x[m, k] * w[n, k] + bias[n], sums in
+ * 32-bit whole numbers (exact: K <= 131071), then float32, rounded once to
+ * y_dtype.  w is PE_I8, x PE_I8 with x_scales, or another type whose rows are
+ * first taken to 8 bits in the workspace (x_scales is not read).  Rows in 8 bits
+ * start on 16 bytes and lie a multiple of 16 bytes apart, at most 2^23; whole
+ * 16-byte groups of them are read, whatever the bytes behind K hold (x_numel and
+ * w_numel cover these).  bias may be NULL; y is [M][N] contiguous. */
+typedef struct pe_q8_desc {
+    int32_t x_dtype, y_dtype;
+    int32_t bias_dtype;                 /* y_dtype or PE_F32 */
+    int32_t reserved;                   /* must be 0 */
+    int64_t M, N, K;
+    int64_t x_ms, w_ns;                 /* row strides */
+    int64_t x_numel, w_numel;
+} pe_q8_desc;
+
+/* Bytes of the workspace (16-byte aligned) that pe_matmul_q8 needs; 0: none. */
+int64_t pe_matmul_q8_workspace_bytes(const pe_q8_desc* d);
+int pe_matmul_q8(const pe_q8_desc* d, const void* x, const float* x_scales, const void* w, const float* w_scales,
+                 const void* bias, void* y, void* ws, int64_t ws_bytes, void* stream);
 
 /* Plan executor: the body of every per-shape run_einsum_exec.  Every
  * workspace region a plan uses is written before it is read, so a workspace

@@ -1,0 +1,336 @@
+// Norms between blocks and rows in 8 bits (gfx950): one pass over each row.
+//
+//   quantize:  q, scale of x                                (pe_rows.h)
+//   gated:     u = x silu(z), y = u / sqrt(mean u^2 + eps) w, or with norm_first
+//              y = x / sqrt(mean x^2 + eps) w silu(z); the mean over each group
+//   residual:  u = x, or x / sqrt(mean x^2 + eps) pw;  r = res + scale gate u;
+//              y = r / sqrt(mean r^2 + eps) w; y comes of r before r is rounded
+//
+// y is rounded once to the type, or goes to rows in 8 bits from float32.  What
+// bounds these is memory: each value is read once into registers, the sums go
+// over the lanes of a row's threads, and the row is written from the registers.
+// TPR threads take a row, NV chunks of eight elements each; a wave alone needs no
+// barrier, and short rows share a block.  Rows too long for the registers, and
+// rows in 8 bits of a grouped norm (whose scale spans the groups), go to a kernel
+// that reads the row again for each step: from the caches, mostly.
+#pragma once
+
+#include "pe_rows.h"
+
+namespace pe {
+namespace rows {
+namespace {
+
+using ssm::load_f32;
+using ssm::silu;
+using ssm::store_f32;
+
+// A chunk as it lies in memory, so that loads go out together and take half the
+// registers in 16 bits.
+template <typename E>
+struct Raw {
+    typename ssm::Vec<E, kChunk>::type v;
+    __device__ __forceinline__ void load(const void* base, int64_t at, int n) {
+        const typename E::T* p = static_cast<const typename E::T*>(base) + at;
+        if (n >= kChunk) {
+            v = *reinterpret_cast<const typename ssm::Vec<E, kChunk>::utype*>(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) v[i] = i < n ? p[i] : (typename E::T)0.0f;
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const { return E::to_f32(v[i]); }
+};
+
+// Sum, and maximum of magnitudes, over the TPR threads of a row.
+template <int TPR>
+struct Across {
+    static constexpr int WAVES = TPR / 64;
+    uint32_t* slots;                  // two sets of WAVES words, used in turn
+    int turn = 0;
+    template <typename F>
+    __device__ __forceinline__ uint32_t over(uint32_t v, F f) {
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) v = f(v, uint32_t(__shfl_xor(int(v), m)));
+        if constexpr (WAVES > 1) {
+            uint32_t* s = slots + turn * WAVES;
+            turn ^= 1;
+            if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = s[0];
+#pragma unroll
+            for (int i = 1; i < WAVES; ++i) v = f(v, s[i]);
+        }
+        return v;
+    }
+    __device__ __forceinline__ float sum(float v) {
+        return __uint_as_float(over(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+            return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+        }));
+    }
+    __device__ __forceinline__ uint32_t most(uint32_t v) {
+        return over(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    }
+};
+
+__device__ __forceinline__ float inv_rms(float sum, float D, float eps) { return 1.0f / sqrtf(sum / D + eps); }
+
+// Where a unit's values start.
+struct Place {
+    int64_t x, g, r, y;               // y: in the contiguous outputs
+    int64_t row;
+    int32_t w;                        // first element of the unit in its row
+    __device__ __forceinline__ Place(const NormArgs& a, uint32_t unit) {
+        uint32_t rw, gr, o, i;
+        a.groups.divmod(unit, rw, gr);
+        a.inner.divmod(rw, o, i);
+        row = rw;
+        w = int32_t(gr) * a.D;
+        x = int64_t(o) * a.x0 + int64_t(i) * a.x1 + w;
+        g = int64_t(o) * a.g0 + int64_t(i) * a.g1 + (a.g_ds ? w : 0);
+        r = int64_t(o) * a.r0 + int64_t(i) * a.r1 + w;
+        y = int64_t(unit) * a.D;
+    }
+};
+
+template <typename E, typename R, int OP, bool Q, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a) {
+    constexpr int THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR;
+    __shared__ uint32_t slots[2 * (TPR / 64)];
+    Across<TPR> across{slots};
+    const int tid = threadIdx.x % TPR;
+    const bool gate = a.g != nullptr, post = a.pw != nullptr, scaled = a.w != nullptr;
+    for (uint64_t unit = uint64_t(blockIdx.x) * RPB + threadIdx.x / TPR; unit < a.units;
+         unit += uint64_t(gridDim.x) * RPB) {
+        const Place at(a, uint32_t(unit));
+        Raw<E> x[NV], g[NV], w[NV], pw[NV];
+        Raw<R> res[NV];
+        float one = 1.0f;             // the row's own gate
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = kChunk * (tid + j * TPR), n = a.D - e;
+            x[j].load(a.x, at.x + e, n);
+            if constexpr (OP == kResidual) res[j].load(a.res, at.r + e, n);
+            if (OP != kQuantize && gate && a.g_ds) g[j].load(a.g, at.g + e, n);
+            if (OP == kResidual && post) pw[j].load(a.pw, e, n);
+            if (OP != kQuantize && scaled) w[j].load(a.w, at.w + e, n);
+        }
+        if (OP == kResidual && gate && !a.g_ds) one = E::to_f32(static_cast<const typename E::T*>(a.g)[at.g]);
+        float v[NV][kChunk];
+        if constexpr (OP == kResidual) {
+            float inv = 1.0f;
+            if (post) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int i = 0; i < kChunk; ++i) ss = fmaf(x[j][i], x[j][i], ss);
+                inv = inv_rms(across.sum(ss), float(a.D), a.eps);
+            }
+            float ss = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int e = kChunk * (tid + j * TPR), n = a.D - e;
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) {
+                    float u = x[j][i];
+                    if (post) u = u * inv * pw[j][i];
+                    if (gate) u *= a.g_ds ? g[j][i] : one;
+                    v[j][i] = res[j][i] + a.scale * u;
+                    // (Lanes past the row hold x = 0, but a gate or a norm of
+                    // its own may be infinite.)
+                    if (n < kChunk && i >= n) v[j][i] = 0.0f;
+                    ss = fmaf(v[j][i], v[j][i], ss);
+                }
+                store_f32<R, kChunk>(static_cast<typename R::T*>(a.r) + at.y + e, n, v[j]);
+            }
+            inv = inv_rms(across.sum(ss), float(a.D), a.eps);
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) {
+                    v[j][i] *= inv;
+                    if (scaled) v[j][i] *= w[j][i];
+                }
+        } else if constexpr (OP == kGated) {
+            const bool first = gate && !a.norm_first;
+            float ss = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) {
+                    v[j][i] = x[j][i];
+                    if (first) v[j][i] *= silu(g[j][i]);
+                    ss = fmaf(v[j][i], v[j][i], ss);
+                }
+            const float inv = inv_rms(across.sum(ss), float(a.D), a.eps);
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) {
+                    v[j][i] *= inv;
+                    if (scaled) v[j][i] *= w[j][i];
+                    if (gate && a.norm_first) v[j][i] *= silu(g[j][i]);
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) v[j][i] = x[j][i];
+        }
+        if constexpr (Q) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) {
+                    // (values past the row count for nothing, whatever they are)
+                    if (kChunk * (tid + j * TPR) + i >= a.D) v[j][i] = 0.0f;
+                    const uint32_t b = magnitude(v[j][i]);
+                    top = b > top ? b : top;
+                }
+            const Quant qt(across.most(top));
+            if (tid == 0) a.qs[at.row] = qt.scale();
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int e = kChunk * (tid + j * TPR);
+                if (e < a.q_ms) store_q8(a.q + at.row * a.q_ms + e, qt, v[j]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int e = kChunk * (tid + j * TPR);
+                store_f32<E, kChunk>(static_cast<typename E::T*>(a.y) + at.y + e, a.D - e, v[j]);
+            }
+        }
+    }
+}
+
+// Any length: the values are formed again, element by element, for each step.
+// `parts` groups within the unit (rows in 8 bits of a grouped norm), whose
+// factors lie in LDS.
+constexpr int kLongThreads = 512;
+
+template <typename E, typename R, int OP, bool Q>
+__global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
+    __shared__ uint32_t slots[2 * (kLongThreads / 64)];
+    extern __shared__ float factor[];  // [parts]
+    Across<kLongThreads> across{slots};
+    const int tid = threadIdx.x;
+    const int part = a.D / a.parts;
+    const bool gate = a.g != nullptr, post = a.pw != nullptr, scaled = a.w != nullptr;
+    for (uint64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        const Place at(a, uint32_t(unit));
+        auto get = [](const void* p, int64_t i, auto e) { return decltype(e)::to_f32(static_cast<const typename decltype(e)::T*>(p)[i]); };
+        float inv0 = 1.0f;            // of the norm of x, in the residual
+        auto value = [&](int e) {
+            float u = get(a.x, at.x + e, E{});
+            if constexpr (OP == kResidual) {
+                if (post) u = u * inv0 * get(a.pw, e, E{});
+                if (gate) u *= get(a.g, at.g + (a.g_ds ? e : 0), E{});
+                u = get(a.res, at.r + e, R{}) + a.scale * u;
+            } else if constexpr (OP == kGated) {
+                if (gate && !a.norm_first) u *= silu(get(a.g, at.g + e, E{}));
+            }
+            return u;
+        };
+        if constexpr (OP == kResidual) {
+            if (post) {
+                float ss = 0.0f;
+                for (int e = tid; e < a.D; e += kLongThreads) {
+                    const float u = get(a.x, at.x + e, E{});
+                    ss = fmaf(u, u, ss);
+                }
+                inv0 = inv_rms(across.sum(ss), float(a.D), a.eps);
+            }
+        }
+        if constexpr (OP != kQuantize) {
+            if (a.parts == 1) {
+                float ss = 0.0f;
+                for (int e = tid; e < a.D; e += kLongThreads) {
+                    const float u = value(e);
+                    if constexpr (OP == kResidual) static_cast<typename R::T*>(a.r)[at.y + e] = (typename R::T)u;
+                    ss = fmaf(u, u, ss);
+                }
+                const float inv = inv_rms(across.sum(ss), float(a.D), a.eps);
+                if (tid == 0) factor[0] = inv;
+            } else {
+                for (int p = tid >> 6; p < a.parts; p += kLongThreads / 64) {
+                    float ss = 0.0f;
+                    for (int e = tid & 63; e < part; e += 64) {
+                        const float u = value(p * part + e);
+                        ss = fmaf(u, u, ss);
+                    }
+                    const float inv = inv_rms(Across<64>{nullptr}.sum(ss), float(part), a.eps);
+                    if ((tid & 63) == 0) factor[p] = inv;
+                }
+            }
+            __syncthreads();
+        }
+        auto result = [&](int e) {
+            float u = value(e);
+            if constexpr (OP != kQuantize) {
+                u *= factor[a.parts == 1 ? 0 : e / part];
+                if (scaled) u *= get(a.w, at.w + e, E{});
+                if (OP == kGated && gate && a.norm_first) u *= silu(get(a.g, at.g + e, E{}));
+            }
+            return u;
+        };
+        if constexpr (Q) {
+            uint32_t top = 0;
+            for (int e = tid; e < a.D; e += kLongThreads) {
+                const uint32_t b = magnitude(result(e));
+                top = b > top ? b : top;
+            }
+            const Quant qt(across.most(top));
+            if (tid == 0) a.qs[at.row] = qt.scale();
+            for (int e = tid; e < a.q_ms; e += kLongThreads)
+                a.q[at.row * a.q_ms + e] = e < a.D ? int8_t(qt.of(result(e))) : int8_t(0);
+        } else {
+            for (int e = tid; e < a.D; e += kLongThreads)
+                static_cast<typename E::T*>(a.y)[at.y + e] = (typename E::T)result(e);
+        }
+        // (the next unit's factors are written behind this unit's reads)
+        __syncthreads();
+    }
+}
+
+// Rows of at most this many elements pass through registers.
+constexpr int kLongest = 1024 * 2 * kChunk;
+constexpr int64_t kMostBlocks = int64_t(1) << 20;
+
+template <typename E, typename R, int OP, bool Q>
+int launch(const NormArgs& a, hipStream_t stream) {
+    if (a.parts > 1 || a.D > kLongest) {
+        const uint32_t grid = uint32_t(std::min<int64_t>(a.units, kMostBlocks));
+        norm_long_kernel<E, R, OP, Q><<<grid, kLongThreads, sizeof(float) * a.parts, stream>>>(a);
+        return ssm::hip_status_of_launch("norm");
+    }
+    auto go = [&](auto t, auto v) {
+        constexpr int TPR = t(), NV = v(), THREADS = TPR < 256 ? 256 : TPR;
+        const uint32_t grid = uint32_t(std::min<int64_t>(ceil_div(a.units, THREADS / TPR), kMostBlocks));
+        norm_kernel<E, R, OP, Q, TPR, NV><<<grid, THREADS, 0, stream>>>(a);
+        return ssm::hip_status_of_launch("norm");
+    };
+    using std::integral_constant;
+    const integral_constant<int, 1> one{};
+    const integral_constant<int, 2> two{};
+    if (a.D <= 64 * kChunk) return go(integral_constant<int, 64>{}, one);
+    if (a.D <= 128 * kChunk) return go(integral_constant<int, 64>{}, two);
+    if (a.D <= 256 * kChunk) return go(integral_constant<int, 256>{}, one);
+    if (a.D <= 512 * kChunk) return go(integral_constant<int, 256>{}, two);
+    if (a.D <= 1024 * kChunk) return go(integral_constant<int, 1024>{}, one);
+    return go(integral_constant<int, 1024>{}, two);
+}
+
+template <typename E>
+int launch_type(Op op, bool q8, bool wide, const NormArgs& a, hipStream_t stream) {
+    if (op == kQuantize) return launch<E, E, kQuantize, true>(a, stream);
+    if (op == kGated) return q8 ? launch<E, E, kGated, true>(a, stream) : launch<E, E, kGated, false>(a, stream);
+    if (wide) return q8 ? launch<E, F32, kResidual, true>(a, stream) : launch<E, F32, kResidual, false>(a, stream);
+    return q8 ? launch<E, E, kResidual, true>(a, stream) : launch<E, E, kResidual, false>(a, stream);
+}
+
+}  // namespace
+}  // namespace rows
+}  // namespace pe

@@ -1,0 +1,12 @@
+// Norms and rows in 8 bits of float16 values.
+#include "pe_norm.h"
+
+namespace pe {
+namespace rows {
+
+int norm_launch_f16(Op op, bool q8, bool wide, const NormArgs& a, hipStream_t stream) {
+    return launch_type<F16>(op, q8, wide, a, stream);
+}
+
+}  // namespace rows
+}  // namespace pe

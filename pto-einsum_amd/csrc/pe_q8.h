@@ -1,0 +1,55 @@
+// Products of rows in 8 bits (gfx950): what its kernels share.
+//
+//   y[m, n] = xs[m] ws[n] sum_k x[m, k] w[n, k] + bias[n]
+//
+// Sums are whole numbers in 32 bits, exact for K up to 131071 (128 * 128 * K <
+// 2^31), so the order and the split of a sum change nothing; one conversion, two
+// multiplications and an addition in float32 follow, then the rounding to the
+// result's type.  x and w are both contiguous along k, rows on 16 bytes, and a
+// 16-byte group of k is what a lane hands to v_mfma_i32_16x16x64_i8 (lane l: row
+// l % 16, k 16 (l / 16) .. + 15; both operands alike, so any fixed order of k
+// would do).  w is the first operand: a lane's four sums are four neighbouring
+// columns of y.
+#pragma once
+
+#include "pe_rows.h"
+
+namespace pe {
+namespace q8 {
+
+using ssm::BF16;
+
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
+struct Q8Args {
+    const int8_t *x, *w;
+    const float *xs, *ws;
+    const void* bias;
+    void* y;
+    int32_t* part;                    // sums of the K splits [splits][M][N] (null: none)
+    int64_t x_ms, w_ns;
+    int32_t M, N, K;
+    int32_t bias_f32;
+    int32_t splits, split_slabs;      // K splits, and 64-byte slabs of each
+    int32_t tiles_m, tiles_n;
+};
+
+// Four neighbouring columns of a row of y from their sums.
+template <typename E>
+__device__ __forceinline__ void finish(const Q8Args& g, int m, int n, i32x4 acc) {
+    const float sx = g.xs[m];
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = min(n + i, g.N - 1);
+        v[i] = float(acc[i]) * sx * g.ws[c];
+        if (g.bias) v[i] += g.bias_f32 ? static_cast<const float*>(g.bias)[c]
+                                       : E::to_f32(static_cast<const typename E::T*>(g.bias)[c]);
+    }
+    ssm::store_f32<E, 4>(static_cast<typename E::T*>(g.y) + int64_t(m) * g.N + n, g.N - n, v);
+}
+
+int tile_launch(int y_dtype, Q8Args& g, hipStream_t stream);
+
+}  // namespace q8
+}  // namespace pe

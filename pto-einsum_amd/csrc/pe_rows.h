@@ -1,0 +1,96 @@
+// Rows in 8 bits: which whole number stands for a value, shared by the row
+// quantiser and the norms that answer with such rows.
+//
+//   a = max |v| of the row,  scale = a / 127 (rounded once to float32),
+//   q = 127 v / a rounded to the nearest whole number, ties to even.
+//
+// The rounding is that of the exact quotient, not of some float32 form of it:
+// half-way values are common (v = a / 2 is always one, 63.5), and forms that
+// differ by a unit in the last place would answer 63 here and 64 there.
+#pragma once
+
+#include "pe_ssm.h"
+
+namespace pe {
+namespace rows {
+
+using ssm::BF16;
+
+constexpr int kChunk = 8;             // elements a lane takes at once: 16 bytes of 16-bit types
+
+// A row's largest absolute value is kept as the bits of |v|: whole numbers order
+// like the values, infinities above them and NaN above those, so neither gets
+// lost in the maximum.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+struct Quant {
+    float amax, inv;                  // inv = 127 / amax, a little off
+    bool none, exactly;
+    __device__ __forceinline__ explicit Quant(uint32_t bits) {
+        none = bits == 0 || bits >= 0x7f800000u;
+        amax = __uint_as_float(bits);
+        // (where 127 / amax overflows float32 every value goes the exact way)
+        exactly = amax < 1e-36f;
+        inv = none || exactly ? 0.0f : 127.0f / amax;
+    }
+    // NaN for a row that holds one or an infinity, so that no finite result comes
+    // of it.
+    __device__ __forceinline__ float scale() const {
+        return __float_as_uint(amax) >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : amax / 127.0f;
+    }
+    // v * inv is off by less than 127 * 1.5 * 2^-23 = 2.3e-5, so only where it
+    // lies that close to a half can the exact quotient round elsewhere: those
+    // values are divided in 64 bits, where 127 v is exact and the quotient of
+    // float32 values is never within an ulp of a half unless it is one.
+    __device__ __forceinline__ int of(float v) const {
+        const float t = v * inv, n = rintf(t);
+        if (__builtin_expect(exactly || fabsf(t - n) > 0.5f - 3.1e-5f, 0))
+            return none ? 0 : int(rint(127.0 * double(v) / double(amax)));
+        return none ? 0 : int(n);
+    }
+};
+
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+    return uint32_t(a & 255) | uint32_t(b & 255) << 8 | uint32_t(c & 255) << 16 | uint32_t(d) << 24;
+}
+
+// Eight values as bytes at q (8-byte aligned).
+__device__ __forceinline__ void store_q8(int8_t* q, const Quant& qt, const float (&v)[kChunk]) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 o;
+    o[0] = pack4(qt.of(v[0]), qt.of(v[1]), qt.of(v[2]), qt.of(v[3]));
+    o[1] = pack4(qt.of(v[4]), qt.of(v[5]), qt.of(v[6]), qt.of(v[7]));
+    *reinterpret_cast<u32x2*>(q) = o;
+}
+
+// Bytes from one row in 8 bits to the next, as the quantisers lay them out and
+// as the product reads them.
+inline int64_t row_bytes(int64_t k) { return ceil_div(k, 16) * 16; }
+
+// What the operators are (pe_norm.hip): rows in 8 bits, a norm with a gate, and a
+// norm behind a residual sum.
+enum Op { kQuantize, kGated, kResidual };
+
+struct NormArgs {
+    const void *x, *w, *pw, *g, *res;  // g: z of the gated norm, the gate of the residual one
+    void *y, *r;
+    int8_t* q;
+    float* qs;
+    int64_t x0, x1, g0, g1, r0, r1;   // strides of the two leading axes
+    int64_t q_ms;
+    uint32_t units;                   // rows times groups
+    FastDiv inner, groups;            // extent of the second leading axis; groups a unit is one of
+    int32_t D;                        // elements of a unit
+    int32_t parts;                    // groups within a unit (rows in 8 bits of a grouped norm)
+    int32_t g_ds;                     // 0: one gate for a row
+    int32_t norm_first;
+    int32_t nt;                       // streaming stores
+    float eps, scale;
+};
+
+int norm_launch_f16(Op op, bool q8, bool wide, const NormArgs& a, hipStream_t stream);
+int norm_launch_bf16(Op op, bool q8, bool wide, const NormArgs& a, hipStream_t stream);
+int norm_launch_f32(Op op, bool q8, bool wide, const NormArgs& a, hipStream_t stream);
+
+}  // namespace rows
+}  // namespace pe

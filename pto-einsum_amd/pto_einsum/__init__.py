@@ -17,6 +17,11 @@ Beyond the reference's surface:
     selective_scan(x, dt, A, B, C, ...)     -> state-space scan of prompts, and
     selective_scan_step(x, ..., state)         the same for one token, its state in place
     matvec_q4(x, packed, scales, ...)       -> product of few rows with 4-bit weights
+    matmul_q8(x, weight, scales, ...)       -> product in 8-bit integers, a scale for each row
+    quantize_q8(x)                          -> rows of x in 8 bits and their scales
+    gated_norm(x, weight, z, ...)           -> norm of groups of channels with its gate
+    residual_norm(x, residual, weight, ...) -> a block's norm, gate and residual sum, and the
+                                               next block's norm
     StageGraph(fn)                          -> fn's launches captured into one HIP graph
 
 Example:
@@ -27,9 +32,11 @@ Example:
 from .builder import EinsumBuilder, INCLUDE_DIR, einsum
 from .graph import StageGraph
 from .linattn import linear_attention
-from .quant import matvec_q4
+from .norm import gated_norm, quantize_q8, residual_norm
+from .quant import matmul_q8, matvec_q4
 from .ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 
 __all__ = ["einsum", "EinsumBuilder", "INCLUDE_DIR", "linear_attention", "StageGraph", "causal_conv",
-           "causal_conv_step", "selective_scan", "selective_scan_step", "matvec_q4"]
+           "causal_conv_step", "selective_scan", "selective_scan_step", "matvec_q4",
+           "matmul_q8", "quantize_q8", "gated_norm", "residual_norm"]
 __version__ = "0.2.0"

@@ -83,6 +83,18 @@ class Q4Desc(ctypes.Structure):
                 + [(f, ctypes.c_int64) for f in ("M", "N", "K", "x_ms", "x_numel")])
 
 
+class RowsDesc(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_int32) for f in ("dtype", "res_dtype", "norm_first", "gate_row")]
+                + [(f, ctypes.c_int64) for f in ("rows0", "rows1", "D", "groups", "x_s0", "x_s1", "g_s0", "g_s1", "r_s0",
+                                                 "r_s1", "q_ms", "x_numel", "g_numel", "r_numel")]
+                + [("eps", ctypes.c_float), ("scale", ctypes.c_float)])
+
+
+class Q8Desc(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_int32) for f in ("x_dtype", "y_dtype", "bias_dtype", "reserved")]
+                + [(f, ctypes.c_int64) for f in ("M", "N", "K", "x_ms", "w_ns", "x_numel", "w_numel")])
+
+
 def _set(arr, values: Sequence[int]):
     for i, v in enumerate(values):
         arr[i] = int(v)
@@ -170,6 +182,12 @@ def bind(lib=None):
     lib.pe_selective_scan_workspace_bytes.restype = ctypes.c_int64
     lib.pe_selective_scan_step.argtypes = [ctypes.POINTER(ScanDesc)] + [vp] * 12
     lib.pe_matvec_q4.argtypes = [ctypes.POINTER(Q4Desc)] + [vp] * 6
+    lib.pe_quantize_q8.argtypes = [ctypes.POINTER(RowsDesc)] + [vp] * 4
+    lib.pe_gated_norm.argtypes = [ctypes.POINTER(RowsDesc)] + [vp] * 7
+    lib.pe_residual_norm.argtypes = [ctypes.POINTER(RowsDesc)] + [vp] * 10
+    lib.pe_matmul_q8.argtypes = [ctypes.POINTER(Q8Desc)] + [vp] * 7 + [ctypes.c_int64, vp]
+    lib.pe_matmul_q8_workspace_bytes.argtypes = [ctypes.POINTER(Q8Desc)]
+    lib.pe_matmul_q8_workspace_bytes.restype = ctypes.c_int64
     lib.pe_probe_mfma.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int64, vp, ctypes.c_int64, vp]
     lib.pe_probe_mfma_flops.argtypes = [ctypes.c_int, ctypes.c_int64]
     lib.pe_probe_mfma_flops.restype = ctypes.c_int64
@@ -178,6 +196,6 @@ def bind(lib=None):
     for f in ("pe_product", "pe_permute", "pe_gemm", "pe_einsum_exec", "pe_einsum_teardown", "pe_einsum_run", "pe_probe_mfma", "pe_probe_launch", "pe_gemm_choice",
               "pe_einsum_exec_noalloc", "pe_linear_attention", "pe_reduce_axes", "pe_reduce_order",
               "pe_causal_conv", "pe_causal_conv_step", "pe_selective_scan", "pe_selective_scan_step",
-              "pe_matvec_q4"):
+              "pe_matvec_q4", "pe_quantize_q8", "pe_gated_norm", "pe_residual_norm", "pe_matmul_q8"):
         getattr(lib, f).restype = ctypes.c_int
     return lib

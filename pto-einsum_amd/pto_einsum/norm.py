@@ -1,0 +1,218 @@
+"""Norms between the blocks of a layer on the GPU.
+
+``gated_norm`` is the norm behind a scan, fused with its gate; ``residual_norm``
+ends one block and starts the next: a norm and a gate of the block's output, the
+residual sum with its scale, and the norm of that sum.  Both read each value once
+and answer either in the operands' type or, with ``quantize=True``, with rows in
+8 bits and their scales: the operands of ``matmul_q8``.
+
+Types, streams, captures and refusals are those of the state-space operators:
+float16, bfloat16 or float32, sums and norms in float32, every output rounded
+once, no gradients.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import abi, runtime
+from .ssm import DTYPES, _plans, _ptr, check, dense, extent, inner, layout, lib, on, ready, remember
+
+
+def row_bytes(k: int) -> int:
+    """Bytes from one row in 8 bits to the next."""
+    return -(-k // 16) * 16
+
+
+def _stride(axes):
+    """The one stride of some (size, stride) axes, or None."""
+    axes = [a for a in axes if a[0] != 1]
+    if any(n == 0 for n, _ in axes):
+        return 0
+    for (_, s), (n, t) in zip(axes, axes[1:]):
+        if s != n * t:
+            return None
+    return axes[-1][1] if axes else 0
+
+
+def places(lead, tensors):
+    """The leading axes ``lead`` as two, and every tensor's strides along them
+    (None: that tensor has no such strides; None in its place: not given): the
+    split that suits most tensors."""
+    best = None
+    for p in range(len(lead) + 1):
+        found = []
+        for t in tensors:
+            if t is None:
+                found.append((0, 0))
+                continue
+            axes = list(zip(lead, t.stride()))
+            pair = _stride(axes[:p]), _stride(axes[p:len(lead)])
+            found.append(None if None in pair else pair)
+        if best is None or found.count(None) < best[1].count(None):
+            best = p, found
+    p, found = best
+    rows0, rows1 = torch.Size(lead[:p]).numel(), torch.Size(lead[p:]).numel()
+    return rows0, rows1, found
+
+
+def _operands(what, x, **others):
+    if x.dtype not in DTYPES:
+        raise TypeError(f"{what}: unsupported dtype {x.dtype} for x")
+    if x.dim() < 1:
+        raise ValueError(f"{what}: x must have an axis")
+    for name, t in others.items():
+        check(what, name, t, (x.shape[-1],), x.dtype)
+
+
+def _eps(what, eps):
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"{what}: eps must be finite and 0 or more, got {eps}")
+    return float(eps)
+
+
+def rows8(x, shape):
+    """Rows in 8 bits for values of that shape: the buffer's values, and scales."""
+    k = shape[-1]
+    q = x.new_empty((*shape[:-1], row_bytes(k)), dtype=torch.int8)
+    return (q[..., :k] if k % 16 else q), x.new_empty(shape[:-1], dtype=torch.float32)
+
+
+def quantize_q8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of x in 8 bits: (q int8 of x's shape, scales float32 [...]) with
+
+        scales = max_k |x| / 127,   q = x / scales rounded to the nearest whole number
+
+    ties to even, as the exact quotient 127 x / max decides.  A row of zeros gets
+    scale 0; one that holds an infinity or NaN gets scale NaN and values 0, so
+    that whatever is formed with it is NaN.  x [..., K] float16, bfloat16 or
+    float32.  q's rows start every 16 bytes (K rounded up to 16, the rest 0),
+    which is how ``matmul_q8`` reads rows of x and of weights."""
+    what = "quantize_q8"
+    key = (what, layout(x))
+    d = _plans.get(key)
+    if d is None:
+        _operands(what, x)
+        ready(what, x)
+        laid = inner(x)
+        rows0, rows1, (pair,) = places(x.shape[:-1], (laid,))
+        if pair is None or laid is not x:
+            return quantize_q8(laid.contiguous())
+        d = remember(key, abi.RowsDesc(dtype=DTYPES[x.dtype], rows0=rows0, rows1=rows1, D=x.shape[-1], groups=1,
+                                       x_s0=pair[0], x_s1=pair[1], q_ms=row_bytes(x.shape[-1]), x_numel=extent(x)))
+    dev = ready(what, x)
+    with on(dev):
+        q, scales = rows8(x, x.shape)
+        rc = lib().pe_quantize_q8(ctypes.byref(d), x.data_ptr(), q.data_ptr(), scales.data_ptr(),
+                                  runtime.raw_stream(dev))
+    runtime.check(rc, "pe_quantize_q8")
+    return q, scales
+
+
+def gated_norm(x: torch.Tensor, weight: torch.Tensor | None = None, z: torch.Tensor | None = None, *,
+               eps: float = 1e-5, groups: int = 1, norm_first: bool = False, quantize: bool = False):
+    """Root-mean-square norm with a gate, over each of ``groups`` equal parts of
+    the last axis:
+
+        u = x * silu(z),  y = u / sqrt(mean(u^2) + eps) * weight                (z given)
+        y = x / sqrt(mean(x^2) + eps) * weight * silu(z)                        (and norm_first)
+
+    with silu(z) = z / (1 + exp(-z)); without z the plain norm.  x and z [..., D]
+    (any strides but along the last axis), weight [D], all of x's dtype.  Returns
+    y of x's shape and dtype, or with ``quantize`` what ``quantize_q8`` gives for
+    the float32 y: (q, scales), one scale for a row of D (at most 8192 groups)."""
+    what = "gated_norm"
+    key = (what, layout(x), layout(weight), layout(z), eps, groups, bool(norm_first), bool(quantize))
+    d = _plans.get(key)
+    if d is None:
+        _operands(what, x, weight=weight)
+        check(what, "z", z, x.shape, x.dtype)
+        D = x.shape[-1]
+        if groups < 1 or D % groups:
+            raise ValueError(f"{what}: {D} elements are no {groups} equal groups")
+        if quantize and groups > 8192:
+            raise ValueError(f"{what}: at most 8192 groups with quantize, got {groups}")
+        eps = _eps(what, eps)
+        ready(what, x, weight, z)
+        given = (x, weight, z)
+        laid = [inner(x), dense(weight), None if z is None else inner(z)]
+        rows0, rows1, pairs = places(x.shape[:-1], (laid[0], laid[2]))
+        for i, pair in zip((0, 2), pairs):
+            if pair is None:
+                laid[i] = laid[i].contiguous()
+        if any(g is not t for g, t in zip(given, laid)):
+            return gated_norm(*laid, eps=eps, groups=groups, norm_first=norm_first, quantize=quantize)
+        d = remember(key, abi.RowsDesc(dtype=DTYPES[x.dtype], norm_first=bool(norm_first), rows0=rows0, rows1=rows1, D=D,
+                                       groups=groups, x_s0=pairs[0][0], x_s1=pairs[0][1], g_s0=pairs[1][0],
+                                       g_s1=pairs[1][1], q_ms=row_bytes(D), x_numel=extent(x),
+                                       g_numel=0 if z is None else extent(z), eps=eps))
+    dev = ready(what, x, weight, z)
+    with on(dev):
+        y, scales = rows8(x, x.shape) if quantize else (x.new_empty(x.shape), None)
+        out = (None, y.data_ptr(), scales.data_ptr()) if quantize else (y.data_ptr(), None, None)
+        rc = lib().pe_gated_norm(ctypes.byref(d), x.data_ptr(), _ptr(weight), _ptr(z), *out, runtime.raw_stream(dev))
+    runtime.check(rc, "pe_gated_norm")
+    return (y, scales) if quantize else y
+
+
+def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None, *,
+                  post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, scale: float = 1.0,
+                  eps: float = 1e-5, quantize: bool = False):
+    """The end of one block, x, and the start of the next:
+
+        u = x / sqrt(mean(x^2) + eps) * post_weight     (post_weight given, else u = x)
+        r = residual + scale * gate * u                 (gate given, else 1)
+        y = r / sqrt(mean(r^2) + eps) * weight
+
+    x [..., D]; residual of x's shape and dtype, or float32; weight and
+    post_weight [D] and gate of x's dtype; gate of any shape that broadcasts to
+    x's (a gate for each channel, sequence, token or value).  Any strides but
+    along the last axis.  Returns (y, r): y of x's dtype, formed from r before r
+    is rounded to the residual's dtype, or with ``quantize`` ((q, scales), r) as
+    ``quantize_q8`` gives them for the float32 y."""
+    what = "residual_norm"
+    key = (what, layout(x), layout(residual), layout(weight), layout(post_weight), layout(gate), scale, eps,
+           bool(quantize))
+    d = _plans.get(key)
+    if d is None:
+        _operands(what, x, weight=weight, post_weight=post_weight)
+        check(what, "residual", residual, x.shape, x.dtype if residual.dtype is x.dtype else torch.float32)
+        D, lead = x.shape[-1], x.shape[:-1]
+        eps, scale = _eps(what, eps), float(scale)
+        wide = gate
+        if gate is not None:
+            check(what, "gate", gate, gate.shape, x.dtype)
+            try:
+                wide = gate.expand((*lead, 1 if gate.shape[-1:] in ((), (1,)) else D))
+            except RuntimeError:
+                raise ValueError(f"{what}: gate of shape {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}") from None
+        ready(what, x, residual, weight, post_weight, gate)
+        given = [x, residual, weight, post_weight, gate]
+        laid = [inner(x), inner(residual), dense(weight), dense(post_weight),
+                gate if gate is None or wide.stride(-1) == 1 or wide.shape[-1] == 1 else gate.clone(
+                    memory_format=torch.contiguous_format)]
+        if laid[4] is gate:
+            rows0, rows1, pairs = places(lead, (laid[0], laid[1], wide))
+            for i, t, pair in zip((0, 1, 4), (laid[0], laid[1], wide), pairs):
+                if pair is None:
+                    laid[i] = t.contiguous()
+        if any(g is not t for g, t in zip(given, laid)):
+            return residual_norm(*laid[:3], post_weight=laid[3], gate=laid[4], scale=scale, eps=eps, quantize=quantize)
+        (xs, rs, gs) = pairs
+        d = remember(key, abi.RowsDesc(dtype=DTYPES[x.dtype], res_dtype=DTYPES[residual.dtype],
+                                       gate_row=gate is not None and wide.shape[-1] == 1, rows0=rows0, rows1=rows1, D=D,
+                                       groups=1, x_s0=xs[0], x_s1=xs[1], g_s0=gs[0], g_s1=gs[1], r_s0=rs[0],
+                                       r_s1=rs[1], q_ms=row_bytes(D), x_numel=extent(x),
+                                       g_numel=0 if gate is None else extent(gate), r_numel=extent(residual), eps=eps,
+                                       scale=scale))
+    dev = ready(what, x, residual, weight, post_weight, gate)
+    with on(dev):
+        y, scales = rows8(x, x.shape) if quantize else (x.new_empty(x.shape), None)
+        r = residual.new_empty(x.shape)
+        out = (None, r.data_ptr(), y.data_ptr(), scales.data_ptr()) if quantize else (y.data_ptr(), r.data_ptr(), None,
+                                                                                     None)
+        rc = lib().pe_residual_norm(ctypes.byref(d), x.data_ptr(), residual.data_ptr(), _ptr(weight),
+                                    _ptr(post_weight), _ptr(gate), *out, runtime.raw_stream(dev))
+    runtime.check(rc, "pe_residual_norm")
+    return ((y, scales) if quantize else y), r
