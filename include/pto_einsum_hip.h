@@ -315,7 +315,8 @@ int pe_matvec_q4(const pe_q4_desc* d, const void* x, const void* packed, const v
  * A row in 8 bits: a = max |v|, scale = a / 127 (float32), q = the whole number
  * nearest to 127 v / a, ties to even, as the exact quotient decides; a = 0 gives
  * scale 0 and zeros, a row with an infinity or NaN the scale NaN and zeros.  Rows
- * in 8 bits lie q_ms bytes apart, D rounded up to 16, the bytes between zero. */
+ * in 8 bits lie q_ms bytes apart, a multiple of 16 from D to D rounded up to 128;
+ * the bytes between are zero. */
 typedef struct pe_rows_desc {
     int32_t dtype;                      /* of x, weights, gate and y */
     int32_t res_dtype;                  /* of the residual: dtype or PE_F32 */
@@ -353,7 +354,8 @@ int pe_residual_norm(const pe_rows_desc* d, const void* x, const void* residual,
 typedef struct pe_q8_desc {
     int32_t x_dtype, y_dtype;
     int32_t bias_dtype;                 /* y_dtype or PE_F32 */
-    int32_t reserved;                   /* must be 0 */
+    int32_t kernel;                     /* 0 = choose; 1 = the one for few rows of x; 2.. = tiles of 256x256,
+                                         * 128x256, 128x128, 64x128 and 64x64 of x's and w's rows (same results) */
     int64_t M, N, K;
     int64_t x_ms, w_ns;                 /* row strides */
     int64_t x_numel, w_numel;

@@ -32,8 +32,8 @@ int arguments(const char* what, const pe_rows_desc* d, const void* x, bool gate,
         if (!ssm::within({{d->rows0, d->r_s0}, {d->rows1, d->r_s1}, {d->D, 1}}, d->r_numel))
             return fail(PE_ERR_BOUNDS, name + ": strides address past the residual");
     }
-    if (q8 && (d->q_ms < row_bytes(d->D) || d->q_ms % 16 || d->q_ms > row_bytes(d->D)))
-        return fail(PE_ERR_INVALID, name + ": q_ms must be D rounded up to 16");
+    if (q8 && (d->q_ms < row_bytes(d->D) || d->q_ms % 16 || d->q_ms > ceil_div(d->D, 128) * 128))
+        return fail(PE_ERR_INVALID, name + ": q_ms must be a multiple of 16 from D to D rounded up to 128");
     if (q8 && d->groups > kMostParts) return fail(PE_ERR_UNSUPPORTED, name + ": more than 8192 groups in 8 bits");
     if (d->rows0 && d->rows1 && d->D && !x) return fail(PE_ERR_INVALID, name + ": null pointer");
     a.x = x;

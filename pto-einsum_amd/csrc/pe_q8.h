@@ -26,30 +26,47 @@ struct Q8Args {
     const float *xs, *ws;
     const void* bias;
     void* y;
-    int32_t* part;                    // sums of the K splits [splits][M][N] (null: none)
     int64_t x_ms, w_ns;
     int32_t M, N, K;
     int32_t bias_f32;
-    int32_t splits, split_slabs;      // K splits, and 64-byte slabs of each
     int32_t tiles_m, tiles_n;
 };
 
-// Four neighbouring columns of a row of y from their sums.
+// Scale and bias of four neighbouring columns (past the end: of the last one).
+struct Column {
+    float scale[4], bias[4];
+};
 template <typename E>
-__device__ __forceinline__ void finish(const Q8Args& g, int m, int n, i32x4 acc) {
-    const float sx = g.xs[m];
-    float v[4];
+__device__ __forceinline__ Column column(const Q8Args& g, int n) {
+    Column c;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int c = min(n + i, g.N - 1);
-        v[i] = float(acc[i]) * sx * g.ws[c];
-        if (g.bias) v[i] += g.bias_f32 ? static_cast<const float*>(g.bias)[c]
-                                       : E::to_f32(static_cast<const typename E::T*>(g.bias)[c]);
+        const int at = min(n + i, g.N - 1);
+        c.scale[i] = g.ws[at];
+        c.bias[i] = !g.bias ? 0.0f : g.bias_f32 ? static_cast<const float*>(g.bias)[at]
+                                                : E::to_f32(static_cast<const typename E::T*>(g.bias)[at]);
     }
-    ssm::store_f32<E, 4>(static_cast<typename E::T*>(g.y) + int64_t(m) * g.N + n, g.N - n, v);
+    return c;
 }
 
-int tile_launch(int y_dtype, Q8Args& g, hipStream_t stream);
+// Column r of those in float32, from its sum and its row's scale.
+__device__ __forceinline__ float value(const Column& c, float sx, int r, int32_t sum) {
+    return fmaf(float(sum) * sx, c.scale[r], c.bias[r]);
+}
+
+// These columns of row m of y from their sums.
+template <typename E>
+__device__ __forceinline__ void finish(const Q8Args& g, const Column& c, float sx, int m, int n, i32x4 acc) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = value(c, sx, i, acc[i]);
+    if (n < g.N) ssm::store_f32<E, 4>(static_cast<typename E::T*>(g.y) + int64_t(m) * g.N + n, g.N - n, v);
+}
+
+int rows_launch(int y_dtype, const Q8Args& g, hipStream_t stream);
+// kernel: 0 chooses a tile, 2 + i takes the i-th.
+constexpr int kTileKernels = 5;
+int tile_launch(int y_dtype, const Q8Args& g, int kernel, hipStream_t stream);
 
 }  // namespace q8
 }  // namespace pe

@@ -18,7 +18,7 @@ Space space_of(const pe_q8_desc* d) {
     Space s;
     if (d->x_dtype != PE_I8) {
         s.rows = 0;
-        s.scales = ceil_div(d->M * rows::row_bytes(d->K), 256) * 256;
+        s.scales = ceil_div(d->M * rows::row_pitch(d->K), 256) * 256;
         s.bytes = s.scales + ceil_div(4 * d->M, 256) * 256;
     }
     return s;
@@ -31,6 +31,7 @@ int check(const pe_q8_desc* d) {
     if (!ssm::dtype_ok(d->y_dtype)) return fail(PE_ERR_UNSUPPORTED, "matmul_q8: y must be PE_F32, PE_F16 or PE_BF16");
     if (d->bias_dtype != d->y_dtype && d->bias_dtype != PE_F32)
         return fail(PE_ERR_UNSUPPORTED, "matmul_q8: the bias must have y's dtype or be PE_F32");
+    if (d->kernel < 0 || d->kernel > 1 + kTileKernels) return fail(PE_ERR_INVALID, "matmul_q8: no such kernel");
     if (d->M < 0 || d->N < 0 || d->K < 0) return fail(PE_ERR_INVALID, "matmul_q8: negative extent");
     if (d->K > kMostK) return fail(PE_ERR_UNSUPPORTED, "matmul_q8: K above 131071 may overflow sums of 32 bits");
     const int64_t big = (int64_t(1) << 31) - 4096;
@@ -86,7 +87,7 @@ extern "C" int pe_matmul_q8(const pe_q8_desc* d, const void* x, const float* x_s
         r.rows0 = 1; r.rows1 = d->M; r.D = d->K; r.groups = 1;
         r.x_s1 = d->x_ms;
         r.x_numel = d->x_numel;
-        r.q_ms = rows::row_bytes(d->K);
+        r.q_ms = rows::row_pitch(d->K);
         if (int rc = pe_quantize_q8(&r, x, q, qs, stream)) return rc;
         g.x = q;
         g.xs = qs;
@@ -99,5 +100,10 @@ extern "C" int pe_matmul_q8(const pe_q8_desc* d, const void* x, const float* x_s
     g.bias_f32 = d->bias_dtype == PE_F32;
     g.y = y;
     g.M = int32_t(d->M); g.N = int32_t(d->N); g.K = int32_t(d->K);
-    return tile_launch(d->y_dtype, g, s);
+    // Up to 64 rows of x, and more where one round of blocks of 64 x 64 holds the
+    // product, whose waves share K: 256 x 4096 x 4096 11.3 us (tiles of the other
+    // kernel 17.2), 512 x 2048 x 8192 17.1 (31.8); with two rounds 512 x 4096 x 4096
+    // 21.0 (20.3) and 256 x 8192 x 2048 15.9 (12.1).
+    const bool few = d->kernel ? d->kernel == 1 : d->M <= 64 || ceil_div(d->M, 64) * ceil_div(d->N, 64) <= cu_count();
+    return few ? rows_launch(d->y_dtype, g, s) : tile_launch(d->y_dtype, g, d->kernel, s);
 }

@@ -91,7 +91,7 @@ class RowsDesc(ctypes.Structure):
 
 
 class Q8Desc(ctypes.Structure):
-    _fields_ = ([(f, ctypes.c_int32) for f in ("x_dtype", "y_dtype", "bias_dtype", "reserved")]
+    _fields_ = ([(f, ctypes.c_int32) for f in ("x_dtype", "y_dtype", "bias_dtype", "kernel")]
                 + [(f, ctypes.c_int64) for f in ("M", "N", "K", "x_ms", "w_ns", "x_numel", "w_numel")])
 
 

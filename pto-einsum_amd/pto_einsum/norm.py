@@ -21,8 +21,13 @@ from .ssm import DTYPES, _plans, _ptr, check, dense, extent, inner, layout, lib,
 
 
 def row_bytes(k: int) -> int:
-    """Bytes from one row in 8 bits to the next."""
+    """Bytes of a row in 8 bits, in the groups of 16 that the product reads."""
     return -(-k // 16) * 16
+
+
+def row_pitch(k: int) -> int:
+    """Bytes from one row in 8 bits to the next: long rows start on whole lines."""
+    return row_bytes(k) if k < 1024 else -(-k // 128) * 128
 
 
 def _stride(axes):
@@ -75,8 +80,8 @@ def _eps(what, eps):
 def rows8(x, shape):
     """Rows in 8 bits for values of that shape: the buffer's values, and scales."""
     k = shape[-1]
-    q = x.new_empty((*shape[:-1], row_bytes(k)), dtype=torch.int8)
-    return (q[..., :k] if k % 16 else q), x.new_empty(shape[:-1], dtype=torch.float32)
+    q = x.new_empty((*shape[:-1], row_pitch(k)), dtype=torch.int8)
+    return (q if k == q.shape[-1] else q[..., :k]), x.new_empty(shape[:-1], dtype=torch.float32)
 
 
 def quantize_q8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -87,8 +92,8 @@ def quantize_q8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     ties to even, as the exact quotient 127 x / max decides.  A row of zeros gets
     scale 0; one that holds an infinity or NaN gets scale NaN and values 0, so
     that whatever is formed with it is NaN.  x [..., K] float16, bfloat16 or
-    float32.  q's rows start every 16 bytes (K rounded up to 16, the rest 0),
-    which is how ``matmul_q8`` reads rows of x and of weights."""
+    float32.  q's rows start every 16 bytes (K rounded up to 16, from 1024 on to
+    128, the rest 0), which is how ``matmul_q8`` reads rows of x and of weights."""
     what = "quantize_q8"
     key = (what, layout(x))
     d = _plans.get(key)
@@ -100,7 +105,7 @@ def quantize_q8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         if pair is None or laid is not x:
             return quantize_q8(laid.contiguous())
         d = remember(key, abi.RowsDesc(dtype=DTYPES[x.dtype], rows0=rows0, rows1=rows1, D=x.shape[-1], groups=1,
-                                       x_s0=pair[0], x_s1=pair[1], q_ms=row_bytes(x.shape[-1]), x_numel=extent(x)))
+                                       x_s0=pair[0], x_s1=pair[1], q_ms=row_pitch(x.shape[-1]), x_numel=extent(x)))
     dev = ready(what, x)
     with on(dev):
         q, scales = rows8(x, x.shape)
@@ -145,7 +150,7 @@ def gated_norm(x: torch.Tensor, weight: torch.Tensor | None = None, z: torch.Ten
             return gated_norm(*laid, eps=eps, groups=groups, norm_first=norm_first, quantize=quantize)
         d = remember(key, abi.RowsDesc(dtype=DTYPES[x.dtype], norm_first=bool(norm_first), rows0=rows0, rows1=rows1, D=D,
                                        groups=groups, x_s0=pairs[0][0], x_s1=pairs[0][1], g_s0=pairs[1][0],
-                                       g_s1=pairs[1][1], q_ms=row_bytes(D), x_numel=extent(x),
+                                       g_s1=pairs[1][1], q_ms=row_pitch(D), x_numel=extent(x),
                                        g_numel=0 if z is None else extent(z), eps=eps))
     dev = ready(what, x, weight, z)
     with on(dev):
@@ -203,7 +208,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor 
         d = remember(key, abi.RowsDesc(dtype=DTYPES[x.dtype], res_dtype=DTYPES[residual.dtype],
                                        gate_row=gate is not None and wide.shape[-1] == 1, rows0=rows0, rows1=rows1, D=D,
                                        groups=1, x_s0=xs[0], x_s1=xs[1], g_s0=gs[0], g_s1=gs[1], r_s0=rs[0],
-                                       r_s1=rs[1], q_ms=row_bytes(D), x_numel=extent(x),
+                                       r_s1=rs[1], q_ms=row_pitch(D), x_numel=extent(x),
                                        g_numel=0 if gate is None else extent(gate), r_numel=extent(residual), eps=eps,
                                        scale=scale))
     dev = ready(what, x, residual, weight, post_weight, gate)

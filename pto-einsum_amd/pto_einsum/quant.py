@@ -18,7 +18,7 @@ import ctypes
 import torch
 
 from . import abi, launch, runtime
-from .norm import _stride, row_bytes
+from .norm import _stride, row_bytes, row_pitch
 from .ssm import DTYPES, _plans, _ptr, check, dense, extent, inner, layout, lib, on, ready, remember
 
 
@@ -95,7 +95,7 @@ def _laid8(t: torch.Tensor) -> bool:
 def _lay8(t: torch.Tensor) -> torch.Tensor:
     """t in rows that start every 16 bytes."""
     k = t.shape[-1]
-    out = t.new_zeros((*t.shape[:-1], row_bytes(k)))[..., :k]
+    out = t.new_zeros((*t.shape[:-1], row_pitch(k)))[..., :k]
     out.copy_(t)
     return out
 

@@ -40,7 +40,12 @@ def check(q, w, dtype, bias=None, fill=0):
 
 SIZES = [(1, 1, 1), (1, 5, 16), (2, 64, 64), (3, 17, 100), (1, 1000, 4096), (5, 129, 65), (16, 256, 2048), (17, 255, 127),
          (33, 513, 1000), (64, 1024, 512), (65, 66, 129), (100, 300, 700), (128, 128, 128), (200, 96, 5000),
-         (257, 1001, 2500), (500, 2000, 192), (1024, 1024, 64), (1, 50000, 48), (3000, 7, 33)]
+         (257, 1001, 2500), (500, 2000, 192), (1024, 1024, 64), (1, 50000, 48), (3000, 7, 33),
+         # weight tiles of the kernel for few rows: one, two and four, whole and not
+         (7, 5000, 130), (16, 9000, 256), (20, 8200, 200), (30, 16500, 64), (64, 8200, 300), (60, 17000, 128), (64, 1000, 6000),
+         # the other kernel's tiles, slabs odd and even, with and without a tail
+         (70, 30000, 64), (2000, 1300, 65), (2100, 2200, 129), (4000, 300, 1000), (1000, 20000, 320), (9000, 2100, 200),
+         (2048, 4096, 1024), (3001, 4100, 777), (6000, 3100, 90)]
 
 
 @pytest.mark.parametrize("dtype", ALL, ids=IDS)
@@ -175,3 +180,31 @@ def test_empty():
     s0 = torch.ones(4, device="cuda")
     assert not matmul_q8(x0.to(torch.int8), w0, ws, scales=s0).any()
     assert matmul_q8(torch.zeros(4, 32, device="cuda"), torch.zeros(0, 32, dtype=torch.int8, device="cuda"), ws[:0]).shape == (4, 0)
+
+
+@pytest.mark.parametrize("kernel", range(1, 7))
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (40, 70, 64), (129, 257, 65), (300, 520, 1000), (513, 300, 4096), (257, 513, 191),
+                                   (70, 1000, 6001), (256, 256, 128)])
+def test_every_kernel(m, n, k, kernel):
+    """The kernels that sizes choose among answer alike, in each type."""
+    import ctypes
+
+    from pto_einsum import abi, launch
+
+    q, w = padded(whole((m, k), m), 93), padded(whole((n, k), n), 93)
+    s, ws = uniform((m,), 5), uniform((n,), 6)
+    g = torch.Generator().manual_seed(3)
+    bias = torch.randn(n, generator=g)
+    ref, size = ru.product(q.cpu(), s, w.cpu(), ws, bias)
+    sg, wg, bg = s.cuda(), ws.cuda(), bias.cuda()
+    lib = abi.bind()
+    for dtype, code in ((torch.float32, launch.DT_F32), (torch.float16, launch.DT_F16), (torch.bfloat16, launch.DT_BF16)):
+        # rows of y past the last stay as they were
+        out = torch.full((m + 3, n), -7.0, dtype=dtype, device="cuda")
+        d = abi.Q8Desc(launch.DT_I8, code, launch.DT_F32, kernel, m, n, k, q.stride(0), w.stride(0), m * q.stride(0),
+                       n * w.stride(0))
+        rc = lib.pe_matmul_q8(ctypes.byref(d), q.data_ptr(), sg.data_ptr(), w.data_ptr(), wg.data_ptr(), bg.data_ptr(),
+                              out.data_ptr(), None, 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        ru.assert_within(out[:m], ref, ru.product_bound(ref, size, dtype), f"kernel {kernel}")
+        assert (out[m:] == -7.0).all()

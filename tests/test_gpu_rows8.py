@@ -82,14 +82,18 @@ def test_float32_near_both_ends(size):
     assert torch.equal(s.cpu(), scale.float())
 
 
-def test_padding_is_zero_and_rows_lie_on_16_bytes():
-    x = torch.randn(37, 1003, device="cuda")
+@pytest.mark.parametrize("k,pitch", [(3, 16), (1003, 1008), (1100, 1152), (5001, 5120), (16300, 16384), (17001, 17024)])
+def test_padding_is_zero(k, pitch):
     from pto_einsum import quantize_q8
 
-    torch.full((1 << 20,), 77, dtype=torch.int8, device="cuda")     # (freed at once: what the rows may get)
-    q, _ = quantize_q8(x)
-    assert q.stride() == (1008, 1)
-    assert not q.as_strided((37, 5), (1008, 1), 1003).any()
+    x = torch.randn(37, k, device="cuda")
+    for _ in range(2):
+        q, _ = quantize_q8(x)
+        assert q.stride() == (pitch, 1)
+        pad = q.as_strided((37, pitch - k), (pitch, 1), k)
+        assert not pad.any()
+        pad.fill_(77)
+        del q, pad          # (what the next rows get)
 
 
 def test_strides_and_broadcast_rows():

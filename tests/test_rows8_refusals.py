@@ -145,7 +145,7 @@ INVALID, BOUNDS, UNSUPPORTED, WORKSPACE = -1, -2, -3, -4
     (dict(groups=0), INVALID), (dict(groups=3), INVALID), (dict(eps=-1.0), INVALID), (dict(eps=float("nan")), INVALID),
     (dict(x_numel=119), BOUNDS), (dict(x_s0=-60), BOUNDS), (dict(x_s1=1 << 62, rows1=1 << 20), BOUNDS),
     (dict(rows0=1 << 40, rows1=1 << 40), UNSUPPORTED), (dict(rows0=1 << 31, rows1=1, x_s0=0), UNSUPPORTED),
-    (dict(D=1 << 32), UNSUPPORTED), (dict(q_ms=16), INVALID), (dict(q_ms=48), INVALID), (dict(q_ms=20), INVALID),
+    (dict(D=1 << 32), UNSUPPORTED), (dict(q_ms=16), INVALID), (dict(q_ms=144), INVALID), (dict(q_ms=20), INVALID),
 ])
 def test_rows_descriptor(kw, want):
     assert status("pe_quantize_q8", rows_desc(**kw), (64, 64, 64, None))[0] == want
@@ -178,7 +178,7 @@ def q8_desc(**kw):
 
 @pytest.mark.parametrize("kw,want", [
     (dict(x_dtype=4), UNSUPPORTED), (dict(y_dtype=3), UNSUPPORTED), (dict(bias_dtype=1), UNSUPPORTED),
-    (dict(M=-1), INVALID), (dict(K=131072, x_ms=131072, w_ns=131072), UNSUPPORTED), (dict(M=1 << 31), UNSUPPORTED),
+    (dict(kernel=-1), INVALID), (dict(kernel=7), INVALID), (dict(M=-1), INVALID), (dict(K=131072, x_ms=131072, w_ns=131072), UNSUPPORTED), (dict(M=1 << 31), UNSUPPORTED),
     (dict(x_ms=100), UNSUPPORTED), (dict(x_ms=96), UNSUPPORTED), (dict(w_ns=104), UNSUPPORTED), (dict(w_ns=96), UNSUPPORTED),
     (dict(w_ns=(1 << 23) + 16), UNSUPPORTED), (dict(x_ms=-112), UNSUPPORTED),
     (dict(x_numel=447), BOUNDS), (dict(w_numel=559), BOUNDS), (dict(x_dtype=1, x_ms=100, x_numel=399), BOUNDS),
