@@ -285,7 +285,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
             const Quant qt(across.most(top));
             if (tid == 0) a.qs[at.row] = qt.scale();
             for (int e = tid; e < a.q_ms; e += kLongThreads)
-                a.q[at.row * a.q_ms + e] = e < a.D ? int8_t(qt.of(result(e))) : int8_t(0);
+                a.q[at.row * a.q_ms + e] = e < a.D ? int8_t(qt.slowly(result(e))) : int8_t(0);
         } else {
             for (int e = tid; e < a.D; e += kLongThreads)
                 static_cast<typename E::T*>(a.y)[at.y + e] = (typename E::T)result(e);
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
 }
 
 // Rows of at most this many elements pass through registers.
-constexpr int kLongest = 1024 * 2 * kChunk;
+constexpr int kLongest = 2048 * kChunk;
 constexpr int64_t kMostBlocks = int64_t(1) << 20;
 
 template <typename E, typename R, int OP, bool Q>
@@ -313,14 +313,21 @@ int launch(const NormArgs& a, hipStream_t stream) {
         return ssm::hip_status_of_launch("norm");
     };
     using std::integral_constant;
+    // Threads and chunks of a row: a wave while its registers do, then 256 threads,
+    // which leave the other rows of a CU something to do at each barrier (rows of
+    // 8192 to 8 bits: 256 threads with four chunks 42 us, 512 with two 48, 1024 with
+    // one 84; 16384: 512 with four 44, 1024 with two 63).
     const integral_constant<int, 1> one{};
     const integral_constant<int, 2> two{};
-    if (a.D <= 64 * kChunk) return go(integral_constant<int, 64>{}, one);
-    if (a.D <= 128 * kChunk) return go(integral_constant<int, 64>{}, two);
-    if (a.D <= 256 * kChunk) return go(integral_constant<int, 256>{}, one);
-    if (a.D <= 512 * kChunk) return go(integral_constant<int, 256>{}, two);
-    if (a.D <= 1024 * kChunk) return go(integral_constant<int, 1024>{}, one);
-    return go(integral_constant<int, 1024>{}, two);
+    const integral_constant<int, 4> four{};
+    const integral_constant<int, 64> wave{};
+    const integral_constant<int, 256> block{};
+    if (a.D <= 64 * kChunk) return go(wave, one);
+    if (a.D <= 128 * kChunk) return go(wave, two);
+    if (a.D <= 256 * kChunk) return go(block, one);
+    if (a.D <= 512 * kChunk) return go(block, two);
+    if (a.D <= 1024 * kChunk) return go(block, four);
+    return go(integral_constant<int, 512>{}, four);
 }
 
 template <typename E>

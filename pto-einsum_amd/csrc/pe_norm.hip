@@ -3,7 +3,6 @@
 #include "pe_rows.h"
 
 #include <algorithm>
-#include <cmath>
 
 namespace pe {
 namespace rows {

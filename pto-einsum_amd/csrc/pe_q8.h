@@ -65,7 +65,7 @@ __device__ __forceinline__ void finish(const Q8Args& g, const Column& c, float s
 
 int rows_launch(int y_dtype, const Q8Args& g, hipStream_t stream);
 // kernel: 0 chooses a tile, 2 + i takes the i-th.
-constexpr int kTileKernels = 5;
+constexpr int kTileKernels = 6;
 int tile_launch(int y_dtype, const Q8Args& g, int kernel, hipStream_t stream);
 
 }  // namespace q8

@@ -234,6 +234,7 @@ constexpr Tile kTiles[kTileKernels] = {
     {256, 256, 1, 12.0f, 0.79f, 0.79f},
     {128, 256, 2, 8.0f, 0.65f, 0.49f},
     {128, 128, 3, 5.0f, 0.56f, 0.30f},
+    {128, 128, 2, 4.5f, 0.43f, 0.30f},
     {64, 128, 3, 4.0f, 0.27f, 0.207f},
     {64, 64, 5, 3.5f, 0.24f, 0.13f},
 };
@@ -256,7 +257,8 @@ int pick(const Q8Args& g, int kernel, hipStream_t stream) {
         case 0: return run<E, 256, 256, 4, 1>(g, stream);
         case 1: return run<E, 128, 256, 3, 2>(g, stream);
         case 2: return run<E, 128, 128, 3, 3>(g, stream);
-        case 3: return run<E, 64, 128, 4, 2>(g, stream);
+        case 3: return run<E, 128, 128, 4, 2>(g, stream);
+        case 4: return run<E, 64, 128, 4, 2>(g, stream);
         default: return run<E, 64, 64, 4, 2>(g, stream);
     }
 }

@@ -24,12 +24,12 @@ constexpr int kChunk = 8;             // elements a lane takes at once: 16 bytes
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 struct Quant {
-    float amax, inv;                  // inv = 127 / amax, a little off
+    float amax, inv;                  // inv = 127 / amax, rounded
     bool none, exactly;
     __device__ __forceinline__ explicit Quant(uint32_t bits) {
         none = bits == 0 || bits >= 0x7f800000u;
         amax = __uint_as_float(bits);
-        // (where 127 / amax overflows float32 every value goes the exact way)
+        // (where 127 / amax overflows float32 every value goes the long way)
         exactly = amax < 1e-36f;
         inv = none || exactly ? 0.0f : 127.0f / amax;
     }
@@ -38,28 +38,42 @@ struct Quant {
     __device__ __forceinline__ float scale() const {
         return __float_as_uint(amax) >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : amax / 127.0f;
     }
-    // v * inv is off by less than 127 * 1.5 * 2^-23 = 2.3e-5, so only where it
-    // lies that close to a half can the exact quotient round elsewhere: those
-    // values are divided in 64 bits, where 127 v is exact and the quotient of
-    // float32 values is never within an ulp of a half unless it is one.
-    __device__ __forceinline__ int of(float v) const {
-        const float t = v * inv, n = rintf(t);
-        if (__builtin_expect(exactly || fabsf(t - n) > 0.5f - 3.1e-5f, 0))
-            return none ? 0 : int(rint(127.0 * double(v) / double(amax)));
-        return none ? 0 : int(n);
+    // The whole number of v in the low byte.  Added to 1.5 * 2^23, a value is rounded
+    // to a whole number that stands in the last bits.  v * inv is off by less than
+    // 127 * 2^-24 = 7.6e-6, so only where it lies that close to a half can the exact
+    // quotient round elsewhere; there 127 v and half * amax are compared in 64 bits,
+    // which hold both exactly.
+    __device__ __forceinline__ uint32_t of(float v) const {
+        constexpr float kRound = 12582912.0f;
+        float n = fmaf(v, inv, kRound) - kRound;
+        const float d = fmaf(v, inv, -n);
+        if (__builtin_expect(fabsf(d) > 0.5f - 1.0f / 65536.0f, 0)) {
+            const float up = copysignf(1.0f, d);
+            const double beyond = (127.0 * double(v) - double(n + 0.5f * up) * double(amax)) * double(up);
+            if (beyond > 0.0 || (beyond == 0.0 && (int(n) & 1))) n += up;
+        }
+        return __float_as_uint(n + kRound);
+    }
+    __device__ __forceinline__ uint32_t slowly(float v) const {
+        return none ? 0u : uint32_t(int(rint(127.0 * double(v) / double(amax)))) & 255u;
     }
 };
-
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-    return uint32_t(a & 255) | uint32_t(b & 255) << 8 | uint32_t(c & 255) << 16 | uint32_t(d) << 24;
-}
 
 // Eight values as bytes at q (8-byte aligned).
 __device__ __forceinline__ void store_q8(int8_t* q, const Quant& qt, const float (&v)[kChunk]) {
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     u32x2 o;
-    o[0] = pack4(qt.of(v[0]), qt.of(v[1]), qt.of(v[2]), qt.of(v[3]));
-    o[1] = pack4(qt.of(v[4]), qt.of(v[5]), qt.of(v[6]), qt.of(v[7]));
+    if (__builtin_expect(qt.none || qt.exactly, 0)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            o[i] = qt.slowly(v[4 * i]) | qt.slowly(v[4 * i + 1]) << 8 | qt.slowly(v[4 * i + 2]) << 16 | qt.slowly(v[4 * i + 3]) << 24;
+    } else {
+        // (the low byte of each of four words)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            o[i] = __builtin_amdgcn_perm(qt.of(v[4 * i + 1]), qt.of(v[4 * i]), 0x0c0c0400u) |
+                   __builtin_amdgcn_perm(qt.of(v[4 * i + 3]), qt.of(v[4 * i + 2]), 0x04000c0cu);
+    }
     *reinterpret_cast<u32x2*>(q) = o;
 }
 
@@ -87,7 +101,6 @@ struct NormArgs {
     int32_t parts;                    // groups within a unit (rows in 8 bits of a grouped norm)
     int32_t g_ds;                     // 0: one gate for a row
     int32_t norm_first;
-    int32_t nt;                       // streaming stores
     float eps, scale;
 };
 
