@@ -25,23 +25,6 @@ using ssm::load_f32;
 using ssm::silu;
 using ssm::store_f32;
 
-// A chunk as it lies in memory, so that loads go out together and take half the
-// registers in 16 bits.
-template <typename E>
-struct Raw {
-    typename ssm::Vec<E, kChunk>::type v;
-    __device__ __forceinline__ void load(const void* base, int64_t at, int n) {
-        const typename E::T* p = static_cast<const typename E::T*>(base) + at;
-        if (n >= kChunk) {
-            v = *reinterpret_cast<const typename ssm::Vec<E, kChunk>::utype*>(p);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) v[i] = i < n ? p[i] : (typename E::T)0.0f;
-        }
-    }
-    __device__ __forceinline__ float operator[](int i) const { return E::to_f32(v[i]); }
-};
-
 // Sum, and maximum of magnitudes, over the TPR threads of a row.
 template <int TPR>
 struct Across {

@@ -22,7 +22,7 @@ using ssm::BF16;
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
 struct Q8Args {
-    const int8_t *x, *w;
+    const int8_t *x, *w;              // (x of another type where the kernel for few rows takes that)
     const float *xs, *ws;
     const void* bias;
     void* y;
@@ -63,6 +63,10 @@ __device__ __forceinline__ void finish(const Q8Args& g, const Column& c, float s
     if (n < g.N) ssm::store_f32<E, 4>(static_cast<typename E::T*>(g.y) + int64_t(m) * g.N + n, g.N - n, v);
 }
 
+// Whether the kernel for few rows takes these to 8 bits itself, and the launch for x
+// of y's type (rows of x as they are in g.x, x_ms in elements).
+bool rows_take_own(int64_t m, int64_t k);
+int rows_launch_own(int dtype, const Q8Args& g, hipStream_t stream);
 int rows_launch(int y_dtype, const Q8Args& g, hipStream_t stream);
 // kernel: 0 chooses a tile, 2 + i takes the i-th.
 constexpr int kTileKernels = 6;

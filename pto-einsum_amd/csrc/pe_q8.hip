@@ -9,6 +9,11 @@ namespace {
 
 constexpr int64_t kMostK = 131071;
 
+// Whether the kernel for few rows takes x to 8 bits itself.
+bool own_rows(const pe_q8_desc* d) {
+    return d->x_dtype == d->y_dtype && d->kernel <= 1 && d->K > 0 && rows_take_own(d->M, d->K);
+}
+
 // Bytes of the workspace: x's rows in 8 bits and their scales, where x comes in
 // another type.
 struct Space {
@@ -16,7 +21,7 @@ struct Space {
 };
 Space space_of(const pe_q8_desc* d) {
     Space s;
-    if (d->x_dtype != PE_I8) {
+    if (d->x_dtype != PE_I8 && !own_rows(d)) {
         s.rows = 0;
         s.scales = ceil_div(d->M * rows::row_pitch(d->K), 256) * 256;
         s.bytes = s.scales + ceil_div(4 * d->M, 256) * 256;
@@ -79,7 +84,20 @@ extern "C" int pe_matmul_q8(const pe_q8_desc* d, const void* x, const float* x_s
     g.x = static_cast<const int8_t*>(x);
     g.x_ms = d->x_ms;
     g.xs = x_scales;
+    g.w = static_cast<const int8_t*>(w);
+    g.w_ns = d->w_ns;
+    g.ws = w_scales;
+    g.bias = bias;
+    g.bias_f32 = d->bias_dtype == PE_F32;
+    g.y = y;
+    g.M = int32_t(d->M); g.N = int32_t(d->N); g.K = int32_t(d->K);
+    // Up to 64 rows of x, and more where one round of blocks of 64 x 64 holds the
+    // product, whose waves share K: 256 x 4096 x 4096 11.3 us (tiles of the other
+    // kernel 17.2), 512 x 2048 x 8192 17.1 (31.8); with two rounds 512 x 4096 x 4096
+    // 21.0 (20.3) and 256 x 8192 x 2048 15.9 (12.1).
+    const bool few = d->kernel ? d->kernel == 1 : d->M <= 64 || ceil_div(d->M, 64) * ceil_div(d->N, 64) <= cu_count();
     if (!whole) {
+        if (own_rows(d)) return rows_launch_own(d->y_dtype, g, s);
         int8_t* q = static_cast<int8_t*>(ws) + space.rows;
         float* qs = reinterpret_cast<float*>(static_cast<char*>(ws) + space.scales);
         pe_rows_desc r{};
@@ -93,17 +111,5 @@ extern "C" int pe_matmul_q8(const pe_q8_desc* d, const void* x, const float* x_s
         g.xs = qs;
         g.x_ms = r.q_ms;
     }
-    g.w = static_cast<const int8_t*>(w);
-    g.w_ns = d->w_ns;
-    g.ws = w_scales;
-    g.bias = bias;
-    g.bias_f32 = d->bias_dtype == PE_F32;
-    g.y = y;
-    g.M = int32_t(d->M); g.N = int32_t(d->N); g.K = int32_t(d->K);
-    // Up to 64 rows of x, and more where one round of blocks of 64 x 64 holds the
-    // product, whose waves share K: 256 x 4096 x 4096 11.3 us (tiles of the other
-    // kernel 17.2), 512 x 2048 x 8192 17.1 (31.8); with two rounds 512 x 4096 x 4096
-    // 21.0 (20.3) and 256 x 8192 x 2048 15.9 (12.1).
-    const bool few = d->kernel ? d->kernel == 1 : d->M <= 64 || ceil_div(d->M, 64) * ceil_div(d->N, 64) <= cu_count();
     return few ? rows_launch(d->y_dtype, g, s) : tile_launch(d->y_dtype, g, d->kernel, s);
 }

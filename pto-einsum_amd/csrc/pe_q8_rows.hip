@@ -7,6 +7,10 @@
 // direct loads of whole lines, eight lanes to a line.  (Loaded straight into the
 // registers of the matrix cores, whose lanes 0 to 15 are 16 rows, a load touches 16
 // lines with every 16 lanes and the address unit takes four times as long.)
+//
+// Where x is a few short rows in another type, each block takes them to 8 bits
+// itself while its first weights are on their way: that costs it less than a launch
+// of its own costs the call.
 #include "pe_q8.h"
 
 #include <algorithm>
@@ -17,12 +21,19 @@ namespace {
 
 constexpr int kStep = 128;            // bytes of k of a step, two products
 
-template <typename E, int MT, int NT, int WAVES, int DEPTH>
+// OWN: x is of type E and goes to 8 bits here, 16 rows at most.
+constexpr int kOwnChunks = 8;         // of a thread
+constexpr int kOwnBytes = 256 * kOwnChunks * rows::kChunk;   // of the rows in 8 bits
+
+template <typename E, int MT, int NT, int WAVES, int DEPTH, bool OWN>
 __global__ __launch_bounds__(64 * WAVES) void q8_rows_kernel(Q8Args g) {
-    constexpr int STEP = (MT + NT) * 16 * kStep, NI = STEP / 1024;
+    constexpr int STEP = ((OWN ? 0 : MT) + NT) * 16 * kStep, NI = STEP / 1024;
     static_assert((DEPTH - 1) * NI < 64, "loads in flight that vmcnt counts");
     static_assert(DEPTH * STEP >= MT * NT * 1024, "the sums fit the rings");
+    static_assert(!OWN || MT == 1, "one tile of rows");
     __shared__ __attribute__((aligned(1024))) int8_t lds[WAVES * DEPTH * STEP];
+    __shared__ __attribute__((aligned(16))) int8_t own[OWN ? kOwnBytes : 16];
+    __shared__ uint32_t top[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = blockDim.x >> 6;
     const int m0 = int(blockIdx.y) * 16 * MT, n0 = int(blockIdx.x) * 16 * NT;
@@ -65,9 +76,52 @@ __global__ __launch_bounds__(64 * WAVES) void q8_rows_kernel(Q8Args g) {
 
     const int row = lane & 15;
     const int mine = wave < steps ? (steps - wave + waves - 1) / waves : 0;
-    if (mine > 0) {
+    const int pitch = steps * kStep;                     // of the rows in LDS
+    if constexpr (OWN) {
+        // Chunks of all rows, dealt to the threads; their loads come back before the
+        // weights' go out, whose number the compiler's waits do not know of.
+        const int threads = 64 * waves, chunks = pitch / rows::kChunk;
+        rows::Raw<E> raw[kOwnChunks];
+        int at[kOwnChunks], of[kOwnChunks];
+#pragma unroll
+        for (int j = 0; j < kOwnChunks; ++j) {
+            const int c = int(threadIdx.x) + j * threads;
+            of[j] = c / chunks;
+            at[j] = rows::kChunk * (c - of[j] * chunks);
+            if (of[j] < g.M) raw[j].load(g.x, int64_t(of[j]) * g.x_ms + at[j], g.K - at[j]);
+        }
+        if (threadIdx.x < 16) top[threadIdx.x] = 0;
+        uint32_t most[kOwnChunks];
+#pragma unroll
+        for (int j = 0; j < kOwnChunks; ++j) {
+            most[j] = 0;
+            if (of[j] < g.M)
+#pragma unroll
+                for (int e = 0; e < rows::kChunk; ++e) most[j] = max(most[j], rows::magnitude(raw[j][e]));
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (mine > 0)
+#pragma unroll
+            for (int i = 0; i < DEPTH - 1; ++i) issue(i, i);
+#pragma unroll
+        for (int j = 0; j < kOwnChunks; ++j)
+            if (of[j] < g.M) atomicMax(&top[of[j]], most[j]);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < kOwnChunks; ++j) {
+            if (of[j] >= g.M) continue;
+            const rows::Quant qt(top[of[j]]);
+            float v[rows::kChunk];
+#pragma unroll
+            for (int e = 0; e < rows::kChunk; ++e) v[e] = raw[j][e];
+            rows::store_q8(own + of[j] * pitch + at[j], qt, v);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    } else if (mine > 0) {
 #pragma unroll
         for (int i = 0; i < DEPTH - 1; ++i) issue(i, i);
+    }
+    if (mine > 0) {
         int slot = 0, free_slot = DEPTH - 1;
         for (int i = 0; i < mine; ++i) {
             issue(i + DEPTH - 1, free_slot);
@@ -85,8 +139,9 @@ __global__ __launch_bounds__(64 * WAVES) void q8_rows_kernel(Q8Args g) {
                     a[t] = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(uintptr_t(at + uint32_t(t) * 16 * kStep));
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
-                    b[t] = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(uintptr_t(at + uint32_t(NT + t) * 16 * kStep));
-                if (left < kStep) {
+                    b[t] = OWN ? *reinterpret_cast<const i32x4*>(own + min(row, g.M - 1) * pitch + s * kStep + 16 * j16)
+                               : *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(uintptr_t(at + uint32_t(NT + t) * 16 * kStep));
+                if (!OWN && left < kStep) {
                     // Zeros for x behind K.
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -118,17 +173,17 @@ __global__ __launch_bounds__(64 * WAVES) void q8_rows_kernel(Q8Args g) {
         i32x4 sum = {0, 0, 0, 0};
         for (int w = 0; w < waves; ++w) sum += sums[(w * NT * MT + t) * 64 + lane];
         const int m = m0 + 16 * (t % MT) + row, n = n0 + 16 * (t / MT) + 4 * (lane >> 4);
-        if (m < g.M) finish<E>(g, column<E>(g, n), g.xs[m], m, n, sum);
+        if (m < g.M) finish<E>(g, column<E>(g, n), OWN ? rows::Quant(top[m]).scale() : g.xs[m], m, n, sum);
     }
 }
 
-template <typename E, int MT, int NT, int DEPTH>
+template <typename E, int MT, int NT, int DEPTH, bool OWN>
 int run(const Q8Args& g, hipStream_t stream) {
     constexpr int WAVES = 4;
     const int64_t cols = ceil_div(g.N, 16 * NT), tall = ceil_div(g.M, 16 * MT);
     const int waves = int(std::max<int64_t>(1, std::min<int64_t>(WAVES, ceil_div(g.K, kStep))));
     if (cols * tall * 64 * waves >= (int64_t(1) << 32)) return fail(PE_ERR_UNSUPPORTED, "matmul_q8: too many weight rows");
-    q8_rows_kernel<E, MT, NT, WAVES, DEPTH><<<dim3(uint32_t(cols), uint32_t(tall)), 64 * waves, 0, stream>>>(g);
+    q8_rows_kernel<E, MT, NT, WAVES, DEPTH, OWN><<<dim3(uint32_t(cols), uint32_t(tall)), 64 * waves, 0, stream>>>(g);
     return ssm::hip_status_of_launch("matmul_q8");
 }
 
@@ -139,16 +194,25 @@ int run(const Q8Args& g, hipStream_t stream) {
 // 10.1 / 12.5, 16384 x 4096 25.7 / 20.7 / 18.6.  Four waves and two or three steps
 // in the ring, whichever lets more blocks share a CU: eight waves or more steps
 // were level or slower.
-template <typename E, int MT>
+template <typename E, int MT, bool OWN = false>
 int pick(const Q8Args& g, hipStream_t stream) {
     auto cost = [&](int nt) { return ceil_div(ceil_div(g.N, 16 * nt) * ceil_div(g.M, 16 * MT), cu_count()) * (nt + MT); };
     const int64_t one = cost(1), two = cost(2), four = cost(4);
-    if (one <= two && one <= four) return run<E, MT, 1, MT == 4 ? 2 : 3>(g, stream);
-    if (two <= four) return run<E, MT, 2, MT == 1 ? 3 : 2>(g, stream);
-    return run<E, MT, 4, 2>(g, stream);
+    if (one <= two && one <= four) return run<E, MT, 1, MT == 4 ? 2 : 3, OWN>(g, stream);
+    if (two <= four) return run<E, MT, 2, MT == 1 ? 3 : 2, OWN>(g, stream);
+    return run<E, MT, 4, 2, OWN>(g, stream);
 }
 
 }  // namespace
+
+bool rows_take_own(int64_t m, int64_t k) {
+    const int64_t steps = ceil_div(k, kStep);
+    return m <= 16 && m * steps * kStep <= kOwnBytes / 4 * std::min<int64_t>(4, steps);
+}
+
+int rows_launch_own(int dtype, const Q8Args& g, hipStream_t stream) {
+    return ssm::with_type(dtype, [&](auto e) { return pick<decltype(e), 1, true>(g, stream); });
+}
 
 int rows_launch(int y_dtype, const Q8Args& g, hipStream_t stream) {
     return ssm::with_type(y_dtype, [&](auto e) {

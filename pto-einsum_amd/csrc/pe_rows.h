@@ -18,6 +18,23 @@ using ssm::BF16;
 
 constexpr int kChunk = 8;             // elements a lane takes at once: 16 bytes of 16-bit types
 
+// A chunk as it lies in memory, so that loads go out together and take half the
+// registers in 16 bits.
+template <typename E>
+struct Raw {
+    typename ssm::Vec<E, kChunk>::type v;
+    __device__ __forceinline__ void load(const void* base, int64_t at, int n) {
+        const typename E::T* p = static_cast<const typename E::T*>(base) + at;
+        if (n >= kChunk) {
+            v = *reinterpret_cast<const typename ssm::Vec<E, kChunk>::utype*>(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) v[i] = i < n ? p[i] : (typename E::T)0.0f;
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const { return E::to_f32(v[i]); }
+};
+
 // A row's largest absolute value is kept as the bits of |v|: whole numbers order
 // like the values, infinities above them and NaN above those, so neither gets
 // lost in the maximum.

@@ -156,6 +156,34 @@ def test_leading_axes_and_float_strides():
     assert torch.equal(matmul_q8(one.expand(7, 100), w, ws), want[0, 0, 0].expand(7, 60))
 
 
+@pytest.mark.parametrize("dtype", ALL, ids=IDS)
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 7), (1, 128), (1, 130), (1, 2500), (1, 16384), (1, 16385), (2, 8192), (3, 5001),
+                                 (4, 4096), (5, 4096), (7, 300), (16, 1024), (16, 1025), (16, 257), (16, 5), (9, 129)])
+def test_few_rows_in_one_launch(m, k, dtype):
+    """Rows that the product's own blocks take to 8 bits, and those one element past
+    it: what quantize_q8 and the product of its rows give, bit for bit, halves,
+    zeros and NaN among them, at any address."""
+    from pto_einsum import matmul_q8, quantize_q8
+
+    g = torch.Generator().manual_seed(k)
+    wide = torch.randn(m, k + 3, generator=g).to(dtype)
+    x = wide.cuda()[:, 1:k + 1]
+    x[m // 2, k // 2] = 2 * x[m // 2].abs().max()
+    if m > 3:
+        x[0] = 0
+        x[1, k - 1] = float("nan")
+        x[2, 0] = float("-inf")
+    for n in (33, 5000, 9000, 17000):
+        w, ws = padded(whole((n, k), 8), 93), uniform((n,), 9).cuda()
+        bias = uniform((n,), 4).cuda()
+        q, s = quantize_q8(x)
+        want = matmul_q8(q, w, ws, scales=s, bias=bias, dtype=dtype)
+        got = matmul_q8(x, w, ws, bias=bias)
+        assert torch.equal(torch.nan_to_num(got, nan=-3.0), torch.nan_to_num(want, nan=-3.0))
+        if m > 3:
+            assert torch.isnan(got[1:3]).all() and torch.isfinite(got[3:]).all()
+
+
 def test_rows_with_nan_scales():
     """A row that held an infinity gives NaN throughout, and no other row does."""
     from pto_einsum import matmul_q8
