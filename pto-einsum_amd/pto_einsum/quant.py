@@ -18,7 +18,7 @@ import ctypes
 import torch
 
 from . import abi, launch, runtime
-from .norm import _stride, row_bytes, row_pitch
+from .norm import _stride, alloc, fresh, row_bytes, row_pitch
 from .ssm import DTYPES, _plans, _ptr, check, dense, extent, inner, layout, lib, on, ready, remember
 
 
@@ -166,13 +166,13 @@ def matmul_q8(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor
                        launch.DT_F32 if bias is None else DTYPES[bias.dtype], 0, M, N, K,
                        _apart8(x) if whole else _apart(x), _apart8(weight),
                        extent(x) + (kp - K if whole else 0), extent(weight) + kp - K)
-        plan = remember(key, (d, (*lead, N), out, whole, lib().pe_matmul_q8_workspace_bytes(ctypes.byref(d))))
-    d, shape, out, whole, ws_bytes = plan
+        plan = remember(key, (d, fresh((*lead, N), out), whole, lib().pe_matmul_q8_workspace_bytes(ctypes.byref(d))))
+    d, result, whole, ws_bytes = plan
     dev = ready(what, x, weight, weight_scales, scales, bias)
     if not (_laid8(weight) and (not whole or _laid8(x))):
         return matmul_q8(_lay8(x) if whole else x, _lay8(weight), weight_scales, scales=scales, bias=bias, dtype=dtype)
     with on(dev):
-        y = weight_scales.new_empty(shape, dtype=out)
+        y = alloc(result, x.device)
         ws = weight.new_empty(ws_bytes) if ws_bytes else None
         rc = lib().pe_matmul_q8(ctypes.byref(d), x.data_ptr(), _ptr(scales), weight.data_ptr(),
                                 weight_scales.data_ptr(), _ptr(bias), y.data_ptr(), _ptr(ws), ws_bytes,
