@@ -355,7 +355,8 @@ typedef struct pe_q8_desc {
     int32_t x_dtype, y_dtype;
     int32_t bias_dtype;                 /* y_dtype or PE_F32 */
     int32_t kernel;                     /* 0 = choose; 1 = the one for few rows of x; 2.. = tiles of 256x256,
-                                         * 128x256, 128x128 (two), 64x128 and 64x64 of x's and w's rows (same results) */
+                                         * 256x192, 128x256, 128x128 (two), 64x128 and 64x64 of x's and w's rows
+                                         * (same results) */
     int64_t M, N, K;
     int64_t x_ms, w_ns;                 /* row strides */
     int64_t x_numel, w_numel;

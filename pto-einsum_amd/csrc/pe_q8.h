@@ -69,7 +69,7 @@ bool rows_take_own(int64_t m, int64_t k);
 int rows_launch_own(int dtype, const Q8Args& g, hipStream_t stream);
 int rows_launch(int y_dtype, const Q8Args& g, hipStream_t stream);
 // kernel: 0 chooses a tile, 2 + i takes the i-th.
-constexpr int kTileKernels = 6;
+constexpr int kTileKernels = 7;
 int tile_launch(int y_dtype, const Q8Args& g, int kernel, hipStream_t stream);
 
 }  // namespace q8

@@ -169,18 +169,18 @@ __global__ __launch_bounds__(256, MINB) void q8_tile_kernel(Q8Args g) {
     // The sums lie four columns a lane, which would store 8 bytes of 16 rows at a time
     // (8192 x 8192 in 16 bits took 60 to 100 us that way, for 21 us of writing), so
     // each 16 rows of the wave's tile go through LDS of the wave's own and out in
-    // whole 16-byte vectors along the rows.
+    // whole 16-byte vectors along the rows, two such places in turn.
     using V = typename ssm::Vec<E, 16 / E::kBytes>;
     constexpr int WN = BN / 2, PITCH = WN * E::kBytes + 16, VPR = WN * E::kBytes / 16;
-    static_assert(4 * 16 * PITCH <= STAGES * STAGE, "the output rows of four waves fit the ring");
+    static_assert(2 * 4 * 16 * PITCH <= STAGES * STAGE, "the output rows of four waves fit the ring twice");
     asm volatile("s_barrier" ::: "memory");
-    int8_t* mine = lds + wave * 16 * PITCH;
     Column c[FN];
 #pragma unroll
     for (int i = 0; i < FN; ++i) c[i] = column<E>(g, nl + 16 * i);
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
         const int m = m0 + wm * (BM / 2) + 16 * j;
+        int8_t* mine = lds + (2 * wave + (j & 1)) * 16 * PITCH;
         const float sx = g.xs[min(m + fr, g.M - 1)];
 #pragma unroll
         for (int i = 0; i < FN; ++i) {
@@ -206,7 +206,6 @@ __global__ __launch_bounds__(256, MINB) void q8_tile_kernel(Q8Args g) {
                 }
             }
         }
-        ssm::wave_sync();
     }
 }
 
@@ -224,7 +223,8 @@ int run(const Q8Args& args, hipStream_t stream) {
 }
 
 // The tile: rounds of blocks times their start and end, and slabs times what the
-// busiest CU takes for each, from fits to 8192 x 8192 x (64 to 8192) (us).  A CU
+// busiest CU takes for each, from fits to 8192 x 8192 x (64 to 8192) and, of the
+// small tiles, to few blocks a CU (us).  A CU
 // with fewer blocks than it holds takes a slab's latency at least.
 struct Tile {
     int bm, bn, blocks;               // blocks that share a CU
@@ -232,11 +232,12 @@ struct Tile {
 };
 constexpr Tile kTiles[kTileKernels] = {
     {256, 256, 1, 12.0f, 0.79f, 0.79f},
+    {256, 192, 1, 9.0f, 0.61f, 0.61f},
     {128, 256, 2, 8.0f, 0.65f, 0.49f},
     {128, 128, 3, 5.0f, 0.56f, 0.30f},
     {128, 128, 2, 4.5f, 0.43f, 0.30f},
-    {64, 128, 3, 4.0f, 0.27f, 0.207f},
-    {64, 64, 5, 3.5f, 0.24f, 0.13f},
+    {64, 128, 3, 4.0f, 0.27f, 0.27f},
+    {64, 64, 5, 3.5f, 0.24f, 0.17f},
 };
 
 template <typename E>
@@ -255,10 +256,11 @@ int pick(const Q8Args& g, int kernel, hipStream_t stream) {
     }
     switch (kernel ? kernel - 2 : best) {
         case 0: return run<E, 256, 256, 4, 1>(g, stream);
-        case 1: return run<E, 128, 256, 3, 2>(g, stream);
-        case 2: return run<E, 128, 128, 3, 3>(g, stream);
-        case 3: return run<E, 128, 128, 4, 2>(g, stream);
-        case 4: return run<E, 64, 128, 4, 2>(g, stream);
+        case 1: return run<E, 256, 192, 4, 1>(g, stream);
+        case 2: return run<E, 128, 256, 3, 2>(g, stream);
+        case 3: return run<E, 128, 128, 3, 3>(g, stream);
+        case 4: return run<E, 128, 128, 4, 2>(g, stream);
+        case 5: return run<E, 64, 128, 4, 2>(g, stream);
         default: return run<E, 64, 64, 4, 2>(g, stream);
     }
 }

@@ -210,7 +210,7 @@ def test_empty():
     assert matmul_q8(torch.zeros(4, 32, device="cuda"), torch.zeros(0, 32, dtype=torch.int8, device="cuda"), ws[:0]).shape == (4, 0)
 
 
-@pytest.mark.parametrize("kernel", range(1, 8))
+@pytest.mark.parametrize("kernel", range(1, 9))
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (40, 70, 64), (129, 257, 65), (300, 520, 1000), (513, 300, 4096), (257, 513, 191),
                                    (70, 1000, 6001), (256, 256, 128)])
 def test_every_kernel(m, n, k, kernel):

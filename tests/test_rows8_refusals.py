@@ -178,7 +178,7 @@ def q8_desc(**kw):
 
 @pytest.mark.parametrize("kw,want", [
     (dict(x_dtype=4), UNSUPPORTED), (dict(y_dtype=3), UNSUPPORTED), (dict(bias_dtype=1), UNSUPPORTED),
-    (dict(kernel=-1), INVALID), (dict(kernel=8), INVALID), (dict(M=-1), INVALID), (dict(K=131072, x_ms=131072, w_ns=131072), UNSUPPORTED), (dict(M=1 << 31), UNSUPPORTED),
+    (dict(kernel=-1), INVALID), (dict(kernel=9), INVALID), (dict(M=-1), INVALID), (dict(K=131072, x_ms=131072, w_ns=131072), UNSUPPORTED), (dict(M=1 << 31), UNSUPPORTED),
     (dict(x_ms=100), UNSUPPORTED), (dict(x_ms=96), UNSUPPORTED), (dict(w_ns=104), UNSUPPORTED), (dict(w_ns=96), UNSUPPORTED),
     (dict(w_ns=(1 << 23) + 16), UNSUPPORTED), (dict(x_ms=-112), UNSUPPORTED),
     (dict(x_numel=447), BOUNDS), (dict(w_numel=559), BOUNDS), (dict(x_dtype=1, x_ms=100, x_numel=399), BOUNDS),
