@@ -86,12 +86,17 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
     for (uint64_t unit = uint64_t(blockIdx.x) * RPB + threadIdx.x / TPR; unit < a.units;
          unit += uint64_t(gridDim.x) * RPB) {
         const Place at(a, uint32_t(unit));
+        // (The length as the compiler cannot see through: the masks of a row's end,
+        // one for each element, are the same for every row, and taken out of the loop
+        // they filled the scalar registers and went through lanes of vector ones.)
+        int len = a.D;
+        asm volatile("" : "+s"(len));
         Raw<E> x[NV], g[NV], w[NV], pw[NV];
         Raw<R> res[NV];
         float one = 1.0f;             // the row's own gate
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int e = kChunk * (tid + j * TPR), n = a.D - e;
+            const int e = kChunk * (tid + j * TPR), n = len - e;
             x[j].load(a.x, at.x + e, n);
             if constexpr (OP == kResidual) res[j].load(a.res, at.r + e, n);
             if (OP != kQuantize && gate && a.g_ds) g[j].load(a.g, at.g + e, n);
@@ -108,12 +113,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
                 for (int j = 0; j < NV; ++j)
 #pragma unroll
                     for (int i = 0; i < kChunk; ++i) ss = fmaf(x[j][i], x[j][i], ss);
-                inv = inv_rms(across.sum(ss), float(a.D), a.eps);
+                inv = inv_rms(across.sum(ss), float(len), a.eps);
             }
             float ss = 0.0f;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int e = kChunk * (tid + j * TPR), n = a.D - e;
+                const int e = kChunk * (tid + j * TPR), n = len - e;
 #pragma unroll
                 for (int i = 0; i < kChunk; ++i) {
                     float u = x[j][i];
@@ -127,7 +132,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
                 }
                 store_f32<R, kChunk>(static_cast<typename R::T*>(a.r) + at.y + e, n, v[j]);
             }
-            inv = inv_rms(across.sum(ss), float(a.D), a.eps);
+            inv = inv_rms(across.sum(ss), float(len), a.eps);
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -146,7 +151,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
                     if (first) v[j][i] *= silu(g[j][i]);
                     ss = fmaf(v[j][i], v[j][i], ss);
                 }
-            const float inv = inv_rms(across.sum(ss), float(a.D), a.eps);
+            const float inv = inv_rms(across.sum(ss), float(len), a.eps);
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -168,7 +173,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
 #pragma unroll
                 for (int i = 0; i < kChunk; ++i) {
                     // (values past the row count for nothing, whatever they are)
-                    if (kChunk * (tid + j * TPR) + i >= a.D) v[j][i] = 0.0f;
+                    if (kChunk * (tid + j * TPR) + i >= len) v[j][i] = 0.0f;
                     const uint32_t b = magnitude(v[j][i]);
                     top = b > top ? b : top;
                 }
@@ -177,13 +182,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int e = kChunk * (tid + j * TPR);
-                if (e < a.q_ms) store_q8(a.q + at.row * a.q_ms + e, qt, v[j]);
+                if (e < a.q_ms) *reinterpret_cast<u32x2*>(a.q + at.row * a.q_ms + e) = eight(qt, v[j]);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int e = kChunk * (tid + j * TPR);
-                store_f32<E, kChunk>(static_cast<typename E::T*>(a.y) + at.y + e, a.D - e, v[j]);
+                store_f32<E, kChunk>(static_cast<typename E::T*>(a.y) + at.y + e, len - e, v[j]);
             }
         }
     }
@@ -267,8 +272,12 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
             }
             const Quant qt(across.most(top));
             if (tid == 0) a.qs[at.row] = qt.scale();
-            for (int e = tid; e < a.q_ms; e += kLongThreads)
-                a.q[at.row * a.q_ms + e] = e < a.D ? int8_t(qt.slowly(result(e))) : int8_t(0);
+            for (int e = kChunk * tid; e < a.q_ms; e += kChunk * kLongThreads) {
+                float v[kChunk];
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) v[i] = e + i < a.D ? result(e + i) : 0.0f;
+                *reinterpret_cast<u32x2*>(a.q + at.row * a.q_ms + e) = eight(qt, v);
+            }
         } else {
             for (int e = tid; e < a.D; e += kLongThreads)
                 static_cast<typename E::T*>(a.y)[at.y + e] = (typename E::T)result(e);

@@ -114,7 +114,7 @@ __global__ __launch_bounds__(64 * WAVES) void q8_rows_kernel(Q8Args g) {
             float v[rows::kChunk];
 #pragma unroll
             for (int e = 0; e < rows::kChunk; ++e) v[e] = raw[j][e];
-            rows::store_q8(own + of[j] * pitch + at[j], qt, v);
+            *reinterpret_cast<rows::u32x2*>(own + of[j] * pitch + at[j]) = rows::eight(qt, v);
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     } else if (mine > 0) {
@@ -182,7 +182,7 @@ int run(const Q8Args& g, hipStream_t stream) {
     constexpr int WAVES = 4;
     const int64_t cols = ceil_div(g.N, 16 * NT), tall = ceil_div(g.M, 16 * MT);
     const int waves = int(std::max<int64_t>(1, std::min<int64_t>(WAVES, ceil_div(g.K, kStep))));
-    if (cols * tall * 64 * waves >= (int64_t(1) << 32)) return fail(PE_ERR_UNSUPPORTED, "matmul_q8: too many weight rows");
+    if (tall > 65535 || cols * tall * 64 * waves >= (int64_t(1) << 32)) return fail(PE_ERR_UNSUPPORTED, "matmul_q8: too many rows");
     q8_rows_kernel<E, MT, NT, WAVES, DEPTH, OWN><<<dim3(uint32_t(cols), uint32_t(tall)), 64 * waves, 0, stream>>>(g);
     return ssm::hip_status_of_launch("matmul_q8");
 }

@@ -1,4 +1,14 @@
 // Products of rows in 8 bits: tiles through LDS (pe_q8.h).
+//
+// Four waves (2 x 2) share a tile.  K walks in slabs of 64 bytes through a ring of LDS
+// stages that direct loads fill; while a slab is multiplied, the next one's fragments
+// are read into a second set of registers and the one STAGES - 1 ahead is loaded, one
+// read or load at a time between the products, so that the matrix cores wait for
+// neither.  The products' rate bounds large ones (8192^3: matrix cores 57 % busy at 1.8
+// GHz, 2.4 POPS where the library's int8 product reaches 2.1); a wave's tile of 128 x
+// 128 reads 16 KB of LDS for 64 products of 16 cycles, half of what LDS delivers, one of
+// 64 x 64 all of it.  A tile's start and end (12 us of a 256 x 256 one, half of it the
+// stores of all CUs at once) bounds products of short K.
 #include "pe_q8.h"
 
 #include <algorithm>
@@ -224,8 +234,11 @@ int run(const Q8Args& args, hipStream_t stream) {
 
 // The tile: rounds of blocks times their start and end, and slabs times what the
 // busiest CU takes for each, from fits to 8192 x 8192 x (64 to 8192) and, of the
-// small tiles, to few blocks a CU (us).  A CU
-// with fewer blocks than it holds takes a slab's latency at least.
+// small tiles, to few blocks a CU (us).  A CU with fewer blocks than it holds takes a
+// slab's latency at least.  Measured, us, in the order below: 8192^3 452 / 526 / 536 /
+// 640 / 649 / 880 / 1090; 4096 x 8512 x 2048 100 / 87 / 94 / 93 / 96 / 127 / 152; 512 x
+// 8192 x 8192 97 / 82 / 102 / 77 / 58 / 72 / 88; 1000 x 2048 x 2048 12.0 with the last two,
+// 17.9 and 13.9 with those of 128 x 128.
 struct Tile {
     int bm, bn, blocks;               // blocks that share a CU
     float fixed, latency, slab;

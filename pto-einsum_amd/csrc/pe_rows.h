@@ -27,9 +27,17 @@ struct Raw {
         const typename E::T* p = static_cast<const typename E::T*>(base) + at;
         if (n >= kChunk) {
             v = *reinterpret_cast<const typename ssm::Vec<E, kChunk>::utype*>(p);
+        } else if (n > 0) {
+            // (the last one again where the row has ended: no load behind it, and no
+            // branch for each)
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+                const typename E::T t = p[min(i, n - 1)];
+                v[i] = i < n ? t : (typename E::T)0.0f;
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) v[i] = i < n ? p[i] : (typename E::T)0.0f;
+            for (int i = 0; i < kChunk; ++i) v[i] = (typename E::T)0.0f;
         }
     }
     __device__ __forceinline__ float operator[](int i) const { return E::to_f32(v[i]); }
@@ -41,57 +49,63 @@ struct Raw {
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 struct Quant {
-    float amax, inv;                  // inv = 127 / amax, rounded
-    bool none, exactly;
+    float given, amax, inv, lift;     // amax = given * lift, inv = 127 / amax, rounded
+    uint32_t keep;
     __device__ __forceinline__ explicit Quant(uint32_t bits) {
-        none = bits == 0 || bits >= 0x7f800000u;
-        amax = __uint_as_float(bits);
-        // (where 127 / amax overflows float32 every value goes the long way)
-        exactly = amax < 1e-36f;
-        inv = none || exactly ? 0.0f : 127.0f / amax;
+        given = __uint_as_float(bits);
+        // Rows far from 1 are multiplied by a power of two first, so that neither
+        // 127 / amax nor 127 v leaves float32's range and v's last bits stay (of a
+        // large row, what those lose rounds to 0).
+        lift = given < 0x1p-60f ? 0x1p90f : given > 0x1p100f ? 0x1p-60f : 1.0f;
+        amax = given * lift;
+        const bool none = bits == 0 || bits >= 0x7f800000u;
+        inv = none ? 0.0f : 127.0f / amax;
+        keep = none ? 0u : 0xffffffffu;
     }
     // NaN for a row that holds one or an infinity, so that no finite result comes
     // of it.
     __device__ __forceinline__ float scale() const {
-        return __float_as_uint(amax) >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : amax / 127.0f;
-    }
-    // The whole number of v in the low byte.  Added to 1.5 * 2^23, a value is rounded
-    // to a whole number that stands in the last bits.  v * inv is off by less than
-    // 127 * 2^-24 = 7.6e-6, so only where it lies that close to a half can the exact
-    // quotient round elsewhere; there 127 v and half * amax are compared in 64 bits,
-    // which hold both exactly.
-    __device__ __forceinline__ uint32_t of(float v) const {
-        constexpr float kRound = 12582912.0f;
-        float n = fmaf(v, inv, kRound) - kRound;
-        const float d = fmaf(v, inv, -n);
-        if (__builtin_expect(fabsf(d) > 0.5f - 1.0f / 65536.0f, 0)) {
-            const float up = copysignf(1.0f, d);
-            const double beyond = (127.0 * double(v) - double(n + 0.5f * up) * double(amax)) * double(up);
-            if (beyond > 0.0 || (beyond == 0.0 && (int(n) & 1))) n += up;
-        }
-        return __float_as_uint(n + kRound);
-    }
-    __device__ __forceinline__ uint32_t slowly(float v) const {
-        return none ? 0u : uint32_t(int(rint(127.0 * double(v) / double(amax)))) & 255u;
+        return __float_as_uint(given) >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : given / 127.0f;
     }
 };
 
-// Eight values as bytes at q (8-byte aligned).
-__device__ __forceinline__ void store_q8(int8_t* q, const Quant& qt, const float (&v)[kChunk]) {
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    u32x2 o;
-    if (__builtin_expect(qt.none || qt.exactly, 0)) {
+// Eight values as bytes.  Added to 1.5 * 2^23, a value is rounded to a whole number
+// that stands in the last bits.  v * inv is off by less than 127 * 2^-24 = 7.6e-6, so
+// only where it lies that close to a half can the exact quotient round elsewhere.
+// There the sign of 127 v - h amax decides, h the half: 127 v is the sum of two
+// floats, and h amax, a multiple of half amax's last bit as 127 v next to it is,
+// differs from the first by a float.  (One branch for eight values: one for each
+// spilled the masks of 32 branches, and the row of 8192 took as long to round as to
+// read.)
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u32x2 eight(const Quant& qt, const float (&v)[kChunk]) {
+    constexpr float kRound = 12582912.0f;
+    float u[kChunk], n[kChunk], d[kChunk], far = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            o[i] = qt.slowly(v[4 * i]) | qt.slowly(v[4 * i + 1]) << 8 | qt.slowly(v[4 * i + 2]) << 16 | qt.slowly(v[4 * i + 3]) << 24;
-    } else {
-        // (the low byte of each of four words)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            o[i] = __builtin_amdgcn_perm(qt.of(v[4 * i + 1]), qt.of(v[4 * i]), 0x0c0c0400u) |
-                   __builtin_amdgcn_perm(qt.of(v[4 * i + 3]), qt.of(v[4 * i + 2]), 0x04000c0cu);
+    for (int i = 0; i < kChunk; ++i) {
+        u[i] = v[i] * qt.lift;
+        n[i] = fmaf(u[i], qt.inv, kRound) - kRound;
+        d[i] = fmaf(u[i], qt.inv, -n[i]);
+        far = fmaxf(far, fabsf(d[i]));
     }
-    *reinterpret_cast<u32x2*>(q) = o;
+    if (__builtin_expect(far > 0.5f - 1.0f / 65536.0f, 0)) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+            const float up = copysignf(1.0f, d[i]), h = n[i] + 0.5f * up, p = 127.0f * u[i];
+            const float beyond = (fmaf(-h, qt.amax, p) + fmaf(127.0f, u[i], -p)) * up;
+            n[i] = beyond > 0.0f ? n[i] + up : beyond == 0.0f ? 2.0f * rintf(0.5f * h) : n[i];
+        }
+    }
+    uint32_t w[kChunk];
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) w[i] = __float_as_uint(n[i] + kRound);
+    u32x2 o;
+    // (the low byte of each of four words)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        o[i] = (__builtin_amdgcn_perm(w[4 * i + 1], w[4 * i], 0x0c0c0400u) |
+                __builtin_amdgcn_perm(w[4 * i + 3], w[4 * i + 2], 0x04000c0cu)) & qt.keep;
+    return o;
 }
 
 // Bytes of a row in 8 bits that the product reads, in groups of 16, and from one

@@ -2,7 +2,8 @@
 
 Lets Python callers (and the component tests) drive the core launchers
 directly: ``pe_product``, ``pe_permute``, ``pe_gemm``, ``pe_linear_attention``,
-``pe_reduce_axes``, the state-space and 4-bit operators and the plan executor.
+``pe_reduce_axes``, the state-space operators, the norms, the products with weights
+of 4 and 8 bits and the plan executor.
 """
 from __future__ import annotations
 

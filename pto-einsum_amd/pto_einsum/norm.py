@@ -13,6 +13,7 @@ once, no gradients.
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -71,10 +72,19 @@ def _operands(what, x, **others):
         check(what, name, t, (x.shape[-1],), x.dtype)
 
 
+def number(what, name, v, kind=float):
+    """A number that a plan may be kept by; a tensor's value is not known here."""
+    if type(v) is kind:
+        return v
+    if isinstance(v, torch.Tensor):
+        raise TypeError(f"{what}: {name} must be a number, got a tensor")
+    return float(v) if kind is float else operator.index(v)
+
+
 def _eps(what, eps):
-    if not 0.0 <= eps < float("inf"):
+    if not 0.0 <= eps <= torch.finfo(torch.float32).max:
         raise ValueError(f"{what}: eps must be finite and 0 or more, got {eps}")
-    return float(eps)
+    return eps
 
 
 def fresh(shape, dtype):
@@ -151,6 +161,7 @@ def gated_norm(x: torch.Tensor, weight: torch.Tensor | None = None, z: torch.Ten
     y of x's shape and dtype, or with ``quantize`` what ``quantize_q8`` gives for
     the float32 y: (q, scales), one scale for a row of D (at most 8192 groups)."""
     what = "gated_norm"
+    eps, groups = number(what, "eps", eps), number(what, "groups", groups, int)
     key = (what, layout(x), layout(weight), layout(z), eps, groups, bool(norm_first), bool(quantize))
     plan = _plans.get(key)
     if plan is None:
@@ -201,6 +212,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor 
     is rounded to the residual's dtype, or with ``quantize`` ((q, scales), r) as
     ``quantize_q8`` gives them for the float32 y."""
     what = "residual_norm"
+    scale, eps = number(what, "scale", scale), number(what, "eps", eps)
     key = (what, layout(x), layout(residual), layout(weight), layout(post_weight), layout(gate), scale, eps,
            bool(quantize))
     plan = _plans.get(key)
@@ -208,7 +220,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor 
         _operands(what, x, weight=weight, post_weight=post_weight)
         check(what, "residual", residual, x.shape, x.dtype if residual.dtype is x.dtype else torch.float32)
         D, lead = x.shape[-1], x.shape[:-1]
-        eps, scale = _eps(what, eps), float(scale)
+        eps = _eps(what, eps)
         wide = gate
         if gate is not None:
             check(what, "gate", gate, gate.shape, x.dtype)

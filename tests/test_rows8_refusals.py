@@ -41,6 +41,10 @@ def gated_args(**kw):
     (dict(eps=-1e-5), ValueError, "eps"),
     (dict(eps=float("nan")), ValueError, "eps"),
     (dict(eps=float("inf")), ValueError, "eps"),
+    (dict(eps=1e39), ValueError, "eps"),
+    (dict(eps=torch.tensor(1e-5)), TypeError, "eps"),
+    (dict(groups=torch.tensor(2)), TypeError, "groups"),
+    (dict(groups=2.0), TypeError, "integer"),
     (dict(z=z(2, 12, dtype=f16, requires_grad=True)), RuntimeError, "gradient"),
     (dict(weight=z(12, dtype=f16, requires_grad=True)), RuntimeError, "gradient"),
 ])
@@ -67,6 +71,7 @@ def residual_args(**kw):
     (dict(gate=z(1, 2, 3, 12, dtype=f16)), ValueError, "gate"),
     (dict(gate=z(12)), TypeError, "gate"),
     (dict(eps=-1.0), ValueError, "eps"),
+    (dict(scale=torch.tensor(0.5)), TypeError, "scale"),
     (dict(gate=z(12, dtype=f16, requires_grad=True)), RuntimeError, "gradient"),
     (dict(residual=z(2, 3, 12, dtype=f16, requires_grad=True)), RuntimeError, "gradient"),
 ])
