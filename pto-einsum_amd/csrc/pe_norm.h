@@ -194,9 +194,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
     }
 }
 
-// Any length: the values are formed again, element by element, for each step.
-// `parts` groups within the unit (rows in 8 bits of a grouped norm), whose
-// factors lie in LDS.
+// Any length: the values are formed again for each step, a chunk at a time.  `parts`
+// groups within the unit (rows in 8 bits of a grouped norm), whose factors lie in LDS.
 constexpr int kLongThreads = 512;
 
 template <typename E, typename R, int OP, bool Q>
@@ -209,45 +208,67 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
     const bool gate = a.g != nullptr, post = a.pw != nullptr, scaled = a.w != nullptr;
     for (uint64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
         const Place at(a, uint32_t(unit));
-        auto get = [](const void* p, int64_t i, auto e) { return decltype(e)::to_f32(static_cast<const typename decltype(e)::T*>(p)[i]); };
+        const float one = OP == kResidual && gate && !a.g_ds ? E::to_f32(static_cast<const typename E::T*>(a.g)[at.g]) : 1.0f;
         float inv0 = 1.0f;            // of the norm of x, in the residual
-        auto value = [&](int e) {
-            float u = get(a.x, at.x + e, E{});
+        // n values from e on, as the norm takes them (past those 0).
+        auto values = [&](int e, int n, float (&v)[kChunk]) {
+            Raw<E> x, g, pw;
+            Raw<R> res;
+            x.load(a.x, at.x + e, n);
+            if (OP != kQuantize && gate && a.g_ds && !(OP == kGated && a.norm_first)) g.load(a.g, at.g + e, n);
             if constexpr (OP == kResidual) {
-                if (post) u = u * inv0 * get(a.pw, e, E{});
-                if (gate) u *= get(a.g, at.g + (a.g_ds ? e : 0), E{});
-                u = get(a.res, at.r + e, R{}) + a.scale * u;
-            } else if constexpr (OP == kGated) {
-                if (gate && !a.norm_first) u *= silu(get(a.g, at.g + e, E{}));
+                res.load(a.res, at.r + e, n);
+                if (post) pw.load(a.pw, e, n);
             }
-            return u;
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+                float u = x[i];
+                if constexpr (OP == kResidual) {
+                    if (post) u = u * inv0 * pw[i];
+                    if (gate) u *= a.g_ds ? g[i] : one;
+                    u = res[i] + a.scale * u;
+                } else if constexpr (OP == kGated) {
+                    if (gate && !a.norm_first) u *= silu(g[i]);
+                }
+                v[i] = i < n ? u : 0.0f;
+            }
+        };
+        auto squares = [](const float (&v)[kChunk], float ss) {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) ss = fmaf(v[i], v[i], ss);
+            return ss;
         };
         if constexpr (OP == kResidual) {
             if (post) {
                 float ss = 0.0f;
-                for (int e = tid; e < a.D; e += kLongThreads) {
-                    const float u = get(a.x, at.x + e, E{});
-                    ss = fmaf(u, u, ss);
+                for (int e = kChunk * tid; e < a.D; e += kChunk * kLongThreads) {
+                    Raw<E> x;
+                    x.load(a.x, at.x + e, a.D - e);
+                    float v[kChunk];
+#pragma unroll
+                    for (int i = 0; i < kChunk; ++i) v[i] = x[i];
+                    ss = squares(v, ss);
                 }
                 inv0 = inv_rms(across.sum(ss), float(a.D), a.eps);
             }
         }
         if constexpr (OP != kQuantize) {
+            float v[kChunk];
             if (a.parts == 1) {
                 float ss = 0.0f;
-                for (int e = tid; e < a.D; e += kLongThreads) {
-                    const float u = value(e);
-                    if constexpr (OP == kResidual) static_cast<typename R::T*>(a.r)[at.y + e] = (typename R::T)u;
-                    ss = fmaf(u, u, ss);
+                for (int e = kChunk * tid; e < a.D; e += kChunk * kLongThreads) {
+                    values(e, a.D - e, v);
+                    if constexpr (OP == kResidual) store_f32<R, kChunk>(static_cast<typename R::T*>(a.r) + at.y + e, a.D - e, v);
+                    ss = squares(v, ss);
                 }
                 const float inv = inv_rms(across.sum(ss), float(a.D), a.eps);
                 if (tid == 0) factor[0] = inv;
             } else {
                 for (int p = tid >> 6; p < a.parts; p += kLongThreads / 64) {
                     float ss = 0.0f;
-                    for (int e = tid & 63; e < part; e += 64) {
-                        const float u = value(p * part + e);
-                        ss = fmaf(u, u, ss);
+                    for (int e = kChunk * (tid & 63); e < part; e += kChunk * 64) {
+                        values(p * part + e, part - e, v);
+                        ss = squares(v, ss);
                     }
                     const float inv = inv_rms(Across<64>{nullptr}.sum(ss), float(part), a.eps);
                     if ((tid & 63) == 0) factor[p] = inv;
@@ -255,32 +276,52 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
             }
             __syncthreads();
         }
-        auto result = [&](int e) {
-            float u = value(e);
+        auto results = [&](int e, float (&v)[kChunk]) {
+            const int n = a.D - e;
+            values(e, n, v);
             if constexpr (OP != kQuantize) {
-                u *= factor[a.parts == 1 ? 0 : e / part];
-                if (scaled) u *= get(a.w, at.w + e, E{});
-                if (OP == kGated && gate && a.norm_first) u *= silu(get(a.g, at.g + e, E{}));
+                Raw<E> w, g;
+                if (scaled) w.load(a.w, at.w + e, n);
+                if (OP == kGated && gate && a.norm_first) g.load(a.g, at.g + e, n);
+                int p = a.parts == 1 ? 0 : e / part, left = a.parts == 1 ? a.D : (p + 1) * part - e;
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) {
+                    if (a.parts > 1 && i < n && left-- == 0) {
+                        ++p;
+                        left = part - 1;
+                    }
+                    v[i] *= factor[p];
+                    if (scaled) v[i] *= w[i];
+                    if (OP == kGated && gate && a.norm_first) v[i] *= silu(g[i]);
+                }
             }
-            return u;
         };
         if constexpr (Q) {
             uint32_t top = 0;
-            for (int e = tid; e < a.D; e += kLongThreads) {
-                const uint32_t b = magnitude(result(e));
-                top = b > top ? b : top;
+            float v[kChunk];
+            for (int e = kChunk * tid; e < a.D; e += kChunk * kLongThreads) {
+                results(e, v);
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) {
+                    const uint32_t b = e + i < a.D ? magnitude(v[i]) : 0u;
+                    top = b > top ? b : top;
+                }
             }
             const Quant qt(across.most(top));
             if (tid == 0) a.qs[at.row] = qt.scale();
             for (int e = kChunk * tid; e < a.q_ms; e += kChunk * kLongThreads) {
-                float v[kChunk];
+                if (e < a.D) results(e, v);
 #pragma unroll
-                for (int i = 0; i < kChunk; ++i) v[i] = e + i < a.D ? result(e + i) : 0.0f;
+                for (int i = 0; i < kChunk; ++i)
+                    if (e + i >= a.D) v[i] = 0.0f;
                 *reinterpret_cast<u32x2*>(a.q + at.row * a.q_ms + e) = eight(qt, v);
             }
         } else {
-            for (int e = tid; e < a.D; e += kLongThreads)
-                static_cast<typename E::T*>(a.y)[at.y + e] = (typename E::T)result(e);
+            for (int e = kChunk * tid; e < a.D; e += kChunk * kLongThreads) {
+                float v[kChunk];
+                results(e, v);
+                store_f32<E, kChunk>(static_cast<typename E::T*>(a.y) + at.y + e, a.D - e, v);
+            }
         }
         // (the next unit's factors are written behind this unit's reads)
         __syncthreads();

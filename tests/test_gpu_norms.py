@@ -7,7 +7,7 @@ from rows_util import ALL, IDS
 
 pytestmark = pytest.mark.gpu
 
-LENGTHS = [1, 7, 64, 511, 512, 520, 1000, 1024, 1283, 2048, 2055, 4096, 5000, 8192, 10001, 16384, 16385, 33000]
+LENGTHS = [1, 7, 64, 511, 512, 520, 1000, 1024, 1283, 2048, 2055, 4096, 5000, 8192, 10001, 16384, 16385, 20479, 33000]
 
 
 def values(shape, dtype, seed, scale=1.0):
@@ -44,7 +44,8 @@ def test_gated(d, dtype):
 
 
 @pytest.mark.parametrize("dtype", ALL, ids=IDS)
-@pytest.mark.parametrize("d,groups", [(512, 8), (4096, 8), (1000, 5), (77, 7), (30000, 3), (8192, 8192), (48000, 2), (9, 9)])
+@pytest.mark.parametrize("d,groups", [(512, 8), (4096, 8), (1000, 5), (77, 7), (30000, 3), (8192, 8192), (48000, 2), (9, 9),
+                                      (33, 11), (40010, 10), (34002, 2)])
 def test_groups(d, groups, dtype):
     x, z, w = values((2, 3, d), dtype, d), values((2, 3, d), dtype, d + 1), values((d,), dtype, d + 2)
     check_gated(x, w, z, groups=groups)
