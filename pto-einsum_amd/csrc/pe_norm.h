@@ -11,8 +11,9 @@
 // over the lanes of a row's threads, and the row is written from the registers.
 // TPR threads take a row, NV chunks of eight elements each; a wave alone needs no
 // barrier, and short rows share a block.  Rows too long for the registers, and
-// rows in 8 bits of a grouped norm (whose scale spans the groups), go to a kernel
-// that reads the row again for each step: from the caches, mostly.
+// rows in 8 bits of a grouped norm (whose scale spans the groups) unless its groups are
+// whole 512 elements, go to a kernel that reads the row again for each step: from the
+// caches, mostly (4096 rows of 4096, 8 groups: 25 us here, 51 there).
 #pragma once
 
 #include "pe_rows.h"
@@ -76,10 +77,15 @@ struct Place {
     }
 };
 
+// What a wave's chunk holds: a grouped norm whose groups are whole ones of these needs
+// no second reading for rows in 8 bits.
+constexpr int kSegment = 64 * kChunk;
+
 template <typename E, typename R, int OP, bool Q, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a) {
     constexpr int THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR;
     __shared__ uint32_t slots[2 * (TPR / 64)];
+    __shared__ float segments[OP == kGated && Q ? RPB * NV * (TPR / 64) : 1];
     Across<TPR> across{slots};
     const int tid = threadIdx.x % TPR;
     const bool gate = a.g != nullptr, post = a.pw != nullptr, scaled = a.w != nullptr;
@@ -142,21 +148,52 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
                 }
         } else if constexpr (OP == kGated) {
             const bool first = gate && !a.norm_first;
-            float ss = 0.0f;
+            float ss[NV], inv[NV];
 #pragma unroll
-            for (int j = 0; j < NV; ++j)
+            for (int j = 0; j < NV; ++j) {
+                ss[j] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < kChunk; ++i) {
                     v[j][i] = x[j][i];
                     if (first) v[j][i] *= silu(g[j][i]);
-                    ss = fmaf(v[j][i], v[j][i], ss);
+                    ss[j] = fmaf(v[j][i], v[j][i], ss[j]);
                 }
-            const float inv = inv_rms(across.sum(ss), float(len), a.eps);
+            }
+            if (Q && a.parts > 1) {
+                // Groups of whole segments, the 512 elements that a wave's chunk holds:
+                // each segment's sum to LDS, and there those of its group together.
+                constexpr int WAVES = TPR / 64;
+                const int wave = tid >> 6, each = len / a.parts / kSegment;
+                float* mine = segments + threadIdx.x / TPR * (NV * WAVES);
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const float sum = Across<64>{nullptr}.sum(ss[j]);
+                    if ((tid & 63) == 0) mine[j * WAVES + wave] = sum;
+                }
+                if constexpr (WAVES > 1) __syncthreads();
+                else ssm::wave_sync();
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int from = (j * WAVES + wave) / each * each;
+                    float sum = 0.0f;
+                    for (int i = from; i < min(from + each, NV * WAVES); ++i) sum += mine[i];
+                    inv[j] = inv_rms(sum, float(len / a.parts), a.eps);
+                }
+                // (across.most below lies between these reads and the next row's sums)
+                if constexpr (WAVES == 1) ssm::wave_sync();
+            } else {
+                float all = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) all += ss[j];
+                inv[0] = inv_rms(across.sum(all), float(len), a.eps);
+#pragma unroll
+                for (int j = 1; j < NV; ++j) inv[j] = inv[0];
+            }
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
                 for (int i = 0; i < kChunk; ++i) {
-                    v[j][i] *= inv;
+                    v[j][i] *= inv[j];
                     if (scaled) v[j][i] *= w[j][i];
                     if (gate && a.norm_first) v[j][i] *= silu(g[j][i]);
                 }
@@ -334,7 +371,7 @@ constexpr int64_t kMostBlocks = int64_t(1) << 20;
 
 template <typename E, typename R, int OP, bool Q>
 int launch(const NormArgs& a, hipStream_t stream) {
-    if (a.parts > 1 || a.D > kLongest) {
+    if (a.D > kLongest || (a.parts > 1 && a.D / a.parts % kSegment)) {
         const uint32_t grid = uint32_t(std::min<int64_t>(a.units, kMostBlocks));
         norm_long_kernel<E, R, OP, Q><<<grid, kLongThreads, sizeof(float) * a.parts, stream>>>(a);
         return ssm::hip_status_of_launch("norm");

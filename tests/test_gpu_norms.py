@@ -45,7 +45,10 @@ def test_gated(d, dtype):
 
 @pytest.mark.parametrize("dtype", ALL, ids=IDS)
 @pytest.mark.parametrize("d,groups", [(512, 8), (4096, 8), (1000, 5), (77, 7), (30000, 3), (8192, 8192), (48000, 2), (9, 9),
-                                      (33, 11), (40010, 10), (34002, 2)])
+                                      (33, 11), (40010, 10), (34002, 2),
+                                      # groups of whole 512 elements, and a few more
+                                      (1024, 2), (1024, 1), (1536, 3), (3584, 7), (4096, 2), (8192, 16), (7168, 7),
+                                      (12288, 3), (16384, 32), (16384, 4), (17408, 2), (1040, 2), (2064, 4)])
 def test_groups(d, groups, dtype):
     x, z, w = values((2, 3, d), dtype, d), values((2, 3, d), dtype, d + 1), values((d,), dtype, d + 2)
     check_gated(x, w, z, groups=groups)
