@@ -124,6 +124,8 @@ __global__ __launch_bounds__(64 * WAVES) void q8_rows_kernel(Q8Args g) {
     if (mine > 0) {
         int slot = 0, free_slot = DEPTH - 1;
         for (int i = 0; i < mine; ++i) {
+            // (the last step's fragments have left the slot that is loaded now)
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             issue(i + DEPTH - 1, free_slot);
             free_slot = slot;
             asm volatile("s_waitcnt vmcnt(%0)" : : "n"((DEPTH - 1) * NI) : "memory");

@@ -80,31 +80,33 @@ struct Quant {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ u32x2 eight(const Quant& qt, const float (&v)[kChunk]) {
     constexpr float kRound = 12582912.0f;
-    float u[kChunk], n[kChunk], d[kChunk], far = 0.0f;
+    float u[kChunk], w[kChunk], d[kChunk], far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) u[i] = v[i];
+    if (__builtin_expect(qt.lift != 1.0f, 0)) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) u[i] *= qt.lift;
+    }
 #pragma unroll
     for (int i = 0; i < kChunk; ++i) {
-        u[i] = v[i] * qt.lift;
-        n[i] = fmaf(u[i], qt.inv, kRound) - kRound;
-        d[i] = fmaf(u[i], qt.inv, -n[i]);
+        w[i] = fmaf(u[i], qt.inv, kRound);
+        d[i] = fmaf(u[i], qt.inv, kRound - w[i]);
         far = fmaxf(far, fabsf(d[i]));
     }
     if (__builtin_expect(far > 0.5f - 1.0f / 65536.0f, 0)) {
 #pragma unroll
         for (int i = 0; i < kChunk; ++i) {
-            const float up = copysignf(1.0f, d[i]), h = n[i] + 0.5f * up, p = 127.0f * u[i];
+            const float n = w[i] - kRound, up = copysignf(1.0f, d[i]), h = n + 0.5f * up, p = 127.0f * u[i];
             const float beyond = (fmaf(-h, qt.amax, p) + fmaf(127.0f, u[i], -p)) * up;
-            n[i] = beyond > 0.0f ? n[i] + up : beyond == 0.0f ? 2.0f * rintf(0.5f * h) : n[i];
+            w[i] = kRound + (beyond > 0.0f ? n + up : beyond == 0.0f ? 2.0f * rintf(0.5f * h) : n);
         }
     }
-    uint32_t w[kChunk];
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) w[i] = __float_as_uint(n[i] + kRound);
     u32x2 o;
     // (the low byte of each of four words)
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-        o[i] = (__builtin_amdgcn_perm(w[4 * i + 1], w[4 * i], 0x0c0c0400u) |
-                __builtin_amdgcn_perm(w[4 * i + 3], w[4 * i + 2], 0x04000c0cu)) & qt.keep;
+        o[i] = (__builtin_amdgcn_perm(__float_as_uint(w[4 * i + 1]), __float_as_uint(w[4 * i]), 0x0c0c0400u) |
+                __builtin_amdgcn_perm(__float_as_uint(w[4 * i + 3]), __float_as_uint(w[4 * i + 2]), 0x04000c0cu)) & qt.keep;
     return o;
 }
 

@@ -169,8 +169,10 @@ def matmul_q8(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor
         plan = remember(key, (d, fresh((*lead, N), out), whole, lib().pe_matmul_q8_workspace_bytes(ctypes.byref(d))))
     d, result, whole, ws_bytes = plan
     dev = ready(what, x, weight, weight_scales, scales, bias)
-    if not (_laid8(weight) and (not whole or _laid8(x))):
-        return matmul_q8(_lay8(x) if whole else x, _lay8(weight), weight_scales, scales=scales, bias=bias, dtype=dtype)
+    rows_lie, weight_lies = not whole or _laid8(x), _laid8(weight)
+    if not (rows_lie and weight_lies):
+        return matmul_q8(x if rows_lie else _lay8(x), weight if weight_lies else _lay8(weight), weight_scales,
+                         scales=scales, bias=bias, dtype=dtype)
     with on(dev):
         y = alloc(result, x.device)
         ws = weight.new_empty(ws_bytes) if ws_bytes else None
