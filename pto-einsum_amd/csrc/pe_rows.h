@@ -74,9 +74,8 @@ struct Quant {
 // only where it lies that close to a half can the exact quotient round elsewhere.
 // There the sign of 127 v - h amax decides, h the half: 127 v is the sum of two
 // floats, and h amax, a multiple of half amax's last bit as 127 v next to it is,
-// differs from the first by a float.  (One branch for eight values: one for each
-// spilled the masks of 32 branches, and the row of 8192 took as long to round as to
-// read.)
+// differs from the first by a float.  (One branch for eight values: with one for
+// each of a thread's 32 the scalar registers spilled.)
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ u32x2 eight(const Quant& qt, const float (&v)[kChunk]) {
     constexpr float kRound = 12582912.0f;
