@@ -22,7 +22,6 @@ namespace pe {
 namespace rows {
 namespace {
 
-using ssm::load_f32;
 using ssm::silu;
 using ssm::store_f32;
 
@@ -57,7 +56,37 @@ struct Across {
     }
 };
 
-__device__ __forceinline__ float inv_rms(float sum, float D, float eps) { return 1.0f / sqrtf(sum / D + eps); }
+// Sums of squares that float32 does not hold, beyond its range (values from about 1e19
+// on) or of squares that it holds in too few bits or not at all (1e-15 and less, where
+// eps is as small): the row is taken once more, with its values times a power of two.
+// Which one, as a number that a wave's lanes share, so that other rows only pass a
+// branch of the wave.
+enum Far { kNear, kLarge, kSmall };
+__device__ __forceinline__ bool lifted(int far) { return __builtin_expect(far != kNear, 0); }
+__device__ __forceinline__ float lift(int far) { return far == kLarge ? 0x1p-80f : far == kSmall ? 0x1p100f : 1.0f; }
+__device__ __forceinline__ int far_of(float mean) {
+    constexpr uint32_t kLeast = (127u - 100u) << 23;                 // 2^-100
+    const uint32_t bits = __float_as_uint(mean);
+    const bool held = bits - kLeast < 0x7f800000u - kLeast;          // (below infinity)
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(int(held)), 1)) return kNear;
+    return __builtin_amdgcn_readfirstlane(bits < kLeast ? kSmall : kLarge);
+}
+
+// The mean of squares of which `sum` is the sum, of values times lift(far); `per` is one
+// divided by their number.
+__device__ __forceinline__ float mean_of(float sum, float per, float eps, int far) {
+    if (lifted(far)) eps = eps * lift(far) * lift(far);
+    return fmaf(sum, per, eps);
+}
+
+// 1 / sqrt(mean).  Of a near one, neither 0 nor infinite, through the hardware's, which
+// is good to a unit, and a step of Newton's: off by less than the division's and the
+// root's two roundings, without the 20 instructions that a row would wait for.
+__device__ __forceinline__ float factor_of(float mean, int far) {
+    if (lifted(far)) return 1.0f / sqrtf(mean);
+    const float r = __builtin_amdgcn_rsqf(mean);
+    return fmaf(0.5f * r, fmaf(-mean * r, r, 1.0f), r);
+}
 
 // Where a unit's values start.
 struct Place {
@@ -77,6 +106,17 @@ struct Place {
     }
 };
 
+// What values are multiplied by, lift(far) and then inv.
+struct Factor {
+    float inv = 1.0f;
+    int far = kNear;
+    // Both in one float32: of lifted ones the sign is set, and a part of the lift brings
+    // inv, 2^-48 to 2^24 of large ones and 2^-50 to 2^50 of small ones, below 1 or above;
+    // and what else a value is multiplied by.
+    __device__ __forceinline__ float packed() const { return inv * (far == kNear ? 1.0f : far == kLarge ? -0x1p-60f : -0x1p60f); }
+    __device__ __forceinline__ static float rest(float f) { return f >= 0.0f ? 1.0f : f > -1.0f ? -0x1p-20f : -0x1p40f; }
+};
+
 // What a wave's chunk holds: a grouped norm whose groups are whole ones of these needs
 // no second reading for rows in 8 bits.
 constexpr int kSegment = 64 * kChunk;
@@ -89,8 +129,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
     Across<TPR> across{slots};
     const int tid = threadIdx.x % TPR;
     const bool gate = a.g != nullptr, post = a.pw != nullptr, scaled = a.w != nullptr;
+    // What the row's values are lifted by: for a residual x's and then the sum's, for
+    // groups within a row each chunk's; and whether this is the second time.
+    constexpr int FAR = OP == kResidual ? 2 : OP == kGated && Q ? NV : 1;
+    int far[FAR] = {};
+    bool again = false;
     for (uint64_t unit = uint64_t(blockIdx.x) * RPB + threadIdx.x / TPR; unit < a.units;
-         unit += uint64_t(gridDim.x) * RPB) {
+         unit += again ? 0 : uint64_t(gridDim.x) * RPB) {
         const Place at(a, uint32_t(unit));
         // (The length as the compiler cannot see through: the masks of a row's end,
         // one for each element, are the same for every row, and taken out of the loop
@@ -111,15 +156,26 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
         }
         if (OP == kResidual && gate && !a.g_ds) one = E::to_f32(static_cast<const typename E::T*>(a.g)[at.g]);
         float v[NV][kChunk];
+        int found = kNear;            // what is to be lifted is not yet, here or (groups within a row) in another wave
         if constexpr (OP == kResidual) {
-            float inv = 1.0f;
+            float inv = 1.0f, raised = 1.0f;
             if (post) {
                 float ss = 0.0f;
+                raised = lift(far[0]);
+                if (lifted(far[0])) {
 #pragma unroll
-                for (int j = 0; j < NV; ++j)
+                    for (int j = 0; j < NV; ++j)
 #pragma unroll
-                    for (int i = 0; i < kChunk; ++i) ss = fmaf(x[j][i], x[j][i], ss);
-                inv = inv_rms(across.sum(ss), float(len), a.eps);
+                        for (int i = 0; i < kChunk; ++i) ss = fmaf(x[j][i] * raised, x[j][i] * raised, ss);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+#pragma unroll
+                        for (int i = 0; i < kChunk; ++i) ss = fmaf(x[j][i], x[j][i], ss);
+                }
+                const float mean = mean_of(across.sum(ss), a.per, a.eps, far[0]);
+                inv = factor_of(mean, far[0]);
+                if (!lifted(far[0])) found = far_of(mean);
             }
             float ss = 0.0f;
 #pragma unroll
@@ -128,17 +184,33 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
 #pragma unroll
                 for (int i = 0; i < kChunk; ++i) {
                     float u = x[j][i];
-                    if (post) u = u * inv * pw[j][i];
+                    if (post) u = u * raised * inv * pw[j][i];
                     if (gate) u *= a.g_ds ? g[j][i] : one;
                     v[j][i] = res[j][i] + a.scale * u;
                     // (Lanes past the row hold x = 0, but a gate or a norm of
                     // its own may be infinite.)
                     if (n < kChunk && i >= n) v[j][i] = 0.0f;
-                    ss = fmaf(v[j][i], v[j][i], ss);
                 }
                 store_f32<R, kChunk>(static_cast<typename R::T*>(a.r) + at.y + e, n, v[j]);
             }
-            inv = inv_rms(across.sum(ss), float(len), a.eps);
+            if (lifted(far[FAR - 1])) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int i = 0; i < kChunk; ++i) v[j][i] *= lift(far[FAR - 1]);
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) ss = fmaf(v[j][i], v[j][i], ss);
+            const float mean = mean_of(across.sum(ss), a.per, a.eps, far[FAR - 1]);
+            // (of a row whose x is to be lifted, the sum written above is not yet it)
+            far[0] |= found;
+            if (!lifted(found) && !lifted(far[FAR - 1])) {
+                found = far_of(mean);
+                far[FAR - 1] = found;
+            }
+            inv = factor_of(mean, far[FAR - 1]);
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -156,8 +228,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
                 for (int i = 0; i < kChunk; ++i) {
                     v[j][i] = x[j][i];
                     if (first) v[j][i] *= silu(g[j][i]);
-                    ss[j] = fmaf(v[j][i], v[j][i], ss[j]);
                 }
+                if (lifted(far[FAR == 1 ? 0 : j]))
+#pragma unroll
+                    for (int i = 0; i < kChunk; ++i) v[j][i] *= lift(far[FAR == 1 ? 0 : j]);
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) ss[j] = fmaf(v[j][i], v[j][i], ss[j]);
             }
             if (Q && a.parts > 1) {
                 // Groups of whole segments, the 512 elements that a wave's chunk holds:
@@ -177,7 +253,14 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
                     const int from = (j * WAVES + wave) / each * each;
                     float sum = 0.0f;
                     for (int i = from; i < min(from + each, NV * WAVES); ++i) sum += mine[i];
-                    inv[j] = inv_rms(sum, float(len / a.parts), a.eps);
+                    const float mean = mean_of(sum, a.per, a.eps, far[FAR == 1 ? 0 : j]);
+                    inv[j] = factor_of(mean, far[FAR == 1 ? 0 : j]);
+                    // (a wave's chunk past the row takes no part)
+                    if (!lifted(far[FAR == 1 ? 0 : j]) && kSegment * (j * WAVES + wave) < len) {
+                        const int f = far_of(mean);
+                        far[FAR == 1 ? 0 : j] = f;
+                        found |= f;
+                    }
                 }
                 // (across.most below lies between these reads and the next row's sums)
                 if constexpr (WAVES == 1) ssm::wave_sync();
@@ -185,7 +268,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
                 float all = 0.0f;
 #pragma unroll
                 for (int j = 0; j < NV; ++j) all += ss[j];
-                inv[0] = inv_rms(across.sum(all), float(len), a.eps);
+                const float mean = mean_of(across.sum(all), a.per, a.eps, far[0]);
+                inv[0] = factor_of(mean, far[0]);
+                if (!lifted(far[0])) found = far_of(mean);
+#pragma unroll
+                for (int j = 0; j < FAR; ++j) far[j] |= found;
 #pragma unroll
                 for (int j = 1; j < NV; ++j) inv[j] = inv[0];
             }
@@ -204,7 +291,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
                 for (int i = 0; i < kChunk; ++i) v[j][i] = x[j][i];
         }
         if constexpr (Q) {
-            uint32_t top = 0;
+            // (above any magnitude, where a wave finds a group that is to be lifted)
+            constexpr uint32_t kBeyond = 0x80000000u;
+            uint32_t top = lifted(found) ? kBeyond : 0u;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -214,7 +303,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
                     const uint32_t b = magnitude(v[j][i]);
                     top = b > top ? b : top;
                 }
-            const Quant qt(across.most(top));
+            top = across.most(top);
+            if (OP != kQuantize && __builtin_expect(__builtin_amdgcn_readfirstlane(int(top >= kBeyond)), 0)) {
+                again = true;
+                continue;
+            }
+            const Quant qt(top);
             if (tid == 0) a.qs[at.row] = qt.scale();
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
@@ -222,12 +316,17 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
                 if (e < a.q_ms) *reinterpret_cast<u32x2*>(a.q + at.row * a.q_ms + e) = eight(qt, v[j]);
             }
         } else {
+            again = lifted(found);
+            if (again) continue;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int e = kChunk * (tid + j * TPR);
                 store_f32<E, kChunk>(static_cast<typename E::T*>(a.y) + at.y + e, len - e, v[j]);
             }
         }
+        again = false;
+#pragma unroll
+        for (int j = 0; j < FAR; ++j) far[j] = kNear;
     }
 }
 
@@ -235,10 +334,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
 // groups within the unit (rows in 8 bits of a grouped norm), whose factors lie in LDS.
 constexpr int kLongThreads = 512;
 
+// (Three blocks a CU, which the lifted path would otherwise leave at two: 4096 rows of
+// 20480, residual to 8 bits, 276 us with two and 234 with three.)
 template <typename E, typename R, int OP, bool Q>
-__global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
+__global__ __launch_bounds__(kLongThreads, OP == kResidual && R::kBytes == 4 ? 5 : 6) void norm_long_kernel(NormArgs a) {
     __shared__ uint32_t slots[2 * (kLongThreads / 64)];
-    extern __shared__ float factor[];  // [parts]
+    extern __shared__ float factor[];  // [parts] where there are several, packed
     Across<kLongThreads> across{slots};
     const int tid = threadIdx.x;
     const int part = a.D / a.parts;
@@ -246,7 +347,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
     for (uint64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
         const Place at(a, uint32_t(unit));
         const float one = OP == kResidual && gate && !a.g_ds ? E::to_f32(static_cast<const typename E::T*>(a.g)[at.g]) : 1.0f;
-        float inv0 = 1.0f;            // of the norm of x, in the residual
+        Factor norm, whole;           // of x, in the residual, and of what is normed, undivided
         // n values from e on, as the norm takes them (past those 0).
         auto values = [&](int e, int n, float (&v)[kChunk]) {
             Raw<E> x, g, pw;
@@ -258,10 +359,15 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
                 if (post) pw.load(a.pw, e, n);
             }
 #pragma unroll
+            for (int i = 0; i < kChunk; ++i) v[i] = x[i];
+            if (OP == kResidual && lifted(norm.far))
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) v[i] *= lift(norm.far);
+#pragma unroll
             for (int i = 0; i < kChunk; ++i) {
-                float u = x[i];
+                float u = v[i];
                 if constexpr (OP == kResidual) {
-                    if (post) u = u * inv0 * pw[i];
+                    if (post) u = u * norm.inv * pw[i];
                     if (gate) u *= a.g_ds ? g[i] : one;
                     u = res[i] + a.scale * u;
                 } else if constexpr (OP == kGated) {
@@ -270,48 +376,53 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
                 v[i] = i < n ? u : 0.0f;
             }
         };
-        auto squares = [](const float (&v)[kChunk], float ss) {
+        // The factor of n values that f(e, v) gives by chunks, dealt to the
+        // threads of `over`, of which this is number `thread`: twice where they are
+        // to be lifted.
+        auto formed = [&](int n, int thread, auto& over, auto f) {
+            constexpr int kThreads = std::decay_t<decltype(over)>::WAVES * 64;
+            for (int far = kNear;;) {
+                float ss = 0.0f;
+                for (int e = kChunk * thread; e < n; e += kChunk * kThreads) {
+                    float v[kChunk];
+                    f(e, v);
+                    if (lifted(far))
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) ss = fmaf(v[i], v[i], ss);
-            return ss;
+                        for (int i = 0; i < kChunk; ++i) v[i] *= lift(far);
+#pragma unroll
+                    for (int i = 0; i < kChunk; ++i) ss = fmaf(v[i], v[i], ss);
+                }
+                const float mean = mean_of(over.sum(ss), a.per, a.eps, far);
+                const int found = lifted(far) ? kNear : far_of(mean);
+                if (found == kNear) return Factor{factor_of(mean, far), far};
+                far = found;
+            }
         };
         if constexpr (OP == kResidual) {
-            if (post) {
-                float ss = 0.0f;
-                for (int e = kChunk * tid; e < a.D; e += kChunk * kLongThreads) {
+            if (post)
+                norm = formed(a.D, tid, across, [&](int e, float (&v)[kChunk]) {
                     Raw<E> x;
                     x.load(a.x, at.x + e, a.D - e);
-                    float v[kChunk];
 #pragma unroll
                     for (int i = 0; i < kChunk; ++i) v[i] = x[i];
-                    ss = squares(v, ss);
-                }
-                inv0 = inv_rms(across.sum(ss), float(a.D), a.eps);
-            }
+                });
         }
         if constexpr (OP != kQuantize) {
-            float v[kChunk];
             if (a.parts == 1) {
-                float ss = 0.0f;
-                for (int e = kChunk * tid; e < a.D; e += kChunk * kLongThreads) {
+                whole = formed(a.D, tid, across, [&](int e, float (&v)[kChunk]) {
                     values(e, a.D - e, v);
                     if constexpr (OP == kResidual) store_f32<R, kChunk>(static_cast<typename R::T*>(a.r) + at.y + e, a.D - e, v);
-                    ss = squares(v, ss);
-                }
-                const float inv = inv_rms(across.sum(ss), float(a.D), a.eps);
-                if (tid == 0) factor[0] = inv;
+                });
             } else {
+                Across<64> wave{nullptr};
                 for (int p = tid >> 6; p < a.parts; p += kLongThreads / 64) {
-                    float ss = 0.0f;
-                    for (int e = kChunk * (tid & 63); e < part; e += kChunk * 64) {
+                    const Factor f = formed(part, tid & 63, wave, [&](int e, float (&v)[kChunk]) {
                         values(p * part + e, part - e, v);
-                        ss = squares(v, ss);
-                    }
-                    const float inv = inv_rms(Across<64>{nullptr}.sum(ss), float(part), a.eps);
-                    if ((tid & 63) == 0) factor[p] = inv;
+                    });
+                    if ((tid & 63) == 0) factor[p] = f.packed();
                 }
+                __syncthreads();
             }
-            __syncthreads();
         }
         auto results = [&](int e, float (&v)[kChunk]) {
             const int n = a.D - e;
@@ -320,14 +431,34 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
                 Raw<E> w, g;
                 if (scaled) w.load(a.w, at.w + e, n);
                 if (OP == kGated && gate && a.norm_first) g.load(a.g, at.g + e, n);
-                int p = a.parts == 1 ? 0 : e / part, left = a.parts == 1 ? a.D : (p + 1) * part - e;
+                if (a.parts == 1) {
+                    if (lifted(whole.far))
+#pragma unroll
+                        for (int i = 0; i < kChunk; ++i) v[i] *= lift(whole.far);
+#pragma unroll
+                    for (int i = 0; i < kChunk; ++i) v[i] *= whole.inv;
+                } else {
+                    const int p0 = e / part, left0 = (p0 + 1) * part - e;
+                    auto factors = [&](auto f) {
+                        int p = p0, left = left0;
+#pragma unroll
+                        for (int i = 0; i < kChunk; ++i) {
+                            if (i < n && left-- == 0) {
+                                ++p;
+                                left = part - 1;
+                            }
+                            f(v[i], factor[p]);
+                        }
+                    };
+                    uint32_t signs = 0;
+                    factors([&](float& u, float f) {
+                        u *= f;
+                        signs |= __float_as_uint(f);
+                    });
+                    if (__builtin_expect(__any(int(signs) < 0), 0)) factors([](float& u, float f) { u *= Factor::rest(f); });
+                }
 #pragma unroll
                 for (int i = 0; i < kChunk; ++i) {
-                    if (a.parts > 1 && i < n && left-- == 0) {
-                        ++p;
-                        left = part - 1;
-                    }
-                    v[i] *= factor[p];
                     if (scaled) v[i] *= w[i];
                     if (OP == kGated && gate && a.norm_first) v[i] *= silu(g[i]);
                 }

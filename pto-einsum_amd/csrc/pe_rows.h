@@ -133,6 +133,7 @@ struct NormArgs {
     int32_t parts;                    // groups within a unit (rows in 8 bits of a grouped norm)
     int32_t g_ds;                     // 0: one gate for a row
     int32_t norm_first;
+    float per;                        // one divided by a group's elements
     float eps, scale;
 };
 
