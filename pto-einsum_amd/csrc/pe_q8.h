@@ -49,9 +49,18 @@ __device__ __forceinline__ Column column(const Q8Args& g, int n) {
     return c;
 }
 
-// Column r of those in float32, from its sum and its row's scale.
+// Column r of those in float32, from its sum and its row's scale.  A sum, at most 2^31,
+// times a scale of 2^96 stays in float32, and times a small one, whichever it is, loses
+// no more than a rounding: above 2^-126 that is one, below it the product, a whole
+// number of the scale's last bits, is exact.  So a larger row's scale comes behind the
+// column's, and nothing but the result leaves the range.  (Rows with such scales are
+// rare: a branch of the wave for its rows, `value` for the others.)
 __device__ __forceinline__ float value(const Column& c, float sx, int r, int32_t sum) {
     return fmaf(float(sum) * sx, c.scale[r], c.bias[r]);
+}
+__device__ __forceinline__ bool large(float sx) { return fabsf(sx) > 0x1p96f; }
+__device__ __forceinline__ float value_of_large(const Column& c, float sx, int r, int32_t sum) {
+    return large(sx) ? fmaf(float(sum) * c.scale[r], sx, c.bias[r]) : value(c, sx, r, sum);
 }
 
 // These columns of row m of y from their sums.
@@ -59,7 +68,7 @@ template <typename E>
 __device__ __forceinline__ void finish(const Q8Args& g, const Column& c, float sx, int m, int n, i32x4 acc) {
     float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = value(c, sx, i, acc[i]);
+    for (int i = 0; i < 4; ++i) v[i] = value_of_large(c, sx, i, acc[i]);
     if (n < g.N) ssm::store_f32<E, 4>(static_cast<typename E::T*>(g.y) + int64_t(m) * g.N + n, g.N - n, v);
 }
 

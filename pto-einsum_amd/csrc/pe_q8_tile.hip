@@ -174,8 +174,10 @@ __global__ __launch_bounds__(256, MINB) void q8_tile_kernel(Q8Args g) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
 
+    // (The lane's number anew: the loop above has a register for nothing else.)
+    const int lane_out = int(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u))), row_out = lane_out & 15;
     // Lane l holds columns 4 (l / 16) .. + 3 of a block, row l % 16.
-    const int nl = n0 + wn * (BN / 2) + 4 * (lane >> 4);
+    const int nl = n0 + wn * (BN / 2) + 4 * (lane_out >> 4);
     // The sums lie four columns a lane, which would store 8 bytes of 16 rows at a time
     // (8192 x 8192 in 16 bits took 60 to 100 us that way, for 21 us of writing), so
     // each 16 rows of the wave's tile go through LDS of the wave's own and out in
@@ -187,36 +189,46 @@ __global__ __launch_bounds__(256, MINB) void q8_tile_kernel(Q8Args g) {
     Column c[FN];
 #pragma unroll
     for (int i = 0; i < FN; ++i) c[i] = column<E>(g, nl + 16 * i);
+    float sx[FM];
+    bool far = false;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-        const int m = m0 + wm * (BM / 2) + 16 * j;
-        int8_t* mine = lds + (2 * wave + (j & 1)) * 16 * PITCH;
-        const float sx = g.xs[min(m + fr, g.M - 1)];
+        sx[j] = g.xs[min(m0 + wm * (BM / 2) + 16 * j + row_out, g.M - 1)];
+        far = far || large(sx[j]);
+    }
+    auto out = [&](auto value_of) {
 #pragma unroll
-        for (int i = 0; i < FN; ++i) {
-            typename ssm::Vec<E, 4>::type v;
+        for (int j = 0; j < FM; ++j) {
+            const int m = m0 + wm * (BM / 2) + 16 * j;
+            int8_t* mine = lds + (2 * wave + (j & 1)) * 16 * PITCH;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (typename E::T)value(c[i], sx, r, acc[i][j][r]);
-            *reinterpret_cast<typename ssm::Vec<E, 4>::type*>(mine + fr * PITCH + (16 * i + 4 * (lane >> 4)) * E::kBytes) = v;
-        }
-        ssm::wave_sync();
+            for (int i = 0; i < FN; ++i) {
+                typename ssm::Vec<E, 4>::type v;
 #pragma unroll
-        for (int u = 0; u < 16 * VPR / 64; ++u) {
-            const int row = (u * 64 + lane) / VPR, at = (u * 64 + lane) % VPR;
-            const typename V::type v = *reinterpret_cast<const typename V::type*>(mine + row * PITCH + 16 * at);
-            const int n = n0 + wn * WN + at * (16 / E::kBytes);
-            if (m + row < g.M && n < g.N) {
-                typename E::T* y = static_cast<typename E::T*>(g.y) + int64_t(m + row) * g.N + n;
-                if (n + 16 / E::kBytes <= g.N) {
-                    *reinterpret_cast<typename V::utype*>(y) = v;
-                } else {
+                for (int r = 0; r < 4; ++r) v[r] = (typename E::T)value_of(c[i], sx[j], r, acc[i][j][r]);
+                *reinterpret_cast<typename ssm::Vec<E, 4>::type*>(mine + row_out * PITCH + (16 * i + 4 * (lane_out >> 4)) * E::kBytes) = v;
+            }
+            ssm::wave_sync();
 #pragma unroll
-                    for (int e = 0; e < 16 / E::kBytes; ++e)
-                        if (n + e < g.N) y[e] = v[e];
+            for (int u = 0; u < 16 * VPR / 64; ++u) {
+                const int row = (u * 64 + lane_out) / VPR, at = (u * 64 + lane_out) % VPR;
+                const typename V::type v = *reinterpret_cast<const typename V::type*>(mine + row * PITCH + 16 * at);
+                const int n = n0 + wn * WN + at * (16 / E::kBytes);
+                if (m + row < g.M && n < g.N) {
+                    typename E::T* y = static_cast<typename E::T*>(g.y) + int64_t(m + row) * g.N + n;
+                    if (n + 16 / E::kBytes <= g.N) {
+                        *reinterpret_cast<typename V::utype*>(y) = v;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16 / E::kBytes; ++e)
+                            if (n + e < g.N) y[e] = v[e];
+                    }
                 }
             }
         }
-    }
+    };
+    if (__builtin_expect(__any(far), 0)) out(value_of_large);
+    else out(value);
 }
 
 constexpr int64_t kMostTiles = (int64_t(1) << 24) - 1;   // blocks of 256 threads in fewer than 2^32
