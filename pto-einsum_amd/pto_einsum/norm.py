@@ -50,7 +50,8 @@ def places(lead, tensors):
     for p in range(len(lead) + 1):
         found = []
         for t in tensors:
-            if t is None:
+            if t is None or not t.numel():
+                # (of no elements nothing is addressed; torch calls them contiguous in any order)
                 found.append((0, 0))
                 continue
             axes = list(zip(lead, t.stride()))

@@ -73,8 +73,9 @@ MAX_K8 = 131071    # sums of 32 bits hold 128 * 128 * K
 
 
 def _apart(t: torch.Tensor):
-    """The one stride of t's rows, all axes but the last taken as one, or None."""
-    return _stride(list(zip(t.shape[:-1], t.stride())))
+    """The one stride of t's rows, all axes but the last taken as one, or None.  (Of no
+    elements, which torch calls contiguous in any order: 0.)"""
+    return 0 if not t.numel() else _stride(list(zip(t.shape[:-1], t.stride())))
 
 
 def _apart8(t: torch.Tensor) -> int:
