@@ -9,9 +9,22 @@ namespace {
 
 constexpr int64_t kMostK = 131071;
 
-// Whether the kernel for few rows takes x to 8 bits itself.
+// Whether the kernel for few rows is the one to take.
+//   Up to 64 rows of x, and more where one round of blocks of 64 x 64 holds the
+// product, whose waves share K: 256 x 4096 x 4096 11.3 us (tiles of the other
+// kernel 17.2), 512 x 2048 x 8192 17.1 (31.8); with two rounds 512 x 4096 x 4096
+// 21.0 (20.3) and 256 x 8192 x 2048 15.9 (12.1).
+//   Fewer channels than a launch of its blocks, 256 threads for 64 of them, has room for;
+// of the other kernel's tiles, 256 of them each, it has for all that there may be.
+bool few_rows(const pe_q8_desc* d) {
+    if (d->kernel) return d->kernel == 1;
+    if (ceil_div(d->N, 64) >= int64_t(1) << 24) return false;
+    return d->M <= 64 || ceil_div(d->M, 64) * ceil_div(d->N, 64) <= cu_count();
+}
+
+// Whether it takes x to 8 bits itself.
 bool own_rows(const pe_q8_desc* d) {
-    return d->x_dtype == d->y_dtype && d->kernel <= 1 && d->K > 0 && rows_take_own(d->M, d->K);
+    return d->x_dtype == d->y_dtype && d->K > 0 && rows_take_own(d->M, d->K) && few_rows(d);
 }
 
 // Bytes of the workspace: x's rows in 8 bits and their scales, where x comes in
@@ -91,11 +104,6 @@ extern "C" int pe_matmul_q8(const pe_q8_desc* d, const void* x, const float* x_s
     g.bias_f32 = d->bias_dtype == PE_F32;
     g.y = y;
     g.M = int32_t(d->M); g.N = int32_t(d->N); g.K = int32_t(d->K);
-    // Up to 64 rows of x, and more where one round of blocks of 64 x 64 holds the
-    // product, whose waves share K: 256 x 4096 x 4096 11.3 us (tiles of the other
-    // kernel 17.2), 512 x 2048 x 8192 17.1 (31.8); with two rounds 512 x 4096 x 4096
-    // 21.0 (20.3) and 256 x 8192 x 2048 15.9 (12.1).
-    const bool few = d->kernel ? d->kernel == 1 : d->M <= 64 || ceil_div(d->M, 64) * ceil_div(d->N, 64) <= cu_count();
     if (!whole) {
         if (own_rows(d)) return rows_launch_own(d->y_dtype, g, s);
         int8_t* q = static_cast<int8_t*>(ws) + space.rows;
@@ -111,5 +119,5 @@ extern "C" int pe_matmul_q8(const pe_q8_desc* d, const void* x, const float* x_s
         g.xs = qs;
         g.x_ms = r.q_ms;
     }
-    return few ? rows_launch(d->y_dtype, g, s) : tile_launch(d->y_dtype, g, d->kernel, s);
+    return few_rows(d) ? rows_launch(d->y_dtype, g, s) : tile_launch(d->y_dtype, g, d->kernel, s);
 }
