@@ -82,10 +82,17 @@ def number(what, name, v, kind=float):
     return float(v) if kind is float else operator.index(v)
 
 
+def _held(what, name, v):
+    """v, which float32 holds: neither as infinity nor, where it is not 0, as 0."""
+    if not abs(v) <= torch.finfo(torch.float32).max or 0.0 < abs(v) < 2.0 ** -149:
+        raise ValueError(f"{what}: {name} must be finite and in float32's range, got {v}")
+    return v
+
+
 def _eps(what, eps):
-    if not 0.0 <= eps <= torch.finfo(torch.float32).max:
+    if not eps >= 0.0:
         raise ValueError(f"{what}: eps must be finite and 0 or more, got {eps}")
-    return eps
+    return _held(what, "eps", eps)
 
 
 def fresh(shape, dtype):
@@ -209,7 +216,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor 
     x [..., D]; residual of x's shape and dtype, or float32; weight and
     post_weight [D] and gate of x's dtype; gate of any shape that broadcasts to
     x's (a gate for each channel, sequence, token or value).  Any strides but
-    along the last axis.  Returns (y, r): y of x's dtype, formed from r before r
+    along the last axis.  scale and eps are numbers, finite and in float32's
+    range.  Returns (y, r): y of x's dtype, formed from r before r
     is rounded to the residual's dtype, or with ``quantize`` ((q, scales), r) as
     ``quantize_q8`` gives them for the float32 y."""
     what = "residual_norm"
@@ -221,7 +229,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor 
         _operands(what, x, weight=weight, post_weight=post_weight)
         check(what, "residual", residual, x.shape, x.dtype if residual.dtype is x.dtype else torch.float32)
         D, lead = x.shape[-1], x.shape[:-1]
-        eps = _eps(what, eps)
+        eps, scale = _eps(what, eps), _held(what, "scale", scale)
         wide = gate
         if gate is not None:
             check(what, "gate", gate, gate.shape, x.dtype)
