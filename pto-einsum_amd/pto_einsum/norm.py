@@ -74,7 +74,7 @@ def _operands(what, x, **others):
 
 
 def number(what, name, v, kind=float):
-    """A number that a plan may be kept by; a tensor's value is not known here."""
+    """A number; a tensor's value is not known here."""
     if type(v) is kind:
         return v
     if isinstance(v, torch.Tensor):
@@ -93,6 +93,21 @@ def _eps(what, eps):
     if not eps >= 0.0:
         raise ValueError(f"{what}: eps must be finite and 0 or more, got {eps}")
     return _held(what, "eps", eps)
+
+
+# eps and scale may change from call to call, and calls on several threads have their
+# own: a plan keeps a descriptor for each of the last numbers, not one plan for each.
+MOST_NUMBERS = 64
+
+
+def numbered(what, base, made, eps, scale):
+    """A plan's descriptor with these numbers, kept with those already made."""
+    d = abi.RowsDesc.from_buffer_copy(base)
+    d.eps, d.scale = _eps(what, eps), _held(what, "scale", scale)
+    if len(made) >= MOST_NUMBERS:
+        made.clear()
+    made[eps, scale] = d
+    return d
 
 
 def fresh(shape, dtype):
@@ -170,7 +185,7 @@ def gated_norm(x: torch.Tensor, weight: torch.Tensor | None = None, z: torch.Ten
     the float32 y: (q, scales), one scale for a row of D (at most 8192 groups)."""
     what = "gated_norm"
     eps, groups = number(what, "eps", eps), number(what, "groups", groups, int)
-    key = (what, layout(x), layout(weight), layout(z), eps, groups, bool(norm_first), bool(quantize))
+    key = (what, layout(x), layout(weight), layout(z), groups, bool(norm_first), bool(quantize))
     plan = _plans.get(key)
     if plan is None:
         _operands(what, x, weight=weight)
@@ -180,7 +195,7 @@ def gated_norm(x: torch.Tensor, weight: torch.Tensor | None = None, z: torch.Ten
             raise ValueError(f"{what}: {D} elements are no {groups} equal groups")
         if quantize and groups > 8192:
             raise ValueError(f"{what}: at most 8192 groups with quantize, got {groups}")
-        eps = _eps(what, eps)
+        _eps(what, eps)
         ready(what, x, weight, z)
         given = (x, weight, z)
         laid = [inner(x), dense(weight), None if z is None else inner(z)]
@@ -192,9 +207,10 @@ def gated_norm(x: torch.Tensor, weight: torch.Tensor | None = None, z: torch.Ten
             return gated_norm(*laid, eps=eps, groups=groups, norm_first=norm_first, quantize=quantize)
         d = abi.RowsDesc(dtype=DTYPES[x.dtype], norm_first=bool(norm_first), rows0=rows0, rows1=rows1, D=D,
                          groups=groups, x_s0=pairs[0][0], x_s1=pairs[0][1], g_s0=pairs[1][0], g_s1=pairs[1][1],
-                         q_ms=row_pitch(D), x_numel=extent(x), g_numel=0 if z is None else extent(z), eps=eps)
-        plan = remember(key, (d, fresh8(x.shape) if quantize else fresh(x.shape, x.dtype)))
-    d, result = plan
+                         q_ms=row_pitch(D), x_numel=extent(x), g_numel=0 if z is None else extent(z))
+        plan = remember(key, (d, {}, fresh8(x.shape) if quantize else fresh(x.shape, x.dtype)))
+    base, made, result = plan
+    d = made.get((eps, 1.0)) or numbered(what, base, made, eps, 1.0)
     dev = ready(what, x, weight, z)
     with on(dev):
         y, scales = alloc8(result, x.device) if quantize else (alloc(result, x.device), None)
@@ -222,14 +238,13 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor 
     ``quantize_q8`` gives them for the float32 y."""
     what = "residual_norm"
     scale, eps = number(what, "scale", scale), number(what, "eps", eps)
-    key = (what, layout(x), layout(residual), layout(weight), layout(post_weight), layout(gate), scale, eps,
-           bool(quantize))
+    key = (what, layout(x), layout(residual), layout(weight), layout(post_weight), layout(gate), bool(quantize))
     plan = _plans.get(key)
     if plan is None:
         _operands(what, x, weight=weight, post_weight=post_weight)
         check(what, "residual", residual, x.shape, x.dtype if residual.dtype is x.dtype else torch.float32)
         D, lead = x.shape[-1], x.shape[:-1]
-        eps, scale = _eps(what, eps), _held(what, "scale", scale)
+        _eps(what, eps), _held(what, "scale", scale)
         wide = gate
         if gate is not None:
             check(what, "gate", gate, gate.shape, x.dtype)
@@ -253,11 +268,11 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor 
         d = abi.RowsDesc(dtype=DTYPES[x.dtype], res_dtype=DTYPES[residual.dtype],
                          gate_row=gate is not None and wide.shape[-1] == 1, rows0=rows0, rows1=rows1, D=D, groups=1,
                          x_s0=xs[0], x_s1=xs[1], g_s0=gs[0], g_s1=gs[1], r_s0=rs[0], r_s1=rs[1], q_ms=row_pitch(D),
-                         x_numel=extent(x), g_numel=0 if gate is None else extent(gate), r_numel=extent(residual),
-                         eps=eps, scale=scale)
-        plan = remember(key, (d, fresh8(x.shape) if quantize else fresh(x.shape, x.dtype),
+                         x_numel=extent(x), g_numel=0 if gate is None else extent(gate), r_numel=extent(residual))
+        plan = remember(key, (d, {}, fresh8(x.shape) if quantize else fresh(x.shape, x.dtype),
                               fresh(x.shape, residual.dtype)))
-    d, result, total = plan
+    base, made, result, total = plan
+    d = made.get((eps, scale)) or numbered(what, base, made, eps, scale)
     dev = ready(what, x, residual, weight, post_weight, gate)
     with on(dev):
         y, scales = alloc8(result, x.device) if quantize else (alloc(result, x.device), None)
