@@ -46,7 +46,8 @@ int arguments(const char* what, const pe_rows_desc* d, const void* x, bool gate,
     a.inner = FastDiv(uint32_t(d->rows1));
     a.groups = FastDiv(uint32_t(apart));
     a.D = int32_t(d->D / apart);
-    a.parts = int32_t(q8 ? d->groups : 1);
+    // (of rows without elements there is nothing to share out)
+    a.parts = int32_t(q8 && d->D ? d->groups : 1);
     a.per = 1.0f / float(d->D / d->groups);
     a.g_ds = d->gate_row ? 0 : 1;
     a.norm_first = d->norm_first;
