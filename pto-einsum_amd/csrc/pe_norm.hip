@@ -20,7 +20,9 @@ int arguments(const char* what, const pe_rows_desc* d, const void* x, bool gate,
     if (!(d->eps >= 0.0f)) return fail(PE_ERR_INVALID, name + ": eps must be 0 or more");
     const int64_t big = (int64_t(1) << 31) - 32768;
     if (d->D > big) return fail(PE_ERR_UNSUPPORTED, name + ": rows of 2^31 elements or more");
-    if (__int128(d->rows0) * d->rows1 * d->groups > big) return fail(PE_ERR_UNSUPPORTED, name + ": 2^31 rows or more");
+    // (in two steps: the three extents' product may pass 128 bits)
+    const __int128 rows = __int128(d->rows0) * d->rows1;
+    if (d->rows0 && d->rows1 && (rows > big || rows * d->groups > big)) return fail(PE_ERR_UNSUPPORTED, name + ": 2^31 rows or more");
     if (!ssm::within({{d->rows0, d->x_s0}, {d->rows1, d->x_s1}, {d->D, 1}}, d->x_numel))
         return fail(PE_ERR_BOUNDS, name + ": strides address past x");
     if (gate && !ssm::within({{d->rows0, d->g_s0}, {d->rows1, d->g_s1}, {d->gate_row ? (d->D > 0) : d->D, 1}}, d->g_numel))
