@@ -25,7 +25,7 @@ int arguments(const char* what, const pe_rows_desc* d, const void* x, bool gate,
     if (d->rows0 && d->rows1 && (rows > big || rows * d->groups > big)) return fail(PE_ERR_UNSUPPORTED, name + ": 2^31 rows or more");
     if (!ssm::within({{d->rows0, d->x_s0}, {d->rows1, d->x_s1}, {d->D, 1}}, d->x_numel))
         return fail(PE_ERR_BOUNDS, name + ": strides address past x");
-    if (gate && !ssm::within({{d->rows0, d->g_s0}, {d->rows1, d->g_s1}, {d->gate_row ? (d->D > 0) : d->D, 1}}, d->g_numel))
+    if (gate && !ssm::within({{d->rows0, d->g_s0}, {d->rows1, d->g_s1}, {d->gate_row ? 1 : d->D, 1}}, d->g_numel))
         return fail(PE_ERR_BOUNDS, name + ": strides address past the gate");
     if (residual) {
         if (d->res_dtype != d->dtype && d->res_dtype != PE_F32)

@@ -23,3 +23,10 @@ def test_products_of_extents_past_128_bits(kw):
 
 def test_no_rows_of_any_number_of_groups():
     assert abi.bind().pe_gated_norm(ctypes.byref(desc(rows0=0, groups=1 << 62)), None, None, None, 64, None, None, None) == 0
+
+
+def test_gates_of_rows_without_elements():
+    """A gate for each row is read although the row has no elements."""
+    d = desc(gate_row=1, g_s0=3, g_s1=1, g_numel=5)
+    args = (None, None, None, None, 64, None, None, 64, 64, None)
+    assert abi.bind().pe_residual_norm(ctypes.byref(d), *args) == BOUNDS
