@@ -27,15 +27,14 @@ bool own_rows(const pe_q8_desc* d) {
     return d->x_dtype == d->y_dtype && d->K > 0 && rows_take_own(d->M, d->K) && few_rows(d);
 }
 
-// Bytes of the workspace: x's rows in 8 bits and their scales, where x comes in
-// another type.
+// The workspace: x's rows in 8 bits and, from `scales` on, their scales, where x comes
+// in another type.
 struct Space {
-    int64_t rows = 0, scales = 0, bytes = 0;
+    int64_t scales = 0, bytes = 0;
 };
 Space space_of(const pe_q8_desc* d) {
     Space s;
     if (d->x_dtype != PE_I8 && !own_rows(d)) {
-        s.rows = 0;
         s.scales = ceil_div(d->M * rows::row_pitch(d->K), 256) * 256;
         s.bytes = s.scales + ceil_div(4 * d->M, 256) * 256;
     }
@@ -106,7 +105,7 @@ extern "C" int pe_matmul_q8(const pe_q8_desc* d, const void* x, const float* x_s
     g.M = int32_t(d->M); g.N = int32_t(d->N); g.K = int32_t(d->K);
     if (!whole) {
         if (own_rows(d)) return rows_launch_own(d->y_dtype, g, s);
-        int8_t* q = static_cast<int8_t*>(ws) + space.rows;
+        int8_t* q = static_cast<int8_t*>(ws);
         float* qs = reinterpret_cast<float*>(static_cast<char*>(ws) + space.scales);
         pe_rows_desc r{};
         r.dtype = d->x_dtype;
