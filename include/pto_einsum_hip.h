@@ -309,7 +309,9 @@ int pe_matvec_q4(const pe_q4_desc* d, const void* x, const void* packed, const v
  * No counterpart in the reference.  Rows of D contiguous elements lie at
  * rows0 x rows1 places (a tensor's leading axes, collapsed to two; strides in
  * elements, 0 where a gate or residual is shared by them).  Sums, norms and
- * gates are float32; each output is rounded once.  Outputs are contiguous,
+ * gates are float32; each output is rounded once.  Rows whose sums of squares
+ * float32 does not hold are formed with values times a power of two; a gate's
+ * product and a residual sum are float32 values.  Outputs are contiguous,
  * [rows][D], and overlap no operand.
  *
  * A row in 8 bits: a = max |v|, scale = a / 127 (float32), q = the whole number

@@ -13,7 +13,7 @@
 // barrier, and short rows share a block.  Rows too long for the registers, and
 // rows in 8 bits of a grouped norm (whose scale spans the groups) unless its groups are
 // whole 512 elements, go to a kernel that reads the row again for each step: from the
-// caches, mostly (4096 rows of 4096, 8 groups: 25 us here, 51 there).
+// caches, mostly (4096 rows of 4096: 8 groups 22 us here, 16 groups 60 there).
 #pragma once
 
 #include "pe_rows.h"
@@ -139,7 +139,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
         const Place at(a, uint32_t(unit));
         // (The length as the compiler cannot see through: the masks of a row's end,
         // one for each element, are the same for every row, and taken out of the loop
-        // they filled the scalar registers and went through lanes of vector ones.)
+        // they filled the scalar registers and went through lanes of vector ones.  The
+        // residual's kernels of four chunks still put 42 or 52 there.)
         int len = a.D;
         asm volatile("" : "+s"(len));
         Raw<E> x[NV], g[NV], w[NV], pw[NV];

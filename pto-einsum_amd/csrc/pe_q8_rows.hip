@@ -207,6 +207,9 @@ int pick(const Q8Args& g, hipStream_t stream) {
 
 }  // namespace
 
+// Against a launch of their own: 1 x 4096 x 4096 6.7 us against 8.2, 8 rows 8.8 against
+// 8.8; but every block takes them again, and with N = 32768 one row takes 32.8 against
+// 31.2, with 131072 110 against 98 (8 rows 100 and 100).
 bool rows_take_own(int64_t m, int64_t k) {
     const int64_t steps = ceil_div(k, kStep);
     return m <= 16 && m * steps * kStep <= kOwnBytes / 4 * std::min<int64_t>(4, steps);

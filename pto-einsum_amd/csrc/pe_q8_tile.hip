@@ -3,12 +3,13 @@
 // Four waves (2 x 2) share a tile.  K walks in slabs of 64 bytes through a ring of LDS
 // stages that direct loads fill; while a slab is multiplied, the next one's fragments
 // are read into a second set of registers and the one STAGES - 1 ahead is loaded, one
-// read or load at a time between the products, so that the matrix cores wait for
-// neither.  The products' rate bounds large ones (8192^3: matrix cores 57 % busy at 1.8
-// GHz, 2.4 POPS where the library's int8 product reaches 2.1); a wave's tile of 128 x
-// 128 reads 16 KB of LDS for 64 products of 16 cycles, half of what LDS delivers, one of
-// 64 x 64 all of it.  A tile's start and end (12 us of a 256 x 256 one, half of it the
-// stores of all CUs at once) bounds products of short K.
+// read or load at a time between the products.  Of 8192^3 the matrix cores are 58 % busy
+// at about 1.8 GHz, 2.4 POPS (the library's int8 product 2.1); a 256 x 256 tile leaves
+// one wave a SIMD, with a barrier for each slab, and which wait takes the rest has not
+// been measured.  A wave's tile of 128 x 128 reads 16 KB of LDS for 64 products of 16
+// cycles, half of what LDS delivers, one of 64 x 64 all of it.  A tile's start and end
+// (12 us of a 256 x 256 one, half of it the stores of all CUs at once) bounds products
+// of short K.
 #include "pe_q8.h"
 
 #include <algorithm>
