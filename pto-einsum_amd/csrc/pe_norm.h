@@ -130,7 +130,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a)
     const int tid = threadIdx.x % TPR;
     const bool gate = a.g != nullptr, post = a.pw != nullptr, scaled = a.w != nullptr;
     // What the row's values are lifted by: for a residual x's and then the sum's, for
-    // groups within a row each chunk's; and whether this is the second time.
+    // groups within a row each chunk's; and whether it is taken once more.
     constexpr int FAR = OP == kResidual ? 2 : OP == kGated && Q ? NV : 1;
     int far[FAR] = {};
     bool again = false;
